@@ -340,6 +340,49 @@ def _check_pages(pages, pool_pages: int):
             raise ValueError(f"page id {p} outside the pool of {pool_pages} pages")
 
 
+def kv_pages_copy(k_pool: torch.Tensor, v_pool: torch.Tensor, src, dst, tokens=None):
+    """Copy pages inside the pools [layers, pages, hkv, ps, D]: page src[i] -> page dst[i] in every layer of K
+    and V, the first tokens[i] tokens of each (default: all; the rest of the destination stays). One launch.
+    Lists are checked here; int32 device tensors (graph capture, no host work) are checked on the device: an id
+    outside the pool is skipped and recorded, a negative one leaves the pair out. No destination may
+    be a source or another pair's destination (recorded as an error, the pages' contents are then undefined)."""
+    if not isinstance(src, torch.Tensor):
+        src, dst = [int(p) for p in src], [int(p) for p in dst]
+        if len(src) != len(dst) or (tokens is not None and len(tokens) != len(src)):
+            raise ValueError(f"{len(src)} source pages, {len(dst)} destinations")
+        _check_pages(src + dst, k_pool.shape[1])
+        if len(set(dst)) != len(dst) or set(dst) & set(src):
+            raise ValueError("a destination page is also a source or another pair's destination")
+        if tokens is not None and any(not 0 <= int(t) <= k_pool.shape[3] for t in tokens):
+            raise ValueError(f"token counts outside a page of {k_pool.shape[3]}")
+        if not src:
+            return
+        n = len(src)
+        idx = torch.tensor(src + dst + [int(t) for t in tokens or ()], dtype=torch.int32)
+        idx = idx.pin_memory().to(k_pool.device, non_blocking=True)
+        src, dst, tokens = idx[:n], idx[n:2 * n], idx[2 * n:] if tokens is not None else None
+    ext().kv_pages_move(k_pool, v_pool, src, dst, tokens, scratch(k_pool.device).err)
+    _count()
+
+
+def kv_pages_compact(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Tensor, counts: torch.Tensor,
+                     reserved: int = 1, out_tables: Optional[torch.Tensor] = None):
+    """Move the live pages of the pools [layers, pages, hkv, ps, D] to the front and rewrite the block tables.
+    Live are the first ``reserved`` pages (they stay) and the first counts[r] entries of each row r of
+    ``block_tables`` [rows, width] int32, which may name a page together. With n live pages, those from n up
+    move, in order, into the holes below n, so the fewest pages move. Returns (tables, remap, live): the tables
+    with new ids (entries past a row's count unchanged; in ``out_tables`` if given, which may be ``block_tables``),
+    the new id of every page ([pages] int32, -1: free) and n ([1] int32). Nothing is read back by the host."""
+    pages = k_pool.shape[1]
+    if out_tables is None:
+        out_tables = torch.empty_like(block_tables)
+    ws = torch.empty(3 * pages + 2, dtype=torch.int32, device=k_pool.device)
+    s = scratch(k_pool.device)
+    ext().kv_pages_compact(k_pool, v_pool, block_tables, counts, out_tables, ws, reserved, s.num_sms, s.err)
+    _count(2)
+    return out_tables, ws[:pages], ws[pages:pages + 1]
+
+
 def argmax_partial(logits: torch.Tensor, vocab_offset: int, out: torch.Tensor):
     ext().argmax_partial(logits, vocab_offset, out)
     _count()
@@ -369,3 +412,7 @@ def rope_tables(head_dim: int, base: float, max_pos: int, device) -> tuple:
     inv = 1.0 / (torch.tensor(base, dtype=torch.float64) ** (torch.arange(half, dtype=torch.float64) * 2.0 / head_dim))
     t = torch.arange(max_pos, dtype=torch.float64)[:, None] * inv[None, :]
     return torch.cos(t).float().to(device), torch.sin(t).float().to(device)
+
+
+from .shared_prefix import PrefixGroups, attn_shared_prefix  # noqa: E402,F401
+from .speculative import verify_drafts  # noqa: E402,F401

@@ -1,0 +1,140 @@
+"""Decode attention for batches in which groups of sequences share a long prefix.
+
+Sequences forked from one another (or behind one system prompt) name the same pages for their first
+keys. ``PrefixGroups`` holds which sequences share how many keys; ``attn_shared_prefix`` reads each
+group's shared pages once for all of its sequences instead of once per sequence.
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+
+_HDR = 8      # header ints of the device table, [0] = number of prefix items
+_ITEM = 8     # ints per prefix item
+_TILE = 64    # query rows per prefix item
+_KEYS = 64    # key ranges of prefix items are multiples of this
+
+
+class PrefixGroups:
+    """Which sequences of a decode batch share a prefix, and the attention's work list and workspace.
+
+    ``batch`` sequences (slots) bring ``q_len`` new tokens each; ``hq`` / ``hkv`` query and KV heads of
+    ``head_dim``. Nothing is shared until ``set``. A call that is being captured into a CUDA graph uses the
+    largest launch this object can need, so replays follow later ``set`` calls, block tables and lengths.
+    All memory is allocated here: use one object per stream (two calls on two streams, or two graphs that may
+    replay at the same time, need one each)."""
+
+    def __init__(self, batch: int, hq: int, hkv: int, head_dim: int, q_len: int = 1, device=None):
+        if batch < 1 or q_len < 1:
+            raise ValueError("PrefixGroups needs at least one sequence and one new token each")
+        if hkv < 1 or hq % hkv or head_dim not in (64, 128):
+            raise ValueError(f"{hq} query heads over {hkv} KV heads of {head_dim}: need hq % hkv == 0 and head_dim 64 or 128")
+        self.group = hq // hkv
+        if q_len * self.group > _TILE:
+            raise ValueError(f"{q_len} new tokens x {self.group} heads per KV head exceed {_TILE} query rows")
+        self.batch, self.hq, self.hkv, self.head_dim, self.q_len = batch, hq, hkv, head_dim, q_len
+        self.device = torch.device(device if device is not None else "cuda")
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        sms = torch.cuda.get_device_properties(self.device).multi_processor_count if self.device.type == "cuda" else 148
+        self._target = 2 * sms
+        # own items of a sequence split over its keys only while (sequence, KV head) pairs leave SMs idle
+        self.own_cap = max(1, min(32, (3 * sms + batch * hkv) // (2 * batch * hkv))) if 4 * batch * hkv < 3 * sms else 1
+        rows = batch * q_len
+        self.item_cap = self._target + hkv * (-(-rows * self.group // _TILE) + batch)
+        slots = _TILE * self._target + rows * hq * (1 + self.own_cap)
+        self._po = torch.empty(slots * head_dim, dtype=torch.float32, device=self.device)
+        self._pml = torch.empty(slots * 2, dtype=torch.float32, device=self.device)
+        self._meta = torch.zeros(_HDR + 5 * batch + _ITEM * self.item_cap, dtype=torch.int32, device=self.device)
+        self.slot_cap = slots
+        self.n_items = 0
+        self.set([])
+
+    def set(self, groups: Sequence[Tuple[Sequence[int], int]]) -> "PrefixGroups":
+        """``groups``: (sequences, shared keys) pairs. The first ``shared`` keys of every sequence of a group
+        must be the same tokens; they are read through the block table of the group's first sequence. A
+        sequence may be in one group at most; one in none attends its own pages alone."""
+        B, T, G = self.batch, self.q_len, self.group
+        seen = set()
+        for seqs, shared in groups:
+            if shared < 0:
+                raise ValueError(f"a shared prefix of {shared} keys")
+            for b in seqs:
+                if not 0 <= int(b) < B:
+                    raise ValueError(f"sequence {b} outside a batch of {B}")
+                if int(b) in seen:
+                    raise ValueError(f"sequence {b} is in two prefix groups")
+                seen.add(int(b))
+        groups = [([int(b) for b in seqs], int(n)) for seqs, n in groups if len(seqs) and n > 0]
+        meta = np.zeros(self._meta.shape[0], dtype=np.int32)
+        prefix, base, slots, pslots = (meta[_HDR + i * B:_HDR + (i + 1) * B] for i in range(4))
+        member = meta[_HDR + 4 * B:_HDR + 5 * B]
+        tiles = [-(-len(seqs) * T * G // _TILE) for seqs, _ in groups]
+        # every item takes about the same number of keys, so that all SMs finish together
+        load = sum(t * self.hkv * n for t, (_, n) in zip(tiles, groups))
+        per = max(_KEYS, -(-(-(-load // self._target)) // _KEYS) * _KEYS)
+        items, off = [], 0
+        for t, (seqs, n) in zip(tiles, groups):
+            splits = -(-n // per)
+            size = -(-(-(-n // splits)) // _KEYS) * _KEYS
+            splits = -(-n // size)
+            member[off:off + len(seqs)] = seqs
+            prefix[seqs], pslots[seqs] = n, splits
+            rows = len(seqs) * T * G
+            h, i, s = np.meshgrid(np.arange(self.hkv), np.arange(t), np.arange(splits), indexing="ij")
+            one = np.zeros((h.size, _ITEM), dtype=np.int32)
+            one[:, 0], one[:, 1] = seqs[0], off
+            one[:, 2] = i.reshape(-1) * _TILE
+            one[:, 3] = np.minimum(_TILE, rows - one[:, 2])
+            one[:, 4], one[:, 5] = h.reshape(-1), s.reshape(-1) * size
+            one[:, 6], one[:, 7] = np.minimum(n, one[:, 5] + size), s.reshape(-1)
+            items.append(one)
+            off += len(seqs)
+        slots[:] = pslots + self.own_cap
+        per_seq = slots.astype(np.int64) * (T * self.hq)
+        base[:] = np.concatenate([[0], np.cumsum(per_seq)[:-1]])
+        n_items = sum(len(x) for x in items)
+        assert n_items <= self.item_cap and int(per_seq.sum()) <= self.slot_cap, "prefix work list exceeds its workspace"
+        if items:
+            meta[_HDR + 5 * B:_HDR + 5 * B + _ITEM * n_items] = np.concatenate(items).reshape(-1)
+        meta[0] = n_items
+        host = torch.from_numpy(meta)
+        if self.device.type == "cuda":
+            with torch.cuda.device(self.device):
+                self._meta.copy_(host.pin_memory(), non_blocking=True)
+        else:
+            self._meta.copy_(host)
+        self.n_items = n_items
+        self.min_prefix = min((n for _, n in groups), default=0) if len(seen) == B else 0
+        return self
+
+
+def attn_shared_prefix(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_tables: torch.Tensor,
+                       seq_lens: torch.Tensor, groups: PrefixGroups, out: torch.Tensor, scale: float, window: int = 0,
+                       max_len_hint: int = 0) -> torch.Tensor:
+    """Causal paged GQA attention of the ``q_len`` newest tokens of every sequence, the shared prefixes of
+    ``groups`` read once per group. q, out [B * q_len, hq * D] bf16 (the tokens of a sequence together);
+    kcache, vcache [pages, hkv, page, D] bf16 (pages of a multiple of 16 tokens); block_tables [B, pages] and
+    seq_lens [B] int32 as in ``attn_decode``, lengths including the new tokens. A token without any key gives
+    zeros. ``window``: attend the last ``window`` keys only. ``max_len_hint``: longest sequence (default: what
+    the tables can hold)."""
+    from . import _count, ext, scratch
+    B, T = groups.batch, groups.q_len
+    if seq_lens.shape[0] != B or q.shape[0] != B * T or q.shape[1] != groups.hq * groups.head_dim:
+        raise ValueError(f"q {tuple(q.shape)} and {seq_lens.shape[0]} lengths do not fit groups of {B} sequences x {T} "
+                         f"tokens x {groups.hq} heads of {groups.head_dim}")
+    if kcache.shape[1] != groups.hkv or kcache.shape[3] != groups.head_dim:
+        raise ValueError(f"cache {tuple(kcache.shape)} does not fit groups of {groups.hkv} KV heads of {groups.head_dim}")
+    if groups.device != q.device:
+        raise ValueError(f"groups on {groups.device}, q on {q.device}")
+    own = max(1, (max_len_hint or block_tables.shape[1] * kcache.shape[2]) - groups.min_prefix)
+    splits = min(groups.own_cap, max(1, own // 128))
+    capturing = torch.cuda.is_current_stream_capturing()
+    if capturing:
+        splits = groups.own_cap
+    ext().attn_shared(q, kcache, vcache, block_tables, seq_lens, groups._meta, groups._po, groups._pml, out,
+                      scratch(q.device).err, groups.item_cap if capturing else groups.n_items, splits, scale, window)
+    _count(2)
+    return out

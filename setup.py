@@ -28,6 +28,10 @@ ext_modules = [
             "csrc/kernels/gemm_2sm.cu",
             "csrc/kernels/sampling.cu",
             "csrc/kernels/allreduce.cu",
+            "csrc/sharing_ops.cpp",
+            "csrc/kernels/kv_moves.cu",
+            "csrc/kernels/attn_shared.cu",
+            "csrc/kernels/verify.cu",
         ],
         include_dirs=[os.path.join(ROOT, "csrc", "include")],
         extra_compile_args={"cxx": CXX, "nvcc": NVCC},
