@@ -47,7 +47,7 @@ struct VerifyArgs {
   int B, K, V, chunks;
   bool logits_bf16, probs_bf16;
 };
-int verify_chunks(int64_t V);
+int verify_chunks(int64_t B, int64_t K, int64_t V);
 int64_t verify_max_vocab();
 int64_t verify_parts_bytes(int64_t B, int64_t K, int64_t V);
 cudaError_t launch_verify(const VerifyArgs& a, cudaStream_t st);

@@ -8,43 +8,57 @@
 
 namespace mesh {
 
+// n 16-byte vectors, at(v) = their place in both pages. Eight loads per thread are in flight before the first store
+// (source and destination lie in one pool, so the compiler would keep each load behind the store before it), and
+// both stream past the caches: nothing is read twice.
+template <typename At>
+__device__ __forceinline__ void copy_vectors(uint4* dp, const uint4* sp, int n, At at) {
+  constexpr int U = 8;
+  for (int v0 = threadIdx.x; v0 < n; v0 += U * blockDim.x) {
+    uint4 r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v0 + u * blockDim.x < n) r[u] = __ldcs(sp + at(v0 + u * blockDim.x));
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v0 + u * blockDim.x < n) __stcs(dp + at(v0 + u * blockDim.x), r[u]);
+  }
+}
+
 // Copies inside one pool (a fork's last page, a branch that will rewrite a page): the first tokens[i]
 // tokens of page src[i] go to page dst[i] in every layer of K and V. A page of one layer is
 // [kv_heads, page_size, D], so the first t tokens are kv_heads runs of t * D elements.
-// grid (pairs, layers, 2): one CTA copies one pair in one layer of K or V, 16 bytes per thread step.
-// Bound by memory: every byte is read once and written once. Ids outside the pool are recorded as an
+// grid (pairs, layers, 2): one CTA copies one pair in one layer of K or V. Ids outside the pool are recorded as an
 // error and skipped; a negative id leaves the pair out (padding of a fixed-size list).
-__global__ void __launch_bounds__(256) kv_pages_move_kernel(uint4* __restrict__ k_pool, uint4* __restrict__ v_pool,
-                                                            const int* __restrict__ src, const int* __restrict__ dst,
-                                                            const int* __restrict__ tokens, int n, long pool_pages,
-                                                            int heads, int page_size, int row_vec, int* err) {
+__global__ void __launch_bounds__(256) kv_pages_move_kernel(const KvMoveArgs a) {
+  griddep_wait();
+  griddep_launch_dependents();
   const int i = blockIdx.x, layer = blockIdx.y;
-  const int s = src[i], d = dst[i];
-  if (layer == 0 && blockIdx.z == 0) {
+  const int s = a.src[i], d = a.dst[i];
+  if (layer == 0 && blockIdx.z == 0 && s >= 0 && d >= 0) {
     // a destination that is also a source or another pair's destination has no defined result
-    for (int j = threadIdx.x; j < n; j += blockDim.x)
-      if (d >= 0 && s >= 0 && ((dst[j] == d && j != i && src[j] >= 0) || (src[j] == d && dst[j] >= 0)))
-        record_error(err, ERR_BAD_ARGUMENT);
-  }
-  if (s < 0 || d < 0) return;
-  if (s >= pool_pages || d >= pool_pages) {
-    if (threadIdx.x == 0) record_error(err, ERR_BAD_ARGUMENT);
-    return;
-  }
-  const int t = tokens ? max(0, min(tokens[i], page_size)) : page_size;
-  uint4* pool = blockIdx.z == 0 ? k_pool : v_pool;
-  const long page_vec = (long)heads * page_size * row_vec;
-  const uint4* sp = pool + ((long)layer * pool_pages + s) * page_vec;
-  uint4* dp = pool + ((long)layer * pool_pages + d) * page_vec;
-  const int run = t * row_vec, head_vec = page_size * row_vec;
-  if (t == page_size) {
-    for (long v = threadIdx.x; v < page_vec; v += blockDim.x) dp[v] = sp[v];
-  } else {
-    for (int v = threadIdx.x; v < heads * run; v += blockDim.x) {
-      const int h = v / run, o = h * head_vec + (v - h * run);
-      dp[o] = sp[o];
+    for (int j = threadIdx.x; j < a.n; j += blockDim.x) {
+      const int sj = a.src[j], dj = a.dst[j];
+      if (sj >= 0 && dj >= 0 && ((dj == d && j != i) || sj == d)) record_error(a.err, ERR_BAD_ARGUMENT);
     }
   }
+  if (s < 0 || d < 0) return;
+  if (s >= a.pool_pages || d >= a.pool_pages) {
+    if (threadIdx.x == 0) record_error(a.err, ERR_BAD_ARGUMENT);
+    return;
+  }
+  const int t = a.tokens ? max(0, min(a.tokens[i], a.page_size)) : a.page_size;
+  uint4* pool = static_cast<uint4*>(blockIdx.z == 0 ? a.k : a.v);
+  const int head_vec = a.page_size * a.row_vec, page_vec = a.heads * head_vec, run = t * a.row_vec;
+  const uint4* sp = pool + ((long)layer * a.pool_pages + s) * page_vec;
+  uint4* dp = pool + ((long)layer * a.pool_pages + d) * page_vec;
+  if (t == a.page_size)
+    copy_vectors(dp, sp, page_vec, [](int v) { return v; });
+  else
+    copy_vectors(dp, sp, a.heads * run, [=](int v) {
+      const int h = v / run;
+      return h * head_vec + (v - h * run);
+    });
 }
 
 // Compaction, step 1 (one CTA): which pages are live (reserved, or named by a used block-table entry), how
@@ -64,20 +78,23 @@ __global__ void __launch_bounds__(1024) kv_compact_plan_kernel(const int* __rest
   uint32_t* bits = sm;
   int* before = reinterpret_cast<int*>(sm + words);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  griddep_wait();
+  griddep_launch_dependents();
   for (int w = tid; w < words; w += blockDim.x) {
     const int lo = w * 32;
     bits[w] = reserved >= lo + 32 ? 0xffffffffu : reserved > lo ? (1u << (reserved - lo)) - 1u : 0u;
   }
   __syncthreads();
-  const long n = (long)rows * width;
-  for (long e = tid; e < n; e += blockDim.x) {
-    const int r = (int)(e / width), c = (int)(e - (long)r * width);
-    if (c >= counts[r]) continue;
-    const int p = tables[e];
-    if (p < 0 || p >= pages)
-      record_error(err, ERR_BAD_ARGUMENT);
-    else
-      atomicOr(&bits[p >> 5], 1u << (p & 31));
+  for (int r = warp; r < rows; r += 32) {
+    const int c1 = min(counts[r], width);
+    const int* row = tables + (long)r * width;
+    for (int c = lane; c < c1; c += 32) {
+      const int p = row[c];
+      if (p < 0 || p >= pages)
+        record_error(err, ERR_BAD_ARGUMENT);
+      else
+        atomicOr(&bits[p >> 5], 1u << (p & 31));
+    }
   }
   __syncthreads();
   // exclusive prefix of the words' live counts: a contiguous run of words per thread
@@ -130,36 +147,30 @@ __global__ void __launch_bounds__(1024) kv_compact_plan_kernel(const int* __rest
 // Compaction, step 2: rewrite the used table entries and copy the moved pages in every layer of K and V.
 // The number of moves is known on the device only, so a fixed grid walks the (move, layer, K or V) blocks.
 // Sources lie at or above the live count and destinations below it, so no block is read after it is written.
-__global__ void __launch_bounds__(256) kv_compact_move_kernel(uint4* __restrict__ k_pool, uint4* __restrict__ v_pool,
-                                                              const int* tables, int* out_tables,
-                                                              const int* __restrict__ counts, int rows, int width,
-                                                              int layers, long pool_pages, long page_vec,
-                                                              const int* __restrict__ remap, const int* __restrict__ src,
-                                                              const int* __restrict__ dst,
-                                                              const int* __restrict__ n_moves) {
-  const long n = (long)rows * width;
-  for (long e = (long)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += (long)gridDim.x * blockDim.x) {
-    const int r = (int)(e / width), c = (int)(e - (long)r * width);
-    const int p = tables[e];
-    out_tables[e] = (c < counts[r] && p >= 0 && p < pool_pages) ? remap[p] : p;
+__global__ void __launch_bounds__(256) kv_compact_move_kernel(const KvCompactArgs a) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int pages = (int)a.pool_pages;
+  const int *remap = a.ws, *src = a.ws + pages + 2, *dst = src + pages;
+  const int moves = a.ws[pages + 1];
+  const int warp = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+  for (int r = warp; r < a.rows; r += (gridDim.x * blockDim.x) >> 5) {
+    const int used = a.counts[r];
+    for (int c = lane; c < a.width; c += 32) {
+      const int p = a.tables[(long)r * a.width + c];
+      a.out_tables[(long)r * a.width + c] = (c < used && p >= 0 && p < pages) ? remap[p] : p;
+    }
   }
-  const long blocks = (long)*n_moves * layers * 2;
+  const long blocks = (long)moves * a.layers * 2;
   for (long b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const int which = (int)(b & 1);
-    const long x = b >> 1;
-    const int layer = (int)(x % layers), i = (int)(x / layers);
-    uint4* pool = which == 0 ? k_pool : v_pool;
-    const uint4* sp = pool + ((long)layer * pool_pages + src[i]) * page_vec;
-    uint4* dp = pool + ((long)layer * pool_pages + dst[i]) * page_vec;
-    for (long v = threadIdx.x; v < page_vec; v += blockDim.x) dp[v] = sp[v];
+    const int i = (int)(b / (2 * a.layers)), x = (int)(b - (long)i * (2 * a.layers));  // x: layer, K or V
+    uint4* pool = static_cast<uint4*>((x & 1) == 0 ? a.k : a.v) + (long)(x >> 1) * a.pool_pages * a.page_vec;
+    copy_vectors(pool + dst[i] * a.page_vec, pool + src[i] * a.page_vec, (int)a.page_vec, [](int v) { return v; });
   }
 }
 
 cudaError_t launch_kv_move(const KvMoveArgs& a, cudaStream_t st) {
-  kv_pages_move_kernel<<<dim3((unsigned)a.n, (unsigned)a.layers, 2), 256, 0, st>>>(
-      static_cast<uint4*>(a.k), static_cast<uint4*>(a.v), a.src, a.dst, a.tokens, a.n, a.pool_pages, a.heads, a.page_size,
-      a.row_vec, a.err);
-  return cudaGetLastError();
+  return launch_k(kv_pages_move_kernel, dim3((unsigned)a.n, (unsigned)a.layers, 2), dim3(256), 0, st, a);
 }
 
 cudaError_t launch_kv_compact(const KvCompactArgs& a, cudaStream_t st) {
@@ -170,14 +181,10 @@ cudaError_t launch_kv_compact(const KvCompactArgs& a, cudaStream_t st) {
   }
   const int pages = (int)a.pool_pages;
   int *remap = a.ws, *live = a.ws + pages, *moves = a.ws + pages + 1, *src = a.ws + pages + 2, *dst = a.ws + 2 * pages + 2;
-  kv_compact_plan_kernel<<<1, 1024, smem, st>>>(a.tables, a.counts, a.rows, a.width, pages, a.reserved, remap, live, src, dst,
-                                                moves, a.err);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_k(kv_compact_plan_kernel, dim3(1), dim3(1024), smem, st, a.tables, a.counts, a.rows, a.width,
+                                 pages, a.reserved, remap, live, src, dst, moves, a.err);
   if (e != cudaSuccess) return e;
-  kv_compact_move_kernel<<<(unsigned)(8 * a.num_sms), 256, 0, st>>>(
-      static_cast<uint4*>(a.k), static_cast<uint4*>(a.v), a.tables, a.out_tables, a.counts, a.rows, a.width, a.layers,
-      a.pool_pages, a.page_vec, remap, src, dst, moves);
-  return cudaGetLastError();
+  return launch_k(kv_compact_move_kernel, dim3((unsigned)(8 * a.num_sms)), dim3(256), 0, st, a);
 }
 
 }  // namespace mesh

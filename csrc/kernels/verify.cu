@@ -18,10 +18,11 @@
 // Two launches:
 //   stats    grid (chunk, row): one CTA reads one chunk of a row once, keeps it in registers, and writes its
 //            maximum (first index) and its mass relative to that maximum. Rows past a session's drafts are
-//            not read. Bound by reading the logits.
-//   resolve  one cluster of 8 CTAs per session: joins the chunks of the session's rows, decides, and for the draw
-//            every CTA sums its eighth of the row tile by tile; the sums meet in distributed shared memory and
-//            the CTA that holds the point scans the one tile it falls into.
+//            not read. Bound by reading the logits and, as closely, by the 64-bit exponentials.
+//   resolve  one cluster of 8 CTAs per session: joins the chunks of the session's rows and decides. Drawing from p (or
+//            p without one token) the chunks' masses are known and one CTA goes on: it picks the chunk, the
+//            256-token unit in it, and the token. For max(p - q, 0) every CTA first sums the units of its eighth of the
+//            row; the shares meet in distributed shared memory and the CTA whose share holds the point goes on.
 #include <cfloat>
 #include <climits>
 
@@ -33,14 +34,15 @@ namespace mesh {
 namespace verify {
 
 constexpr int SNT = 256;                // threads of a stats CTA
-constexpr int EPT = 32;                 // logits per thread
-constexpr int CHUNK = SNT * EPT;        // logits per stats CTA
 constexpr int RNT = 512;                // threads of a resolve CTA
 constexpr int CLUSTER = 8;
-constexpr int TILE_EPT = 8;
-constexpr int TILE = RNT * TILE_EPT;    // logits per tile of the draw
 constexpr int MAX_DRAFTS = VERIFY_MAX_DRAFTS;
-constexpr int MAX_TILES = 256;          // tiles of one CTA's share of a row
+constexpr int PER_LANE = 8;            // tokens of a unit per lane
+constexpr int UNIT = 32 * PER_LANE;     // tokens whose sum one warp of the resolve kernel makes
+constexpr int MAX_SUMS = 4096;          // chunks of a row, units of a CTA's share
+// Logits per stats thread. 32 where the rows fill the GPU (fewer partials, more loads in flight), 8 where
+// they do not: one session of 5 rows over 128256 tokens then makes 315 CTAs instead of 80.
+constexpr int EPT_MANY = 32, EPT_FEW = 8;
 
 struct Part {
   float m;    // maximum of the chunk (-inf: no selectable token)
@@ -57,11 +59,59 @@ __device__ __forceinline__ int drafts_of(const Args& a, int b) {
   return a.lens ? max(0, min(a.lens[b], a.K)) : a.K;
 }
 
-// mass of logit x in a row with maximum m (m > -inf); equal infinities count as the maximum
-__device__ __forceinline__ double mass(float x, float m, double inv_t) {
-  if (x == m) return 1.0;
-  if (!(x > -INFINITY)) return 0.0;  // -inf or NaN
-  return exp(((double)x - (double)m) * inv_t);
+// e^((x - m) / T) in 64 bits for one row with a finite maximum m. Reduction by a table (Tang, 1989): with
+// z = (x - m) 32 / (T ln 2) = n + f, |f| <= 1/2, it is 2^(n / 32) e^(f ln2 / 32): lane j of the warp holds 2^(j / 32),
+// fetched by shuffle, and a polynomial of degree 4 does the rest (its next term, (ln2 / 64)^5 / 120 = 1.2e-12, bounds
+// the relative error). Ten 64-bit operations and about as many others; the loops below are bound by their issue,
+// and CUDA's exp() made them four times slower. All 32 lanes of a warp must call it together.
+// The exponential has to stay a normal number, so tokens below `low` = m - 700 T (masked ones, NaN) are taken
+// there, and what is not well above their mass, `none`, has none. T is taken as at most 1e30 and at least 1e-30.
+struct Exp {
+  double scale, top, table, none;
+  float low, m;
+  bool only;  // no logit other than m itself is within 700 T (m is infinite, or its neighbours are further): equal shares
+  __device__ __forceinline__ Exp(float m_, float inv_t) : m(m_) {
+    constexpr double PER = 46.166241308446828384;  // 32 / ln 2
+    inv_t = fmaxf(fminf(inv_t, 1e30f), 1e-30f);
+    low = __fsub_ru(m_, 700.f / inv_t);
+    only = low >= m_;
+    if (only) {
+      low = -700.f;
+      inv_t = 1.f;
+    }
+    scale = (double)inv_t * PER;
+    top = only ? 0.0 : (double)m_;
+    table = exp2((double)(threadIdx.x & 31) * 0.03125);
+    double w, p;
+    split(low, w, p);
+    none = w * p * 1e12;  // above the sum of any chunk of masked tokens
+  }
+  // what split takes for logit x
+  __device__ __forceinline__ float arg(float x) const { return only ? (x == m ? 0.f : -INFINITY) : x; }
+  __device__ __forceinline__ void split(float x, double& w, double& poly) const {  // the mass is w * poly
+    constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the nearest integer
+    constexpr double L = 0.021660849392498290;     // ln 2 / 32
+    constexpr double C2 = L * L / 2, C3 = C2 * L / 3, C4 = C3 * L / 4;
+    const double z = ((double)fmaxf(x, low) - top) * scale;
+    const double k = z + MAGIC;
+    const int n = __double2loint(k);
+    const double f = z - (k - MAGIC);
+    const double t = __shfl_sync(0xffffffffu, table, n);  // the low five bits choose the lane
+    w = __hiloint2double(__double2hiint(t) + (n & ~31) * 32768, __double2loint(t));
+    poly = fma(fma(fma(fma(C4, f, C3), f, C2), f, L), f, 1.0);
+  }
+  __device__ __forceinline__ double operator()(float x) const {
+    double w, p;
+    split(arg(x), w, p);
+    return w * p;
+  }
+};
+
+// sum over the warp, the same value in every lane
+__device__ __forceinline__ double warp_sum(double s) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
 }
 
 // larger value first, then the lower index
@@ -72,52 +122,92 @@ __device__ __forceinline__ void take(float& m, int& i, float om, int oi) {
   }
 }
 
-template <typename T>
+// N consecutive elements of a row from index i on, those at or past V as -inf (q: 0). VEC: the row starts
+// on a 16-byte boundary, and i is a multiple of N.
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ void load_run(const T* x, int i, int V, float fill, float (&v)[N]) {
+  constexpr int PER = 16 / sizeof(T);
+  if constexpr (VEC && N % PER == 0) {
+#pragma unroll
+    for (int c = 0; c < N; c += PER) {
+      if (i + c + PER <= V) {
+        const uint4 u = *reinterpret_cast<const uint4*>(x + i + c);
+        const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) v[c + j] = to_f(e[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) v[c + j] = i + c + j < V ? to_f(x[i + c + j]) : fill;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = i + j < V ? to_f(x[i + j]) : fill;
+  }
+}
+
+// Logits of a chunk in a stats thread: runs of RUN elements, SNT * RUN apart.
+template <typename T, int EPT, bool VEC>
 __global__ void __launch_bounds__(SNT) stats_kernel(const Args a) {
+  constexpr int RUN = VEC ? 16 / (int)sizeof(T) : 1;
+  constexpr int CHUNK = SNT * EPT;
   __shared__ float red_m[SNT / 32];
-  __shared__ int red_i[SNT / 32];
+  __shared__ int first;
   __shared__ double red_s[SNT / 32];
-  griddep_launch_dependents();
   griddep_wait();
+  griddep_launch_dependents();
   const int row = blockIdx.y, b = row / (a.K + 1), k = row - b * (a.K + 1);
   if (k > drafts_of(a, b)) return;
   const T* x = static_cast<const T*>(a.logits) + (long)b * a.ld_seq + (long)k * a.ld_row;
   const float t = a.inv_t ? a.inv_t[b] : 1.f;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int i0 = blockIdx.x * CHUNK;
-  float v[EPT];
+  const int i0 = blockIdx.x * CHUNK + tid * RUN;
+  float v[EPT / RUN][RUN];
+#pragma unroll
+  for (int e = 0; e < EPT / RUN; ++e) load_run<T, RUN, VEC>(x, i0 + e * SNT * RUN, a.V, -INFINITY, v[e]);
   float m = -INFINITY;
-  int idx = INT_MAX;
 #pragma unroll
-  for (int e = 0; e < EPT; ++e) {
-    const int i = i0 + e * SNT + tid;
-    v[e] = i < a.V ? to_f(x[i]) : -INFINITY;
-  }
+  for (int e = 0; e < EPT / RUN; ++e)
 #pragma unroll
-  for (int e = 0; e < EPT; ++e) {
-    if (v[e] > m) {
-      m = v[e];
-      idx = i0 + e * SNT + tid;
-    }
-  }
+    for (int j = 0; j < RUN; ++j) m = fmaxf(m, v[e][j]);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    take(m, idx, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, idx, o));
-  if (lane == 0) {
-    red_m[warp] = m;
-    red_i[warp] = idx;
-  }
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (tid == 0) first = INT_MAX;
+  if (lane == 0) red_m[warp] = m;
   __syncthreads();
+  const float own = m;
 #pragma unroll
-  for (int w = 0; w < SNT / 32; ++w) take(m, idx, red_m[w], red_i[w]);
+  for (int w = 0; w < SNT / 32; ++w) m = fmaxf(m, red_m[w]);
+  if (own == m && m > -INFINITY) {  // few warps hold the maximum: only they look for its index
+    int at = INT_MAX;
+#pragma unroll
+    for (int e = EPT / RUN - 1; e >= 0; --e)
+#pragma unroll
+      for (int j = RUN - 1; j >= 0; --j)
+        if (v[e][j] == m) at = i0 + e * SNT * RUN + j;
+    if (at != INT_MAX) atomicMin(&first, at);
+  }
   double s = 0.0;
   if (t > 0.f && m > -INFINITY) {
-#pragma unroll 4
-    for (int e = 0; e < EPT; ++e) s += mass(v[e], m, (double)t);
+    const Exp mass(m, t);
+    if (mass.only)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      for (int e = 0; e < EPT / RUN; ++e)
+#pragma unroll
+        for (int j = 0; j < RUN; ++j) v[e][j] = mass.arg(v[e][j]);
+#pragma unroll
+    for (int e = 0; e < EPT / RUN; ++e)
+#pragma unroll
+      for (int j = 0; j < RUN; ++j) {
+        double w, p;
+        mass.split(v[e][j], w, p);
+        s = fma(w, p, s);
+      }
+    s = warp_sum(s);
     if (lane == 0) red_s[warp] = s;
-    __syncthreads();
+  }
+  __syncthreads();
+  if (t > 0.f && m > -INFINITY) {
     s = 0.0;
 #pragma unroll
     for (int w = 0; w < SNT / 32; ++w) s += red_s[w];
@@ -125,39 +215,10 @@ __global__ void __launch_bounds__(SNT) stats_kernel(const Args a) {
   if (tid == 0) {
     Part p;
     p.m = m;
-    p.idx = idx;
+    p.idx = first;
     p.s = s;
     static_cast<Part*>(a.parts)[(long)row * a.chunks + blockIdx.x] = p;
   }
-}
-
-// What is drawn from: 0 p, 1 max(p - q, 0), 2 p without one token.
-struct Draw {
-  int mode, skip;
-  float m;
-  double inv_t, inv_z;
-};
-
-template <typename T, typename Q>
-__device__ __forceinline__ double weight(const Draw& d, const T* x, const Q* q, int i) {
-  const double p = mass(to_f(x[i]), d.m, d.inv_t) * d.inv_z;
-  if (d.mode == 0) return p;
-  if (d.mode == 2) return i == d.skip ? 0.0 : p;
-  const float f = to_f(q[i]);
-  const double r = p - (f > 0.f ? (double)f : 0.0);  // a NaN or negative q counts as none
-  return r > 0.0 ? r : 0.0;
-}
-
-// sum over the CTA, the same value in every thread
-__device__ __forceinline__ double block_sum(double s, double* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
-  __syncthreads();
-  s = 0.0;
-  for (int w = 0; w < RNT / 32; ++w) s += red[w];
-  return s;
 }
 
 __device__ __forceinline__ double ld_dsmem_f64(uint32_t cluster_addr) {
@@ -166,27 +227,49 @@ __device__ __forceinline__ double ld_dsmem_f64(uint32_t cluster_addr) {
   return v;
 }
 
-template <typename T, typename Q>
-__global__ void __launch_bounds__(RNT) resolve_kernel(const Args a) {
+template <typename T, typename Q, bool VEC>
+__global__ void __launch_bounds__(RNT, 2) resolve_kernel(const Args a, int chunk) {
+  constexpr int WARPS = RNT / 32;
+  constexpr int RUN = VEC ? 16 / (int)sizeof(T) : 1;  // consecutive tokens of a lane
   __shared__ float row_m[MAX_DRAFTS + 1];
-  __shared__ int row_i[MAX_DRAFTS + 1];
+  __shared__ int row_i[MAX_DRAFTS + 1], row_x[MAX_DRAFTS + 1], row_ok[MAX_DRAFTS + 1];
   __shared__ double row_z[MAX_DRAFTS + 1], row_p[MAX_DRAFTS + 1];
-  __shared__ double tile_sum[MAX_TILES];
-  __shared__ double red[RNT / 32];
+  __shared__ double sums[MAX_SUMS];
   __shared__ double share;  // this CTA's mass of the row, read by its cluster
-  __shared__ int s_n;
   const int b = blockIdx.x / CLUSTER, rank = blockIdx.x % CLUSTER;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  griddep_wait();
-  griddep_launch_dependents();
-  const int n = drafts_of(a, b), K = a.K;
-  const float t = a.inv_t ? a.inv_t[b] : 1.f;
-  const bool greedy = !(t > 0.f);
+  const int K = a.K, V = a.V;
   const T* xs = static_cast<const T*>(a.logits) + (long)b * a.ld_seq;
   const Q* qs = static_cast<const Q*>(a.probs) + (a.probs ? (long)b * a.lq_seq : 0);
+  // The stats kernel lets this one start once everything before it is complete, so all inputs but its
+  // partials may be read already.
+  const int n = drafts_of(a, b);
+  const float t = a.inv_t ? a.inv_t[b] : 1.f;
+  const float u_draw = a.uniforms[(long)b * (K + 1) + K];
+  const bool greedy = !(t > 0.f);
+  int id = -1;
+  float at_x = -INFINITY, at_q = 0.f, u = 0.f;
+  auto fetch = [&](int k) {  // of the draft of row k: its token, logit, draft probability and uniform
+    id = -1;
+    at_x = -INFINITY;
+    at_q = 0.f;
+    if (k < n) {
+      id = a.ids[(long)b * K + k];
+      u = a.uniforms[(long)b * (K + 1) + k];
+      if (id >= 0 && id < V) {
+        at_x = to_f(xs[(long)k * a.ld_row + id]);
+        at_q = a.probs ? to_f(qs[(long)k * a.lq_row + id]) : 1.f;
+      }
+    }
+  };
+  fetch(warp);
+  griddep_wait();
+  griddep_launch_dependents();
 
   // every CTA of the cluster joins the chunks of the session's rows: a warp per row
-  for (int k = warp; k <= n; k += RNT / 32) {
+#pragma unroll 1
+  for (int k = warp; k <= n; k += WARPS) {
+    if (k != warp) fetch(k);
     const Part* p = static_cast<const Part*>(a.parts) + ((long)b * (K + 1) + k) * a.chunks;
     float m = -INFINITY;
     int idx = INT_MAX;
@@ -194,52 +277,35 @@ __global__ void __launch_bounds__(RNT) resolve_kernel(const Args a) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
       take(m, idx, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, idx, o));
-    double z = 0.0;
-    if (!greedy && m > -INFINITY)
-      for (int c = lane; c < a.chunks; c += 32)
-        if (p[c].m > -INFINITY) z += p[c].s * mass(p[c].m, m, (double)t);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    double z = 0.0, px = 0.0;
+    if (!greedy && m > -INFINITY) {
+      const Exp mass(m, t);
+#pragma unroll 1
+      for (int c = lane; c - lane < a.chunks; c += 32) {
+        const double f = mass(c < a.chunks ? p[c].m : -INFINITY);
+        if (c < a.chunks) z += p[c].s * f;
+      }
+      z = warp_sum(z);
+      const double w = mass(at_x);
+      px = w > mass.none ? w / z : 0.0;
+    } else if (greedy) {
+      px = m > -INFINITY && k < n && idx == id ? 1.0 : 0.0;
+    }
     if (lane == 0) {
       row_m[k] = m;
       row_i[k] = m > -INFINITY ? idx : -1;
       row_z[k] = z;
-      double px = 0.0;
-      if (k < n) {
-        const int x = a.ids[(long)b * K + k];
-        if (greedy)
-          px = (m > -INFINITY && idx == x) ? 1.0 : 0.0;
-        else if (x >= 0 && x < a.V && m > -INFINITY)
-          px = mass(to_f(xs[(long)k * a.ld_row + x]), m, (double)t) / z;
-      }
+      row_x[k] = id;
       row_p[k] = px;
+      row_ok[k] = k < n && px > 0.0 && (greedy || (double)u * (at_q > 0.f ? (double)at_q : 0.0) < px);
     }
   }
   __syncthreads();
-  if (tid == 0) {
-    int k = 0;
-    for (; k < n; ++k) {
-      bool ok = row_p[k] > 0.0;
-      if (ok && !greedy) {
-        double qx = 1.0;
-        if (a.probs) {
-          const float f = to_f(qs[(long)k * a.lq_row + a.ids[(long)b * K + k]]);
-          qx = f > 0.f ? (double)f : 0.0;
-        }
-        ok = (double)a.uniforms[(long)b * (K + 1) + k] * qx < row_p[k];
-      }
-      if (!ok) break;
-    }
-    s_n = k;
-  }
-  __syncthreads();
-  const int acc = s_n;
+  int acc = 0;
+  while (acc < n && row_ok[acc]) ++acc;
   if (rank == 0) {
     for (int k = tid; k <= K; k += RNT) {
-      if (k < acc)
-        a.tokens[(long)b * (K + 1) + k] = a.ids[(long)b * K + k];
-      else if (k > acc)
-        a.tokens[(long)b * (K + 1) + k] = -1;
+      if (k != acc) a.tokens[(long)b * (K + 1) + k] = k < acc ? row_x[k] : -1;
       if (k < K) a.draft_p[(long)b * K + k] = k < n ? (float)row_p[k] : 0.f;
     }
     if (tid == 0) a.accepted[b] = acc;
@@ -252,113 +318,210 @@ __global__ void __launch_bounds__(RNT) resolve_kernel(const Args a) {
   }
   const T* x = xs + (long)acc * a.ld_row;
   const Q* q = qs + (a.probs && acc < n ? (long)acc * a.lq_row : 0);
-  Draw d;
-  d.m = m;
-  d.inv_t = (double)t;
-  d.inv_z = 1.0 / row_z[acc];
-  d.skip = acc < n ? a.ids[(long)b * K + acc] : -1;
-  d.mode = acc == n ? 0 : a.probs ? 1 : 2;
-  const int tiles = (a.V + TILE - 1) / TILE, per = (tiles + CLUSTER - 1) / CLUSTER;
-  const int t0 = min(tiles, rank * per), t1 = min(tiles, t0 + per);
-  double total = 0.0, ahead = 0.0, own = 0.0;
-  for (int round = 0; round < 2; ++round) {
-    own = 0.0;
-    for (int w = t0; w < t1; ++w) {
-      double s = 0.0;
+  const Part* parts = static_cast<const Part*>(a.parts) + ((long)b * (K + 1) + acc) * a.chunks;
+  const Exp mass(m, t);
+  const double inv_z = 1.0 / row_z[acc];
+  // what is drawn from: 0 p, 1 max(p - q, 0), 2 p without the token `skip`
+  const int skip = acc < n ? row_x[acc] : -1;
+  int mode = acc == n ? 0 : a.probs ? 1 : skip >= 0 && skip < V ? 2 : 0;
+  const float u_low = fmaxf(0.f, fminf(u_draw, 1.f - FLT_EPSILON / 2));  // the point lies below the whole
+
+  // Mass of lane's tokens of the unit at token i0, in runs of RUN, 32 * RUN apart.
+  auto weights = [&](int i0, int end, double (&w)[PER_LANE / RUN][RUN]) {
 #pragma unroll
-      for (int e = 0; e < TILE_EPT; ++e) {
-        const int i = w * TILE + e * RNT + tid;
-        if (i < a.V) s += weight(d, x, q, i);
+    for (int e = 0; e < PER_LANE / RUN; ++e) {
+      const int i = i0 + (e * 32 + lane) * RUN;
+      float v[RUN], f[RUN];
+      load_run<T, RUN, VEC>(x, i, end, -INFINITY, v);
+      if (mode == 1) load_run<Q, RUN, VEC>(q, i, end, 0.f, f);
+#pragma unroll
+      for (int j = 0; j < RUN; ++j) {
+        double p = mass(v[j]);
+        if (mode == 1) {
+          // a NaN or negative q counts as none
+          p = fma(p, inv_z, -(double)fmaxf(f[j], 0.f));
+        } else {
+          p *= inv_z;
+          if (i + j == skip && mode == 2) p = 0.0;
+        }
+        w[e][j] = p > mass.none ? p : 0.0;
       }
-      s = block_sum(s, red);
-      if (tid == 0) tile_sum[w - t0] = s;
-      own += s;
     }
+  };
+  // sums[] of the units of [i0, end): a warp each
+  auto unit_sums = [&](int i0, int end) {
+#pragma unroll 1
+    for (int y = warp; i0 + y * UNIT < end; y += WARPS) {
+      double w[PER_LANE / RUN][RUN], s = 0.0;
+      weights(i0 + y * UNIT, end, w);
+#pragma unroll
+      for (int e = 0; e < PER_LANE / RUN; ++e)
+#pragma unroll
+        for (int j = 0; j < RUN; ++j) s += w[e][j];
+      s = warp_sum(s);
+      if (lane == 0) sums[y] = s;
+    }
+    __syncthreads();
+  };
+  // the entry of sums[0, n) that holds the point, `before` = the mass before it; the last one with mass takes what
+  // the rounding of the sums leaves over
+  auto choose = [&](int n_sums, double point, double& before) {
+    double run = before;
+    int at = -1;
+    for (int c = 0; c < n_sums; ++c) {
+      const double s = sums[c];
+      if (s > 0.0) {
+        at = c;
+        before = run;
+        run += s;
+        if (run > point) break;
+      }
+    }
+    return at;
+  };
+
+  double before = 0.0, point = 0.0;
+  int i0 = 0, end = 0;  // tokens whose unit sums are in sums[]
+  if (mode == 1) {
+    const int units = (V + UNIT - 1) / UNIT, per = (units + CLUSTER - 1) / CLUSTER;
+    i0 = min(V, rank * per * UNIT);
+    end = min(V, i0 + per * UNIT);
+    unit_sums(i0, end);
+    double own = 0.0, total = 0.0;
+    for (int c = 0; i0 + c * UNIT < end; ++c) own += sums[c];
     if (tid == 0) share = own;
     cluster_sync();
-    total = ahead = 0.0;
+#pragma unroll
     for (int r = 0; r < CLUSTER; ++r) {
       const double s = ld_dsmem_f64(mapa_shared(smem_u32(&share), (uint32_t)r));
-      if (r < rank) ahead += s;
+      if (r < rank) before += s;
       total += s;
     }
     cluster_sync();  // the shares have been read
-    if (total > 0.0 || d.mode == 0) break;
-    d.mode = 0;  // nothing is left of p: the draft's distribution covers it, so p itself is drawn from
+    point = (double)u_low * total;
+    if (!(total > 0.0))
+      mode = 0;  // nothing is left of p: the draft's distribution covers it, so p itself is drawn from
+    else if (!(before <= point && point < before + own))
+      return;  // the shares' ends are the same sums in every CTA: the point lies in exactly one share
   }
-  // the shares' ends are the same sums in every CTA, so the point (below the whole) lies in exactly one share
-  const float u = fmaxf(0.f, fminf(a.uniforms[(long)b * (K + 1) + K], 1.f - FLT_EPSILON / 2));
-  const double point = (double)u * total;
-  if (!(ahead <= point && point < ahead + own)) return;
-  // tile, then element
-  double run = ahead, before = ahead;  // mass before tile c, and before the chosen tile
-  int w = t0;
-  for (int c = t0; c < t1; ++c) {
-    const double s = tile_sum[c - t0];
-    if (s > 0.0) {  // the last tile with mass takes what the rounding of these sums leaves over
-      w = c;
-      before = run;
-      run += s;
-      if (run > point) break;
+  if (mode != 1) {
+    if (rank != 0) return;
+    if (mode == 2) {
+      // the chunk that holds the token left out is summed again without it
+      i0 = skip / chunk * chunk;
+      end = min(V, i0 + chunk);
+      unit_sums(i0, end);
+      for (int c = 0; i0 + c * UNIT < end; ++c) before += sums[c];
     }
-  }
-  __shared__ double pre[RNT];
-  __shared__ int best, fallback;
-  // thread t holds elements t * TILE_EPT .. of the tile, so the scan follows vocabulary order
-  double mine = 0.0;
-  int top = -1;
-  for (int e = 0; e < TILE_EPT; ++e) {
-    const int i = w * TILE + tid * TILE_EPT + e;
-    if (i < a.V) {
-      const double f = weight(d, x, q, i);
-      mine += f;
-      if (f > 0.0) top = i;
-    }
-  }
-  if (tid == 0) {
-    best = INT_MAX;
-    fallback = -1;
-  }
-  pre[tid] = mine;
-  __syncthreads();
-  for (int o = 1; o < RNT; o <<= 1) {
-    const double f = tid >= o ? pre[tid - o] : 0.0;
+    const double without = before;
     __syncthreads();
-    pre[tid] += f;
-    __syncthreads();
-  }
-  double c = before + (tid ? pre[tid - 1] : 0.0);
-  if (top >= 0) atomicMax(&fallback, top);
-  for (int e = 0; e < TILE_EPT; ++e) {
-    const int i = w * TILE + tid * TILE_EPT + e;
-    if (i >= a.V) break;
-    const double f = weight(d, x, q, i);
-    c += f;
-    if (f > 0.0 && c > point) {
-      atomicMin(&best, i);
-      break;
+#pragma unroll 1
+    for (int c = warp * 32; c < a.chunks; c += RNT) {
+      const int e = c + lane;
+      const double f = mass(e < a.chunks ? parts[e].m : -INFINITY);
+      if (e < a.chunks) {
+        const double s = mode == 2 && e == skip / chunk ? without : parts[e].s * f * inv_z;
+        sums[e] = s > mass.none ? s : 0.0;
+      }
     }
+    __syncthreads();
+    double total = 0.0;
+    for (int c = 0; c < a.chunks; ++c) total += sums[c];
+    if (mode == 2 && !(total > 0.0)) {  // the token left out had all the mass: it is drawn after all
+      if (tid == 0) *new_token = skip;
+      return;
+    }
+    point = (double)u_low * total;
+    before = 0.0;
+    const int c = choose(a.chunks, point, before);
+    __syncthreads();
+    i0 = max(c, 0) * chunk;
+    end = min(V, i0 + chunk);
+    unit_sums(i0, end);
   }
-  __syncthreads();
-  if (tid == 0) *new_token = best != INT_MAX ? best : fallback;
+  const int n_units = (end - i0 + UNIT - 1) / UNIT;
+  const int y = choose(n_units, point, before);
+  if (warp != 0) return;
+  double w[PER_LANE / RUN][RUN];
+  i0 += max(y, 0) * UNIT;
+  weights(i0, end, w);
+  int last = -1;
+  double run = before;  // mass before the runs of step e
+#pragma unroll
+  for (int e = 0; e < PER_LANE / RUN; ++e) {
+    double mine = 0.0;
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) mine += w[e][j];
+    double incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double f = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += f;
+    }
+    double c = run + (incl - mine);
+    int hit = INT_MAX;
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) {
+      c += w[e][j];
+      if (w[e][j] > 0.0) {
+        last = i0 + (e * 32 + lane) * RUN + j;
+        if (c > point && hit == INT_MAX) hit = last;
+      }
+    }
+    hit = __reduce_min_sync(0xffffffffu, hit);
+    if (hit != INT_MAX) {
+      if (lane == 0) *new_token = hit;
+      return;
+    }
+    run += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  last = __reduce_max_sync(0xffffffffu, last);
+  if (lane == 0) *new_token = last;
 }
+
+// 16-byte loads where every row of both operands starts on a 16-byte boundary
+bool vectors(const VerifyArgs& a) {
+  auto ok = [](const void* p, long ld_row, long ld_seq, int size) {
+    return (uintptr_t)p % 16 == 0 && ld_row * size % 16 == 0 && ld_seq * size % 16 == 0;
+  };
+  return ok(a.logits, a.ld_row, a.ld_seq, a.logits_bf16 ? 2 : 4) &&
+         (!a.probs || ok(a.probs, a.lq_row, a.lq_seq, a.probs_bf16 ? 2 : 4));
+}
+
+template <typename T, typename Q, int EPT, bool VEC>
+cudaError_t launch(const VerifyArgs& a, cudaStream_t st) {
+  const cudaError_t e =
+      launch_k(stats_kernel<T, EPT, VEC>, dim3((unsigned)a.chunks, (unsigned)(a.B * (a.K + 1))), dim3(SNT), 0, st, a);
+  if (e != cudaSuccess) return e;
+  return launch_kc(resolve_kernel<T, Q, VEC>, dim3((unsigned)(a.B * CLUSTER)), dim3(RNT), 0, st, CLUSTER, a, SNT * EPT);
+}
+
+template <typename T, typename Q>
+cudaError_t pick(const VerifyArgs& a, bool few, cudaStream_t st) {
+  if (vectors(a)) return few ? launch<T, Q, EPT_FEW, true>(a, st) : launch<T, Q, EPT_MANY, true>(a, st);
+  return few ? launch<T, Q, EPT_FEW, false>(a, st) : launch<T, Q, EPT_MANY, false>(a, st);
+}
+
+// Too few chunks of the larger kind for two per SM of a 148-SM GPU: smaller ones.
+bool few_rows(int64_t rows, int64_t V) { return rows * ((V + SNT * EPT_MANY - 1) / (SNT * EPT_MANY)) < 2 * 148; }
 
 }  // namespace verify
 
-int verify_chunks(int64_t V) { return (int)((V + verify::CHUNK - 1) / verify::CHUNK); }
-int64_t verify_max_vocab() { return (int64_t)verify::TILE * verify::MAX_TILES * verify::CLUSTER; }
+int verify_chunks(int64_t B, int64_t K, int64_t V) {
+  const int64_t c = verify::SNT * (verify::few_rows(B * (K + 1), V) ? verify::EPT_FEW : verify::EPT_MANY);
+  return (int)((V + c - 1) / c);
+}
+int64_t verify_max_vocab() { return (int64_t)verify::SNT * verify::EPT_FEW * verify::MAX_SUMS; }
 int64_t verify_parts_bytes(int64_t B, int64_t K, int64_t V) {
-  return B * (K + 1) * verify_chunks(V) * (int64_t)sizeof(verify::Part);
+  return B * (K + 1) * verify_chunks(B, K, V) * (int64_t)sizeof(verify::Part);
 }
 
 cudaError_t launch_verify(const VerifyArgs& a, cudaStream_t st) {
   using namespace verify;
-  const dim3 sg((unsigned)a.chunks, (unsigned)(a.B * (a.K + 1)));
-  const cudaError_t e = launch_k(a.logits_bf16 ? stats_kernel<__nv_bfloat16> : stats_kernel<float>, sg, dim3(SNT), 0, st, a);
-  if (e != cudaSuccess) return e;
-  auto kern = a.logits_bf16 ? (a.probs_bf16 ? resolve_kernel<__nv_bfloat16, __nv_bfloat16> : resolve_kernel<__nv_bfloat16, float>)
-                            : (a.probs_bf16 ? resolve_kernel<float, __nv_bfloat16> : resolve_kernel<float, float>);
-  return launch_kc(kern, dim3((unsigned)(a.B * CLUSTER)), dim3(RNT), 0, st, CLUSTER, a);
+  using bf = __nv_bfloat16;
+  const bool few = few_rows((int64_t)a.B * (a.K + 1), a.V);
+  if (a.logits_bf16) return a.probs_bf16 ? pick<bf, bf>(a, few, st) : pick<bf, float>(a, few, st);
+  return a.probs_bf16 ? pick<float, bf>(a, few, st) : pick<float, float>(a, few, st);
 }
 
 }  // namespace mesh

@@ -149,7 +149,7 @@ void verify_drafts(const at::Tensor& logits, const at::Tensor& ids, const at::Te
   a.B = (int)B;
   a.K = (int)K;
   a.V = (int)V;
-  a.chunks = verify_chunks(V);
+  a.chunks = verify_chunks(B, K, V);
   a.logits_bf16 = x.scalar_type() == at::kBFloat16;
   a.probs_bf16 = qs && probs->scalar_type() == at::kBFloat16;
   C10_CUDA_CHECK(launch_verify(a, at::cuda::getCurrentCUDAStream()));
