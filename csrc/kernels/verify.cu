@@ -34,7 +34,7 @@ namespace mesh {
 namespace verify {
 
 constexpr int SNT = 256;                // threads of a stats CTA
-constexpr int RNT = 512;                // threads of a resolve CTA
+constexpr int RNT = 256;                // threads of a resolve CTA
 constexpr int CLUSTER = 8;
 constexpr int MAX_DRAFTS = VERIFY_MAX_DRAFTS;
 constexpr int PER_LANE = 8;            // tokens of a unit per lane
@@ -111,6 +111,16 @@ struct Exp {
 __device__ __forceinline__ double warp_sum(double s) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+// inclusive sums over the lanes
+__device__ __forceinline__ double warp_scan(double s, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double f = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += f;
+  }
   return s;
 }
 
@@ -228,7 +238,7 @@ __device__ __forceinline__ double ld_dsmem_f64(uint32_t cluster_addr) {
 }
 
 template <typename T, typename Q, bool VEC>
-__global__ void __launch_bounds__(RNT, 2) resolve_kernel(const Args a, int chunk) {
+__global__ void __launch_bounds__(RNT, 4) resolve_kernel(const Args a, int chunk) {
   constexpr int WARPS = RNT / 32;
   constexpr int RUN = VEC ? 16 / (int)sizeof(T) : 1;  // consecutive tokens of a lane
   __shared__ float row_m[MAX_DRAFTS + 1];
@@ -326,57 +336,71 @@ __global__ void __launch_bounds__(RNT, 2) resolve_kernel(const Args a, int chunk
   int mode = acc == n ? 0 : a.probs ? 1 : skip >= 0 && skip < V ? 2 : 0;
   const float u_low = fmaxf(0.f, fminf(u_draw, 1.f - FLT_EPSILON / 2));  // the point lies below the whole
 
-  // Mass of lane's tokens of the unit at token i0, in runs of RUN, 32 * RUN apart.
-  auto weights = [&](int i0, int end, double (&w)[PER_LANE / RUN][RUN]) {
+  // a lane's tokens of the unit at token i0, in runs of RUN, 32 * RUN apart
+  struct Raw {
+    float v[PER_LANE / RUN][RUN], f[PER_LANE / RUN][RUN];
+  };
+  auto fetch_unit = [&](int i0, int end, Raw& r) {
 #pragma unroll
     for (int e = 0; e < PER_LANE / RUN; ++e) {
       const int i = i0 + (e * 32 + lane) * RUN;
-      float v[RUN], f[RUN];
-      load_run<T, RUN, VEC>(x, i, end, -INFINITY, v);
-      if (mode == 1) load_run<Q, RUN, VEC>(q, i, end, 0.f, f);
-#pragma unroll
-      for (int j = 0; j < RUN; ++j) {
-        double p = mass(v[j]);
-        if (mode == 1) {
-          // a NaN or negative q counts as none
-          p = fma(p, inv_z, -(double)fmaxf(f[j], 0.f));
-        } else {
-          p *= inv_z;
-          if (i + j == skip && mode == 2) p = 0.0;
-        }
-        w[e][j] = p > mass.none ? p : 0.0;
-      }
+      load_run<T, RUN, VEC>(x, i, end, -INFINITY, r.v[e]);
+      if (mode == 1) load_run<Q, RUN, VEC>(q, i, end, 0.f, r.f[e]);
     }
   };
-  // sums[] of the units of [i0, end): a warp each
+  auto weight = [&](const Raw& r, int i0, int e, int j) -> double {
+    double p = mass(r.v[e][j]);
+    if (mode == 1) {
+      p = fma(p, inv_z, -(double)fmaxf(r.f[e][j], 0.f));  // a NaN or negative q counts as none
+    } else {
+      p *= inv_z;
+      if (mode == 2 && i0 + (e * 32 + lane) * RUN + j == skip) p = 0.0;
+    }
+    return p > mass.none ? p : 0.0;
+  };
+  // sums[] of the units of [i0, end): a warp each, the next unit's loads in flight under this one's exponentials
   auto unit_sums = [&](int i0, int end) {
+    Raw r, next;
+    int i = i0 + warp * UNIT;
+    if (i < end) fetch_unit(i, end, r);
 #pragma unroll 1
-    for (int y = warp; i0 + y * UNIT < end; y += WARPS) {
-      double w[PER_LANE / RUN][RUN], s = 0.0;
-      weights(i0 + y * UNIT, end, w);
+    for (; i < end; i += WARPS * UNIT) {
+      if (i + WARPS * UNIT < end) fetch_unit(i + WARPS * UNIT, end, next);
+      double s = 0.0;
 #pragma unroll
       for (int e = 0; e < PER_LANE / RUN; ++e)
 #pragma unroll
-        for (int j = 0; j < RUN; ++j) s += w[e][j];
+        for (int j = 0; j < RUN; ++j) s += weight(r, i, e, j);
       s = warp_sum(s);
-      if (lane == 0) sums[y] = s;
+      if (lane == 0) sums[(i - i0) / UNIT] = s;
+      r = next;
     }
     __syncthreads();
   };
-  // the entry of sums[0, n) that holds the point, `before` = the mass before it; the last one with mass takes what
-  // the rounding of the sums leaves over
-  auto choose = [&](int n_sums, double point, double& before) {
-    double run = before;
+  // Over sums[0, n), 32 at a time: the running sum from `run` on. choose: the entry that holds the point, `run` = the
+  // mass before it; the last one with mass takes what the rounding of the sums leaves over.
+  auto total_of = [&](int n_sums) {
+    double run = 0.0;
+    for (int c = 0; c < n_sums; c += 32) run += warp_sum(c + lane < n_sums ? sums[c + lane] : 0.0);
+    return run;
+  };
+  auto choose = [&](int n_sums, double point, double& run) {
     int at = -1;
-    for (int c = 0; c < n_sums; ++c) {
-      const double s = sums[c];
-      if (s > 0.0) {
-        at = c;
-        before = run;
-        run += s;
-        if (run > point) break;
+    double before = run;
+    for (int c = 0; c < n_sums; c += 32) {
+      const double s = c + lane < n_sums ? sums[c + lane] : 0.0;
+      const double incl = warp_scan(s, lane), ahead = run + (incl - s);
+      const unsigned some = __ballot_sync(0xffffffffu, s > 0.0);
+      const unsigned hit = __ballot_sync(0xffffffffu, s > 0.0 && run + incl > point);
+      if (some) {
+        const int l = hit ? __ffs(hit) - 1 : 31 - __clz(some);
+        at = c + l;
+        before = __shfl_sync(0xffffffffu, ahead, l);
+        if (hit) break;
       }
+      run += __shfl_sync(0xffffffffu, incl, 31);
     }
+    run = before;
     return at;
   };
 
@@ -387,8 +411,8 @@ __global__ void __launch_bounds__(RNT, 2) resolve_kernel(const Args a, int chunk
     i0 = min(V, rank * per * UNIT);
     end = min(V, i0 + per * UNIT);
     unit_sums(i0, end);
-    double own = 0.0, total = 0.0;
-    for (int c = 0; i0 + c * UNIT < end; ++c) own += sums[c];
+    const double own = total_of((end - i0 + UNIT - 1) / UNIT);
+    double total = 0.0;
     if (tid == 0) share = own;
     cluster_sync();
 #pragma unroll
@@ -406,15 +430,15 @@ __global__ void __launch_bounds__(RNT, 2) resolve_kernel(const Args a, int chunk
   }
   if (mode != 1) {
     if (rank != 0) return;
+    double without = 0.0;
     if (mode == 2) {
       // the chunk that holds the token left out is summed again without it
       i0 = skip / chunk * chunk;
       end = min(V, i0 + chunk);
       unit_sums(i0, end);
-      for (int c = 0; i0 + c * UNIT < end; ++c) before += sums[c];
+      without = total_of((end - i0 + UNIT - 1) / UNIT);
+      __syncthreads();
     }
-    const double without = before;
-    __syncthreads();
 #pragma unroll 1
     for (int c = warp * 32; c < a.chunks; c += RNT) {
       const int e = c + lane;
@@ -425,8 +449,7 @@ __global__ void __launch_bounds__(RNT, 2) resolve_kernel(const Args a, int chunk
       }
     }
     __syncthreads();
-    double total = 0.0;
-    for (int c = 0; c < a.chunks; ++c) total += sums[c];
+    const double total = total_of(a.chunks);
     if (mode == 2 && !(total > 0.0)) {  // the token left out had all the mass: it is drawn after all
       if (tid == 0) *new_token = skip;
       return;
@@ -442,28 +465,25 @@ __global__ void __launch_bounds__(RNT, 2) resolve_kernel(const Args a, int chunk
   const int n_units = (end - i0 + UNIT - 1) / UNIT;
   const int y = choose(n_units, point, before);
   if (warp != 0) return;
-  double w[PER_LANE / RUN][RUN];
   i0 += max(y, 0) * UNIT;
-  weights(i0, end, w);
+  Raw r;
+  fetch_unit(i0, end, r);
   int last = -1;
-  double run = before;  // mass before the runs of step e
 #pragma unroll
-  for (int e = 0; e < PER_LANE / RUN; ++e) {
-    double mine = 0.0;
+  for (int e = 0; e < PER_LANE / RUN; ++e) {  // the runs of step e lie before those of step e + 1
+    double w[RUN], mine = 0.0;
 #pragma unroll
-    for (int j = 0; j < RUN; ++j) mine += w[e][j];
-    double incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double f = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += f;
+    for (int j = 0; j < RUN; ++j) {
+      w[j] = weight(r, i0, e, j);
+      mine += w[j];
     }
-    double c = run + (incl - mine);
+    const double incl = warp_scan(mine, lane);
+    double c = before + (incl - mine);
     int hit = INT_MAX;
 #pragma unroll
     for (int j = 0; j < RUN; ++j) {
-      c += w[e][j];
-      if (w[e][j] > 0.0) {
+      c += w[j];
+      if (w[j] > 0.0) {
         last = i0 + (e * 32 + lane) * RUN + j;
         if (c > point && hit == INT_MAX) hit = last;
       }
@@ -473,7 +493,7 @@ __global__ void __launch_bounds__(RNT, 2) resolve_kernel(const Args a, int chunk
       if (lane == 0) *new_token = hit;
       return;
     }
-    run += __shfl_sync(0xffffffffu, incl, 31);
+    before += __shfl_sync(0xffffffffu, incl, 31);
   }
   last = __reduce_max_sync(0xffffffffu, last);
   if (lane == 0) *new_token = last;
