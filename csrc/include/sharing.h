@@ -56,6 +56,11 @@ cudaError_t launch_verify(const VerifyArgs& a, cudaStream_t st);
 constexpr int SHARED_MAX_ROWS = 64;  // query rows (new tokens x heads of a KV group) of one sequence
 constexpr int SHARED_HDR = 8;        // header ints of meta, [0] = number of prefix items
 constexpr int SHARED_ITEM = 8;       // ints per prefix item
+inline
+#ifdef __CUDACC__
+    __host__ __device__
+#endif
+    int shared_items_at(int batch) { return SHARED_HDR + ((5 * batch + 3) & ~3); }  // items start on 16 bytes
 // meta layout: header | per sequence: prefix length, first partial slot, slots per row, prefix slots per row |
 // member lists | items {first member, offset of the members, first row, rows, KV head, first key, end key, slot}
 struct SharedAttnArgs {
@@ -68,7 +73,7 @@ struct SharedAttnArgs {
   float2* pml;              // partial (m, l) [slots]
   __nv_bfloat16* out;
   int* err;
-  int B, T, G, hkv, max_pages, page_size, n_prefix, own_splits, window;
+  int B, T, G, hkv, max_pages, page_size, n_prefix, own_splits, window, num_sms;
   long slot_cap, pool_pages;
 };
 cudaError_t launch_attn_shared(const SharedAttnArgs& a, int head_dim, double scale, cudaStream_t st);

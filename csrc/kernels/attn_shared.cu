@@ -4,8 +4,8 @@
 // the keys of its block table: o = softmax(q K^T scale) V. Sequences that were forked from one another, or
 // that begin with the same prompt, name the same pages for their first keys. Reading those pages once per
 // sequence costs B times the traffic they need, so the work is cut differently:
-//   prefix items   (group, KV head, tile of query rows, key range): the rows (sequence, token, head of the KV group) of
-//                  ALL sequences of the group against the shared keys, which are read once per tile of rows;
+//   prefix items   (group, KV head, up to 256 query rows, key range): the rows (sequence, token, head of the KV group) of
+//                  ALL sequences of the group against the shared keys, read once for them (attn_shared_tc.cu);
 //   own items      (sequence, KV head, key range): the rows of one sequence against the rest of its keys.
 // Every item leaves, per row, the maximum m, the sum l of 2^(s - m) and the unnormalised output in fp32; the
 // combine kernel merges a row's partials: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i. All partials of a row
@@ -13,34 +13,14 @@
 //
 // The item list is made on the host when the groups change (PrefixGroups) and lives in device memory, so a
 // captured step follows later changes of groups, lengths and tables.
-#include "../include/launch.h"
-#include "../include/sharing.h"
-#include "../include/sm100.cuh"
-#include "../include/tma_host.h"
+#include "attn_shared.cuh"
 
 namespace mesh {
 namespace shared_attn {
+namespace {
 
 constexpr int STAGES = 3;
-constexpr int SLICE = 16;                   // keys per slice (one TMA box row block)
-constexpr int KEYS = 64;                    // keys per stage
-constexpr int MAX_ROWS = SHARED_MAX_ROWS;   // query rows per item
-constexpr int HDR = SHARED_HDR, ITEM = SHARED_ITEM;
-constexpr uint64_t WAIT_NS = 2000000000ull;
-
-// meta layout: header | per sequence: prefix length, first partial slot, slots per row, prefix slots per row |
-// member lists | items {first member, offset of the members, first row, rows, KV head, first key, end key, slot}
-struct Args : SharedAttnArgs {
-  int slices_per_page;
-  float scale_log2;
-};
-
-__device__ __forceinline__ int seq_prefix(const Args& a, int b) { return a.meta[HDR + b]; }
-__device__ __forceinline__ int seq_base(const Args& a, int b) { return a.meta[HDR + a.B + b]; }
-__device__ __forceinline__ int seq_slots(const Args& a, int b) { return a.meta[HDR + 2 * a.B + b]; }
-__device__ __forceinline__ int seq_prefix_slots(const Args& a, int b) { return a.meta[HDR + 3 * a.B + b]; }
-__device__ __forceinline__ const int* members(const Args& a) { return a.meta + HDR + 4 * a.B; }
-__device__ __forceinline__ const int* items(const Args& a) { return a.meta + HDR + 5 * a.B; }
+constexpr int KEYS = 64;  // keys per stage
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -71,10 +51,11 @@ struct Geo {
   static constexpr size_t smem() { return 1024 + STAGES * STAGE_BYTES + MAX_ROWS * Q_LD * 2 + 2 * STAGES * 8; }
 };
 
-// One item: up to 64 rows against keys [k0, k1) of one table row. With at most 16 rows the four warps split the
-// keys (a 16-key slice each, merged at the end); otherwise each warp owns 16 rows and walks all four slices of a stage.
+// The rows of one sequence and KV head (new tokens x heads of the group, at most 64) against a range of the keys
+// behind its shared prefix. With at most 16 rows the four warps split the keys (a 16-key slice each, merged at the
+// end); otherwise each warp owns 16 rows and walks all four slices of a stage. Bound by reading K and V.
 template <int D>
-__global__ void __launch_bounds__(160) partial_kernel(const __grid_constant__ CUtensorMap tmK,
+__global__ void __launch_bounds__(160) own_kernel(const __grid_constant__ CUtensorMap tmK,
                                                       const __grid_constant__ CUtensorMap tmV, const Args a) {
   using g = Geo<D>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -89,33 +70,20 @@ __global__ void __launch_bounds__(160) partial_kernel(const __grid_constant__ CU
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   griddep_launch_dependents();
-  griddep_wait();
-  int table_row, row0, rows, h, k0, k1, slot, moff;
-  const int TG = a.T * a.G;
-  bool own = false;
-  if ((int)blockIdx.x < a.n_prefix) {
-    if ((int)blockIdx.x >= a.meta[0]) return;
-    const int* it = items(a) + (long)blockIdx.x * ITEM;
-    table_row = it[0], moff = it[1], row0 = it[2], rows = it[3], h = it[4], k0 = it[5], k1 = it[6], slot = it[7];
-    k1 = min(k1, a.max_pages * a.page_size);
-  } else {
-    const int x = (int)blockIdx.x - a.n_prefix;
-    const int split = x % a.own_splits, y = x / a.own_splits;
-    h = y % a.hkv;
-    table_row = y / a.hkv;
-    own = true;
-    moff = 0, row0 = 0, rows = TG;
-    const int L = min(a.seq_lens[table_row], a.max_pages * a.page_size);
-    int first = seq_prefix(a, table_row);
-    if (a.window > 0) first = max(first, L - a.T + 1 - a.window);
-    const int n = max(0, L - first);
-    // key ranges start on slice boundaries of the table
-    const int f0 = first / SLICE;
-    const int per = ((first + n + SLICE - 1) / SLICE - f0 + a.own_splits - 1) / a.own_splits;
-    k0 = max(first, (f0 + split * per) * SLICE);
-    k1 = min(L, (f0 + (split + 1) * per) * SLICE);
-    slot = seq_prefix_slots(a, table_row) + split;
-  }
+  // behind a prefix kernel, whose own inputs are complete when it lets this one start, only the end has to wait
+  if (a.n_prefix == 0) griddep_wait();
+  const int split = blockIdx.x % a.own_splits, y = blockIdx.x / a.own_splits;
+  const int h = y % a.hkv, seq = y / a.hkv, hq = a.hkv * a.G, rows = a.T * a.G;
+  const int L = min(a.seq_lens[seq], a.max_pages * a.page_size);
+  int first = seq_prefix(a, seq);
+  if (a.window > 0) first = max(first, L - a.T + 1 - a.window);
+  const int n_keys = max(0, L - first);
+  // key ranges start on slice boundaries of the table
+  const int f0 = first / SLICE;
+  const int per = ((first + n_keys + SLICE - 1) / SLICE - f0 + a.own_splits - 1) / a.own_splits;
+  const int k0 = max(first, (f0 + split * per) * SLICE);
+  const int k1 = min(L, (f0 + (split + 1) * per) * SLICE);
+  const int slot = seq_prefix_slots(a, seq) + split;
   const int s0 = k0 / SLICE;                                   // first slice
   const int ns = k1 > k0 ? (k1 + SLICE - 1) / SLICE - s0 : 0;  // slices
   const int nst = (ns + KEYS / SLICE - 1) / (KEYS / SLICE);
@@ -127,24 +95,18 @@ __global__ void __launch_bounds__(160) partial_kernel(const __grid_constant__ CU
     fence_mbar_init();
   }
   for (int r = threadIdx.x; r < MAX_ROWS; r += blockDim.x) {
-    long sl = -1, qo = 0;
-    int pos = -1;
+    const int t = r / a.G, qh = h * a.G + r % a.G;
+    long sl = -1;
     if (r < rows) {
-      const int x = row0 + r;
-      const int b = own ? table_row : members(a)[moff + x / TG];
-      const int t = (x / a.G) % a.T, qh = h * a.G + x % a.G;
-      const int hq = a.hkv * a.G;
-      pos = a.seq_lens[b] - a.T + t;
-      sl = (long)seq_base(a, b) + (long)(t * hq + qh) * seq_slots(a, b) + slot;
-      if (sl < 0 || sl >= a.slot_cap || slot >= seq_slots(a, b)) {
+      sl = (long)seq_base(a, seq) + (long)(t * hq + qh) * seq_slots(a, seq) + slot;
+      if (sl < 0 || sl >= a.slot_cap || slot >= seq_slots(a, seq)) {
         record_error(a.err, ERR_BAD_ARGUMENT);
         sl = -1;
       }
-      qo = ((long)(b * a.T + t) * hq + qh) * D;
     }
     row_slot[r] = sl;
-    row_pos[r] = pos;
-    row_q[r] = qo;
+    row_pos[r] = r < rows ? L - a.T + t : -1;
+    row_q[r] = ((long)(seq * a.T + t) * hq + qh) * D;
   }
   __syncthreads();
 
@@ -153,7 +115,7 @@ __global__ void __launch_bounds__(160) partial_kernel(const __grid_constant__ CU
       tma_prefetch_desc(&tmK);
       tma_prefetch_desc(&tmV);
       const uint64_t pol = policy_evict_first();
-      const int* bt = a.block_tables + (long)table_row * a.max_pages;
+      const int* bt = a.block_tables + (long)seq * a.max_pages;
       for (int i = 0; i < nst; ++i) {
         const int s = i % STAGES;
         if (!mbar_wait_bounded(&empty[s], ((i / STAGES) & 1) ^ 1, a.err, ERR_MBAR_TIMEOUT_PRODUCER, nullptr, WAIT_NS)) break;
@@ -172,6 +134,7 @@ __global__ void __launch_bounds__(160) partial_kernel(const __grid_constant__ CU
         }
       }
     }
+    if (a.n_prefix != 0) griddep_wait();
     return;
   }
   const bool by_rows = rows > 16;
@@ -293,6 +256,7 @@ __global__ void __launch_bounds__(160) partial_kernel(const __grid_constant__ CU
         *reinterpret_cast<float2*>(a.po + sl * D + x * 8 + (lane & 3) * 2) = make_float2(o[x][2 * j], o[x][2 * j + 1]);
       if ((lane & 3) == 0) a.pml[sl] = make_float2(m[j], l[j]);
     }
+    if (a.n_prefix != 0) griddep_wait();
     return;
   }
   // merge the four warps' keys
@@ -328,6 +292,7 @@ __global__ void __launch_bounds__(160) partial_kernel(const __grid_constant__ CU
     a.po[sl * D + d] = ov;
     if (d == 0) a.pml[sl] = make_float2(M, ls);
   }
+  if (a.n_prefix != 0) griddep_wait();  // this grid is complete only when the prefix grid is
 }
 
 // One warp per row (sequence, token, head): merge its partials in slot order.
@@ -353,6 +318,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const Args a) {
     if (M != -INFINITY)
       for (int i = 0; i < n; ++i) {
         const float2 ml = a.pml[base + i];
+        if (ml.x == -INFINITY) continue;  // nothing seen there, and no output written
         const float f = exp2f(ml.x - M);
         den += ml.y * f;
         const float* p = a.po + (base + i) * D + lane * V;
@@ -368,16 +334,19 @@ __global__ void __launch_bounds__(128) combine_kernel(const Args a) {
   for (int v = 0; v < V; v += 2) *reinterpret_cast<uint32_t*>(dst + v) = pack_bf16x2(acc[v] * inv, acc[v + 1] * inv);
 }
 
+}  // namespace
+
 template <int D>
-cudaError_t launch(const Args& a, cudaStream_t st) {
+static cudaError_t launch(const Args& a, cudaStream_t st) {
   const uint64_t rows = (uint64_t)a.pool_pages * a.hkv * a.page_size;
   const CUtensorMap tk = tma_map_2d_bf16(a.k, D, rows, D, 64, SLICE);
   const CUtensorMap tv = tma_map_2d_bf16(a.v, D, rows, D, 64, SLICE);
-  auto kern = partial_kernel<D>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<D>::smem());
+  cudaError_t e = cudaSuccess;
+  if (a.n_prefix > 0 && (e = launch_prefix<D>(a, tk, tv, st)) != cudaSuccess) return e;
+  auto kern = own_kernel<D>;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<D>::smem());
   if (e != cudaSuccess) return e;
-  const unsigned grid = (unsigned)(a.n_prefix + a.B * a.hkv * a.own_splits);
-  e = launch_k(kern, dim3(grid), dim3(160), Geo<D>::smem(), st, tk, tv, a);
+  e = launch_k(kern, dim3((unsigned)(a.B * a.hkv * a.own_splits)), dim3(160), Geo<D>::smem(), st, tk, tv, a);
   if (e != cudaSuccess) return e;
   const long out_rows = (long)a.B * a.T * a.hkv * a.G;
   return launch_k(combine_kernel<D>, dim3((unsigned)((out_rows + 3) / 4)), dim3(128), 0, st, a);

@@ -40,9 +40,15 @@ constexpr int MAX_DRAFTS = VERIFY_MAX_DRAFTS;
 constexpr int PER_LANE = 8;            // tokens of a unit per lane
 constexpr int UNIT = 32 * PER_LANE;     // tokens whose sum one warp of the resolve kernel makes
 constexpr int MAX_SUMS = 4096;          // chunks of a row, units of a CTA's share
-// Logits per stats thread. 32 where the rows fill the GPU (fewer partials, more loads in flight), 8 where
-// they do not: one session of 5 rows over 128256 tokens then makes 315 CTAs instead of 80.
-constexpr int EPT_MANY = 32, EPT_FEW = 8;
+// Logits per stats thread, by the CTAs that 32 each would make: 8 below two per SM (one session of 5 rows over 128256
+// tokens then makes 315 CTAs instead of 80), 16 below sixteen per SM (33 sessions of 1-8 rows over 32000 tokens: 19.8 us,
+// with 32 each 25.9), else 32, which spreads a CTA's fixed work over more logits (64 sessions of 5 rows over 128256:
+// 77 us, with 16 each 86).
+constexpr int EPT_MANY = 32, EPT_SOME = 16, EPT_FEW = 8;
+inline int logits_per_thread(int64_t rows, int64_t V) {
+  const int64_t ctas = rows * ((V + SNT * EPT_MANY - 1) / (SNT * EPT_MANY));
+  return ctas < 2 * 148 ? EPT_FEW : ctas < 16 * 148 ? EPT_SOME : EPT_MANY;
+}
 
 struct Part {
   float m;    // maximum of the chunk (-inf: no selectable token)
@@ -516,19 +522,24 @@ cudaError_t launch(const VerifyArgs& a, cudaStream_t st) {
   return launch_kc(resolve_kernel<T, Q, VEC>, dim3((unsigned)(a.B * CLUSTER)), dim3(RNT), 0, st, CLUSTER, a, SNT * EPT);
 }
 
-template <typename T, typename Q>
-cudaError_t pick(const VerifyArgs& a, bool few, cudaStream_t st) {
-  if (vectors(a)) return few ? launch<T, Q, EPT_FEW, true>(a, st) : launch<T, Q, EPT_MANY, true>(a, st);
-  return few ? launch<T, Q, EPT_FEW, false>(a, st) : launch<T, Q, EPT_MANY, false>(a, st);
+template <typename T, typename Q, bool VEC>
+cudaError_t pick(const VerifyArgs& a, cudaStream_t st) {
+  switch (logits_per_thread((int64_t)a.B * (a.K + 1), a.V)) {
+    case EPT_FEW: return launch<T, Q, EPT_FEW, VEC>(a, st);
+    case EPT_SOME: return launch<T, Q, EPT_SOME, VEC>(a, st);
+    default: return launch<T, Q, EPT_MANY, VEC>(a, st);
+  }
 }
 
-// Too few chunks of the larger kind for two per SM of a 148-SM GPU: smaller ones.
-bool few_rows(int64_t rows, int64_t V) { return rows * ((V + SNT * EPT_MANY - 1) / (SNT * EPT_MANY)) < 2 * 148; }
+template <typename T, typename Q>
+cudaError_t pick(const VerifyArgs& a, cudaStream_t st) {
+  return vectors(a) ? pick<T, Q, true>(a, st) : pick<T, Q, false>(a, st);
+}
 
 }  // namespace verify
 
 int verify_chunks(int64_t B, int64_t K, int64_t V) {
-  const int64_t c = verify::SNT * (verify::few_rows(B * (K + 1), V) ? verify::EPT_FEW : verify::EPT_MANY);
+  const int64_t c = verify::SNT * verify::logits_per_thread(B * (K + 1), V);
   return (int)((V + c - 1) / c);
 }
 int64_t verify_max_vocab() { return (int64_t)verify::SNT * verify::EPT_FEW * verify::MAX_SUMS; }
@@ -539,9 +550,8 @@ int64_t verify_parts_bytes(int64_t B, int64_t K, int64_t V) {
 cudaError_t launch_verify(const VerifyArgs& a, cudaStream_t st) {
   using namespace verify;
   using bf = __nv_bfloat16;
-  const bool few = few_rows((int64_t)a.B * (a.K + 1), a.V);
-  if (a.logits_bf16) return a.probs_bf16 ? pick<bf, bf>(a, few, st) : pick<bf, float>(a, few, st);
-  return a.probs_bf16 ? pick<float, bf>(a, few, st) : pick<float, float>(a, few, st);
+  if (a.logits_bf16) return a.probs_bf16 ? pick<bf, bf>(a, st) : pick<bf, float>(a, st);
+  return a.probs_bf16 ? pick<float, bf>(a, st) : pick<float, float>(a, st);
 }
 
 }  // namespace mesh

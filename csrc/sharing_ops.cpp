@@ -180,7 +180,7 @@ void attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor
   TORCH_CHECK(T >= 1 && T * G <= SHARED_MAX_ROWS, std::string(what) + ": " + num(T) + " new tokens x " + num(G) +
               " heads of a KV group, at most " + num(SHARED_MAX_ROWS) + " rows");
   TORCH_CHECK(meta.device() == q.device() && meta.scalar_type() == at::kInt && meta.is_contiguous() &&
-                  meta.numel() >= SHARED_HDR + 5 * B + SHARED_ITEM * n_prefix,
+                  meta.numel() >= shared_items_at((int)B) + SHARED_ITEM * n_prefix && (uintptr_t)meta.data_ptr() % 16 == 0,
               what, ": groups of another batch");
   TORCH_CHECK(po.scalar_type() == at::kFloat && pml.scalar_type() == at::kFloat && po.device() == q.device() &&
                   pml.device() == q.device() && po.numel() / D <= pml.numel() / 2,
@@ -209,6 +209,7 @@ void attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor
   a.own_splits = (int)own_splits;
   a.window = (int)window;
   a.slot_cap = po.numel() / D;
+  a.num_sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   a.pool_pages = kcache.size(0);
   C10_CUDA_CHECK(launch_attn_shared(a, (int)D, scale, at::cuda::getCurrentCUDAStream()));
 }

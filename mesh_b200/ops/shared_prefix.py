@@ -13,8 +13,9 @@ import torch
 
 _HDR = 8      # header ints of the device table, [0] = number of prefix items
 _ITEM = 8     # ints per prefix item
-_TILE = 64    # query rows per prefix item
-_KEYS = 64    # key ranges of prefix items are multiples of this
+_ROWS = 64    # query rows of a sequence: new tokens x heads of a KV group
+_TILE = 256   # query rows per prefix item
+_KEYS = 128   # key ranges of prefix items are multiples of this
 
 
 class PrefixGroups:
@@ -32,22 +33,24 @@ class PrefixGroups:
         if hkv < 1 or hq % hkv or head_dim not in (64, 128):
             raise ValueError(f"{hq} query heads over {hkv} KV heads of {head_dim}: need hq % hkv == 0 and head_dim 64 or 128")
         self.group = hq // hkv
-        if q_len * self.group > _TILE:
-            raise ValueError(f"{q_len} new tokens x {self.group} heads per KV head exceed {_TILE} query rows")
+        if q_len * self.group > _ROWS:
+            raise ValueError(f"{q_len} new tokens x {self.group} heads per KV head exceed {_ROWS} query rows")
         self.batch, self.hq, self.hkv, self.head_dim, self.q_len = batch, hq, hkv, head_dim, q_len
         self.device = torch.device(device if device is not None else "cuda")
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         sms = torch.cuda.get_device_properties(self.device).multi_processor_count if self.device.type == "cuda" else 148
-        self._target = 2 * sms
+        self._sms = sms
         # own items of a sequence split over its keys only while (sequence, KV head) pairs leave SMs idle
         self.own_cap = max(1, min(32, (3 * sms + batch * hkv) // (2 * batch * hkv))) if 4 * batch * hkv < 3 * sms else 1
         rows = batch * q_len
-        self.item_cap = self._target + hkv * (-(-rows * self.group // _TILE) + batch)
-        slots = _TILE * self._target + rows * hq * (1 + self.own_cap)
+        # one wave of prefix items, or one for each tile of rows where there are more of those
+        self.item_cap = sms + hkv * (-(-rows * self.group // _TILE) + batch)
+        self._items_at = _HDR + (5 * batch + 3) // 4 * 4
+        slots = _TILE * sms + rows * hq * (1 + self.own_cap)
         self._po = torch.empty(slots * head_dim, dtype=torch.float32, device=self.device)
         self._pml = torch.empty(slots * 2, dtype=torch.float32, device=self.device)
-        self._meta = torch.zeros(_HDR + 5 * batch + _ITEM * self.item_cap, dtype=torch.int32, device=self.device)
+        self._meta = torch.zeros(self._items_at + _ITEM * self.item_cap, dtype=torch.int32, device=self.device)
         self.slot_cap = slots
         self.n_items = 0
         self.set([])
@@ -72,9 +75,13 @@ class PrefixGroups:
         prefix, base, slots, pslots = (meta[_HDR + i * B:_HDR + (i + 1) * B] for i in range(4))
         member = meta[_HDR + 4 * B:_HDR + 5 * B]
         tiles = [-(-len(seqs) * T * G // _TILE) for seqs, _ in groups]
-        # every item takes about the same number of keys, so that all SMs finish together
-        load = sum(t * self.hkv * n for t, (_, n) in zip(tiles, groups))
-        per = max(_KEYS, -(-(-(-load // self._target)) // _KEYS) * _KEYS)
+        # Every item takes the same number of 128-key blocks, the fewest with which the items make one wave: a
+        # block costs the same whether it serves 256 rows (tensor cores) or few (memory).
+        blocks = [-(-n // _KEYS) for _, n in groups]
+        per = max(1, -(-sum(t * self.hkv * k for t, k in zip(tiles, blocks)) // self._sms))
+        while per < max(blocks, default=1) and sum(t * self.hkv * -(-k // per) for t, k in zip(tiles, blocks)) > self._sms:
+            per += 1
+        per *= _KEYS
         items, off = [], 0
         for t, (seqs, n) in zip(tiles, groups):
             splits = -(-n // per)
@@ -98,7 +105,7 @@ class PrefixGroups:
         n_items = sum(len(x) for x in items)
         assert n_items <= self.item_cap and int(per_seq.sum()) <= self.slot_cap, "prefix work list exceeds its workspace"
         if items:
-            meta[_HDR + 5 * B:_HDR + 5 * B + _ITEM * n_items] = np.concatenate(items).reshape(-1)
+            meta[self._items_at:self._items_at + _ITEM * n_items] = np.concatenate(items).reshape(-1)
         meta[0] = n_items
         host = torch.from_numpy(meta)
         if self.device.type == "cuda":
@@ -136,5 +143,5 @@ def attn_shared_prefix(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tens
         splits = groups.own_cap
     ext().attn_shared(q, kcache, vcache, block_tables, seq_lens, groups._meta, groups._po, groups._pml, out,
                       scratch(q.device).err, groups.item_cap if capturing else groups.n_items, splits, scale, window)
-    _count(2)
+    _count(2 + (capturing or groups.n_items > 0))
     return out

@@ -31,6 +31,7 @@ ext_modules = [
             "csrc/sharing_ops.cpp",
             "csrc/kernels/kv_moves.cu",
             "csrc/kernels/attn_shared.cu",
+            "csrc/kernels/attn_shared_tc.cu",
             "csrc/kernels/verify.cu",
         ],
         include_dirs=[os.path.join(ROOT, "csrc", "include")],
