@@ -48,7 +48,7 @@ struct Geo {
   static constexpr uint32_t SLICE_BYTES = 2 * HALVES * BOX; // K halves then V halves
   static constexpr uint32_t STAGE_BYTES = (KEYS / SLICE) * SLICE_BYTES;
   static constexpr int Q_LD = D + 8;
-  static constexpr size_t smem() { return 1024 + STAGES * STAGE_BYTES + MAX_ROWS * Q_LD * 2 + 2 * STAGES * 8; }
+  static constexpr size_t smem(int rows) { return 1024 + STAGES * STAGE_BYTES + 2 * STAGES * 8 + rows * Q_LD * 2; }
 };
 
 // The rows of one sequence and KV head (new tokens x heads of the group, at most 64) against a range of the keys
@@ -60,9 +60,9 @@ __global__ void __launch_bounds__(160) own_kernel(const __grid_constant__ CUtens
   using g = Geo<D>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __nv_bfloat16* q_s = reinterpret_cast<__nv_bfloat16*>(stages + STAGES * g::STAGE_BYTES);
-  uint64_t* full = reinterpret_cast<uint64_t*>(stages + STAGES * g::STAGE_BYTES + MAX_ROWS * g::Q_LD * 2);
+  uint64_t* full = reinterpret_cast<uint64_t*>(stages + STAGES * g::STAGE_BYTES);
   uint64_t* empty = full + STAGES;
+  __nv_bfloat16* q_s = reinterpret_cast<__nv_bfloat16*>(empty + STAGES);  // 16 rows, or 64
   __shared__ float red_m[4][16], red_l[4][16];
   __shared__ long row_slot[MAX_ROWS];  // partial slot of each row
   __shared__ int row_pos[MAX_ROWS];    // key position of each row's token
@@ -295,39 +295,55 @@ __global__ void __launch_bounds__(160) own_kernel(const __grid_constant__ CUtens
   if (a.n_prefix != 0) griddep_wait();  // this grid is complete only when the prefix grid is
 }
 
-// One warp per row (sequence, token, head): merge its partials in slot order.
+// One warp per row (sequence, token, head): merge its partials in slot order. Lane i holds the (m, l) of slot i (of the
+// current 32), so the weights are known before the outputs arrive and eight of those are in flight at a time.
 template <int D>
 __global__ void __launch_bounds__(128) combine_kernel(const Args a) {
-  griddep_launch_dependents();
   griddep_wait();
+  griddep_launch_dependents();
+  constexpr int V = D / 32, U = 8;
   const int lane = threadIdx.x & 31, hq = a.hkv * a.G;
   const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 5);  // (b * T + t) * hq + head
   if (row >= (long)a.B * a.T * hq) return;
   const int b = (int)(row / (a.T * hq));
   const int x = (int)(row - (long)b * a.T * hq);
   const long base = (long)seq_base(a, b) + (long)x * seq_slots(a, b);
-  const int n = seq_prefix_slots(a, b) + a.own_splits;
-  constexpr int V = D / 32;
-  float acc[V] = {};
-  float den = 0.f;
-  if (base >= 0 && base + n <= a.slot_cap) {
-    float M = -INFINITY;
-    for (int i = lane; i < n; i += 32) M = fmaxf(M, a.pml[base + i].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    if (M != -INFINITY)
-      for (int i = 0; i < n; ++i) {
-        const float2 ml = a.pml[base + i];
-        if (ml.x == -INFINITY) continue;  // nothing seen there, and no output written
-        const float f = exp2f(ml.x - M);
-        den += ml.y * f;
-        const float* p = a.po + (base + i) * D + lane * V;
-#pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] += p[v] * f;
-      }
-  } else if (lane == 0) {
-    record_error(a.err, ERR_BAD_ARGUMENT);
+  int n = seq_prefix_slots(a, b) + a.own_splits;
+  if (base < 0 || base + n > a.slot_cap) {
+    if (lane == 0) record_error(a.err, ERR_BAD_ARGUMENT);
+    n = 0;
   }
+  float acc[V] = {}, den = 0.f, M = -INFINITY;
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, a.pml[base + i].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  for (int i0 = 0; i0 < n && M > -INFINITY; i0 += 32) {
+    const float2 ml = i0 + lane < n ? a.pml[base + i0 + lane] : make_float2(-INFINITY, 0.f);
+    const float f = exp2f(ml.x - M);  // 0 for a slot that saw nothing; its output was not written
+    den += ml.x > -INFINITY ? ml.y * f : 0.f;
+    for (int i = i0; i < min(n, i0 + 32); i += U) {
+      float p[U][V], w[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        w[u] = i + u < i0 + 32 ? __shfl_sync(0xffffffffu, f, (i + u) & 31) : 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) p[u][v] = 0.f;
+        if (i + u < n && w[u] > 0.f) {
+          const float* src = a.po + (base + i + u) * D + lane * V;
+          if constexpr (V == 4)
+            *reinterpret_cast<float4*>(p[u]) = *reinterpret_cast<const float4*>(src);
+          else
+            *reinterpret_cast<float2*>(p[u]) = *reinterpret_cast<const float2*>(src);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] = fmaf(p[u][v], w[u], acc[v]);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
   const float inv = den > 0.f ? 1.f / den : 0.f;
   __nv_bfloat16* dst = a.out + row * D + lane * V;
 #pragma unroll
@@ -344,9 +360,11 @@ static cudaError_t launch(const Args& a, cudaStream_t st) {
   cudaError_t e = cudaSuccess;
   if (a.n_prefix > 0 && (e = launch_prefix<D>(a, tk, tv, st)) != cudaSuccess) return e;
   auto kern = own_kernel<D>;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<D>::smem());
+  // up to 16 rows need no more than 16 in shared memory: two CTAs fit an SM
+  const size_t smem = Geo<D>::smem(a.T * a.G <= 16 ? 16 : MAX_ROWS);
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<D>::smem(MAX_ROWS));
   if (e != cudaSuccess) return e;
-  e = launch_k(kern, dim3((unsigned)(a.B * a.hkv * a.own_splits)), dim3(160), Geo<D>::smem(), st, tk, tv, a);
+  e = launch_k(kern, dim3((unsigned)(a.B * a.hkv * a.own_splits)), dim3(160), smem, st, tk, tv, a);
   if (e != cudaSuccess) return e;
   const long out_rows = (long)a.B * a.T * a.hkv * a.G;
   return launch_k(combine_kernel<D>, dim3((unsigned)((out_rows + 3) / 4)), dim3(128), 0, st, a);

@@ -47,9 +47,25 @@ struct Bars {
   int abort;
 };
 
+static_assert(BM * (128 * 4 + 16) <= (NS + Cfg<128>::STAGES) * Cfg<128>::TILE && BM * (64 * 4 + 16) <= (NS + Cfg<64>::STAGES) * Cfg<64>::TILE &&
+                  NS * BM * (128 * 4 + 16) <= (NS + 2 * Cfg<128>::STAGES) * Cfg<128>::TILE,
+              "staged rows fit");
+
 template <int D>
 constexpr size_t smem_bytes() {
-  return 1024 + (NS + 2 * Cfg<D>::STAGES) * Cfg<D>::TILE + BM * 8 + sizeof(Bars<D>);
+  return 1024 + (NS + 2 * Cfg<D>::STAGES) * Cfg<D>::TILE + BM * 8 + NS * BM * 8 + sizeof(Bars<D>);
+}
+
+// One contiguous copy shared -> global (16-byte aligned, a multiple of 16 bytes).
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(reinterpret_cast<uint64_t>(dst)),
+               "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
+}
+// This thread's bulk copies have read their sources (the shared memory may be used again).
+__device__ __forceinline__ void bulk_commit_wait_read() {
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 
 struct Item {
@@ -75,7 +91,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint8_t* k_sm = q_sm + NS * C::TILE;
   uint8_t* v_sm = k_sm + STAGES * C::TILE;
   float2* ml_sm = reinterpret_cast<float2*>(v_sm + STAGES * C::TILE);
-  Bars<D>* bars = reinterpret_cast<Bars<D>*>(ml_sm + BM);
+  long* row_sm = reinterpret_cast<long*>(ml_sm + BM);  // offsets of the query rows, then partial slots
+  Bars<D>* bars = reinterpret_cast<Bars<D>*>(row_sm + NS * BM);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -264,40 +281,46 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int x = (two ? t * BM : 0) + r;  // row of the item
       const bool valid = x < it.rows;
       const int TG = a.T * a.G, hq = a.hkv * a.G;
-      // gather the query rows: 16 bytes per lane, the two tiles by all 256 threads
-      {
-        constexpr int CH = D / 8;
-        const int lt = threadIdx.x - 64;
-        const int rows = two ? 2 * BM : BM;
-        for (int c = lt; c < rows * CH; c += NS * BM) {
-          const int rr = c / CH, ch = c - rr * CH;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (rr < it.rows) {
-            const int y = it.row0 + rr;
-            const int b = members(a)[it.moff + y / TG];
-            const long src = ((long)(b * a.T + (y / a.G) % a.T) * hq + it.h * a.G + y % a.G) * D;
-            v = *reinterpret_cast<const uint4*>(a.q + src + ch * 8);
-          }
-          const int tr = rr & (BM - 1);
-          *reinterpret_cast<uint4*>(q_sm + (rr / BM) * C::TILE + (ch >> 3) * C::ATOM + tr * 128 + (((ch & 7) ^ (tr & 7)) << 4)) = v;
-        }
-        fence_proxy_async();
-        mbar_arrive(&bars->q_full);
-      }
-      long slot = -1;
+      long slot = -1, src = -1;
       int lim = 0, low = 0;  // keys [low, lim) of the range are this row's
       if (valid) {
         const int y = it.row0 + x;
         const int b = members(a)[it.moff + y / TG];
-        const int tok = (y / a.G) % a.T;
+        const int tok = (y / a.G) % a.T, head = it.h * a.G + y % a.G;
         const int pos = a.seq_lens[b] - a.T + tok;
+        src = ((long)(b * a.T + tok) * hq + head) * D;
         lim = min(it.k1, pos + 1);
         low = a.window > 0 ? pos + 1 - a.window : 0;
-        slot = (long)seq_base(a, b) + (long)(tok * hq + it.h * a.G + y % a.G) * seq_slots(a, b) + it.slot;
+        slot = (long)seq_base(a, b) + (long)(tok * hq + head) * seq_slots(a, b) + it.slot;
         if (slot < 0 || slot >= a.slot_cap || it.slot >= seq_slots(a, b)) {
           record_error(a.err, ERR_BAD_ARGUMENT);
           slot = -1;
         }
+      }
+      row_sm[t * BM + r] = src;
+      named_bar_sync(1, NS * BM);
+      // gather the query rows (one tile, or one per stream): a row's 16-byte pieces by consecutive lanes, eight loads
+      // in flight per thread
+      {
+        constexpr int CH = D / 8, U = 8;
+        const int total = (two ? NS * BM : BM) * CH;
+        for (int c0 = threadIdx.x - 64; c0 < total; c0 += U * NS * BM) {
+          uint4 v[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int c = c0 + u * NS * BM;
+            const long from = c < total ? row_sm[c / CH] : -1;
+            v[u] = from >= 0 ? *reinterpret_cast<const uint4*>(a.q + from + (c % CH) * 8) : make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int c = c0 + u * NS * BM, rr = c / CH, ch = c % CH, tr = rr & (BM - 1);
+            if (c < total)
+              *reinterpret_cast<uint4*>(q_sm + (rr / BM) * C::TILE + (ch >> 3) * C::ATOM + tr * 128 + (((ch & 7) ^ (tr & 7)) << 4)) = v[u];
+          }
+        }
+        fence_proxy_async();
+        mbar_arrive(&bars->q_full);
       }
       const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
       const uint32_t s_addr = tmem + lane_off + (uint32_t)(t * BK);
@@ -383,9 +406,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       // one row: 16 columns at a time, 16-byte pieces rotated by the row so that a warp's rows fall on all banks
       auto piece = [&](int p) {
-        return reinterpret_cast<float4*>(k_sm) + r * (D / 4) + ((p + r) & (D / 4 - 1));
+        return reinterpret_cast<float4*>(v_sm) + r * (D / 4) + ((p + r) & (D / 4 - 1));
       };
       const bool merge = !two && nblk > 1;
+      named_bar_sync(1, NS * BM);  // both streams are done with the rings and the query tiles
       if (ok && merge) {
         if (t == 1) {
           if (warp_live) {
@@ -417,6 +441,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         if (slot >= 0) a.pml[slot] = make_float2(mo, l);
         if (any) {
+          // A row is 4 D consecutive bytes in memory but one lane here: it is laid out in shared memory (16 bytes of
+          // padding a row keep the lanes on different banks) and leaves in one bulk copy. 256 rows reach into the V
+          // ring, one stream's 128 end before it, where the other stream's rows wait to be merged.
+          float4* mine = reinterpret_cast<float4*>(q_sm + x * (D * 4 + 16));
 #pragma unroll 1
           for (int c = 0; c < D / 16; ++c) {
             uint32_t ov[16];
@@ -430,8 +458,13 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const float4 w = *piece(c * 4 + p);
                 v = make_float4(v.x * f0 + w.x * f1, v.y * f0 + w.y * f1, v.z * f0 + w.z * f1, v.w * f0 + w.w * f1);
               }
-              if (slot >= 0 && l > 0.f) reinterpret_cast<float4*>(a.po + slot * D)[c * 4 + p] = v;
+              mine[c * 4 + p] = v;
             }
+          }
+          fence_proxy_async();
+          if (slot >= 0 && l > 0.f) {
+            bulk_store(a.po + slot * D, mine, D * 4);
+            bulk_commit_wait_read();
           }
         }
       }
