@@ -64,8 +64,8 @@ void verify_drafts(const at::Tensor& logits, const at::Tensor& ids, const at::Te
                    const c10::optional<at::Tensor>& lens, at::Tensor& parts, at::Tensor& tokens, at::Tensor& accepted,
                    at::Tensor& draft_p);
 void attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor& vcache, const at::Tensor& block_tables,
-                 const at::Tensor& seq_lens, const at::Tensor& meta, at::Tensor& po, at::Tensor& pml, at::Tensor& out,
-                 at::Tensor& err, int64_t n_prefix, int64_t own_splits, double scale, int64_t window);
+                 const at::Tensor& seq_lens, at::Tensor& meta, at::Tensor& po, at::Tensor& pml, at::Tensor& out,
+                 at::Tensor& err, int64_t n_prefix, int64_t own_at, double scale, int64_t window);
 void ar_fused_norm(const at::Tensor& bases, int64_t off_flags, int64_t off_p0, int64_t off_p1, int64_t off_resid,
                    int64_t off_normed, int64_t rank, int64_t world, int64_t T, int64_t H, int64_t parity,
                    const at::Tensor& gamma, double eps, at::Tensor& epoch, at::Tensor& err, int64_t nblocks,

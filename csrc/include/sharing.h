@@ -60,21 +60,22 @@ inline
 #ifdef __CUDACC__
     __host__ __device__
 #endif
-    int shared_items_at(int batch) { return SHARED_HDR + ((5 * batch + 3) & ~3); }  // items start on 16 bytes
-// meta layout: header | per sequence: prefix length, first partial slot, slots per row, prefix slots per row |
-// member lists | items {first member, offset of the members, first row, rows, KV head, first key, end key, slot}
+    int shared_items_at(int batch) { return SHARED_HDR + ((5 * batch + 2 + 3) & ~3); }  // items start on 16 bytes
+constexpr int SHARED_MAX_BATCH = 1024;
+// meta layout: header | per sequence: prefix length, first partial slot, prefix slots per row | member lists |
+// scratch [B + 2] | items {first member, offset of the members, first row, rows, KV head, first key, end key, slot}
 struct SharedAttnArgs {
   const __nv_bfloat16* q;   // [B * T, hq, D]
   const void *k, *v;        // [pages, hkv, page_size, D]
   const int* block_tables;  // [B, max_pages]
   const int* seq_lens;      // [B] keys including the new tokens
-  const int* meta;
+  int* meta;
   float* po;                // partial outputs [slots, D]
   float2* pml;              // partial (m, l) [slots]
   __nv_bfloat16* out;
   int* err;
-  int B, T, G, hkv, max_pages, page_size, n_prefix, own_splits, window, num_sms;
-  long slot_cap, pool_pages;
+  int B, T, G, hkv, max_pages, page_size, n_prefix, window, num_sms;
+  long slot_cap, own_at, pool_pages;  // own_at: first slot of the partials of own keys
 };
 cudaError_t launch_attn_shared(const SharedAttnArgs& a, int head_dim, double scale, cudaStream_t st);
 

@@ -19,8 +19,10 @@ namespace mesh {
 namespace shared_attn {
 namespace {
 
-constexpr int STAGES = 3;
-constexpr int KEYS = 64;  // keys per stage
+constexpr int WARPS = 4;         // workers of a CTA
+constexpr int TILE_ROWS = 16;    // query rows of a worker
+constexpr int PIECE_COST = 2;    // what a piece costs besides its slices, in slices
+constexpr int MIN_QUOTA = 4;     // units (slices and piece costs) a worker takes at least
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -46,290 +48,369 @@ struct Geo {
   static constexpr int HALVES = D / 64;
   static constexpr uint32_t BOX = SLICE * 64 * 2;           // one [16 x 64] box
   static constexpr uint32_t SLICE_BYTES = 2 * HALVES * BOX; // K halves then V halves
-  static constexpr uint32_t STAGE_BYTES = (KEYS / SLICE) * SLICE_BYTES;
-  static constexpr int Q_LD = D + 8;
-  static constexpr size_t smem(int rows) { return 1024 + STAGES * STAGE_BYTES + 2 * STAGES * 8 + rows * Q_LD * 2; }
+  static constexpr int SLOTS = 24 * 1024 / SLICE_BYTES;     // slices in flight per worker: 96 KB per CTA
+  // rings | what is known of each sequence
+  static size_t smem(int B) { return 1024 + WARPS * SLOTS * SLICE_BYTES + 16 * (B + 1); }
 };
 
-// The rows of one sequence and KV head (new tokens x heads of the group, at most 64) against a range of the keys
-// behind its shared prefix. With at most 16 rows the four warps split the keys (a 16-key slice each, merged at the
-// end); otherwise each warp owns 16 rows and walks all four slices of a stage. Bound by reading K and V.
-template <int D>
-__global__ void __launch_bounds__(160) own_kernel(const __grid_constant__ CUtensorMap tmK,
-                                                      const __grid_constant__ CUtensorMap tmV, const Args a) {
-  using g = Geo<D>;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(stages + STAGES * g::STAGE_BYTES);
-  uint64_t* empty = full + STAGES;
-  __nv_bfloat16* q_s = reinterpret_cast<__nv_bfloat16*>(empty + STAGES);  // 16 rows, or 64
-  __shared__ float red_m[4][16], red_l[4][16];
-  __shared__ long row_slot[MAX_ROWS];  // partial slot of each row
-  __shared__ int row_pos[MAX_ROWS];    // key position of each row's token
-  __shared__ long row_q[MAX_ROWS];     // offset of each row in q
+// A sequence's keys behind its shared prefix (and inside the window).
+struct Seq {
+  int before;  // units of the sequences before it, for one KV head and tile of rows
+  int first;   // first key
+  int L;       // end
+  int slots;   // partials of its shared prefix per row
+  __device__ __forceinline__ int slices() const { return L > first ? (L + SLICE - 1) / SLICE - first / SLICE : 0; }
+};
 
+// The keys behind the shared prefixes: 16 rows (new tokens x heads of a KV group) of one sequence against that sequence's
+// own slices of 16 keys. All of them, in the order (sequence, KV head, tile of rows, slice), are cut into equal quotas,
+// one per warp, eight warps an SM: lengths from one token to long ones then keep every SM as busy. A quota is a run of
+// pieces, one for each (sequence, head, tile) it touches; a piece counts as PIECE_COST slices besides its own, about
+// what loading its queries and writing its result take. Piece number = worker + (sequence, head, tile), which no other
+// piece has. A warp works by itself: it requests slices SLOTS ahead (TMA, 128-byte swizzle) and multiplies on m16n8k16
+// fragments, without a barrier between warps; four warps that split each piece and merged it took twice as long
+// (64 sessions of up to 512 keys). Bound by reading K and V. HALF: 1 for up to 8 rows, whose half of the fragments is the
+// only one that counts; else 2.
+template <int D, int HALF>
+__global__ void __launch_bounds__(WARPS * 32, 2) own_kernel(const __grid_constant__ CUtensorMap tmK,
+                                                            const __grid_constant__ CUtensorMap tmV, const Args a) {
+  using g = Geo<D>;
+  constexpr int SLOTS = g::SLOTS;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rows = a.T * a.G, hq = a.hkv * a.G, tiles = (rows + TILE_ROWS - 1) / TILE_ROWS;
+  const int per_seq = a.hkv * tiles;
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = base + warp * SLOTS * g::SLICE_BYTES;
+  Seq* seqs = reinterpret_cast<Seq*>(base + WARPS * SLOTS * g::SLICE_BYTES);  // [B + 1]
+  __shared__ uint64_t bars[WARPS][SLOTS];
+  uint64_t* full = bars[warp];
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < WARPS * SLOTS; ++i) mbar_init(&bars[0][0] + i, 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
   griddep_launch_dependents();
   // behind a prefix kernel, whose own inputs are complete when it lets this one start, only the end has to wait
   if (a.n_prefix == 0) griddep_wait();
-  const int split = blockIdx.x % a.own_splits, y = blockIdx.x / a.own_splits;
-  const int h = y % a.hkv, seq = y / a.hkv, hq = a.hkv * a.G, rows = a.T * a.G;
-  const int L = min(a.seq_lens[seq], a.max_pages * a.page_size);
-  int first = seq_prefix(a, seq);
-  if (a.window > 0) first = max(first, L - a.T + 1 - a.window);
-  const int n_keys = max(0, L - first);
-  // key ranges start on slice boundaries of the table
-  const int f0 = first / SLICE;
-  const int per = ((first + n_keys + SLICE - 1) / SLICE - f0 + a.own_splits - 1) / a.own_splits;
-  const int k0 = max(first, (f0 + split * per) * SLICE);
-  const int k1 = min(L, (f0 + (split + 1) * per) * SLICE);
-  const int slot = seq_prefix_slots(a, seq) + split;
-  const int s0 = k0 / SLICE;                                   // first slice
-  const int ns = k1 > k0 ? (k1 + SLICE - 1) / SLICE - s0 : 0;  // slices
-  const int nst = (ns + KEYS / SLICE - 1) / (KEYS / SLICE);
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 4);
-    }
-    fence_mbar_init();
-  }
-  for (int r = threadIdx.x; r < MAX_ROWS; r += blockDim.x) {
-    const int t = r / a.G, qh = h * a.G + r % a.G;
-    long sl = -1;
-    if (r < rows) {
-      sl = (long)seq_base(a, seq) + (long)(t * hq + qh) * seq_slots(a, seq) + slot;
-      if (sl < 0 || sl >= a.slot_cap || slot >= seq_slots(a, seq)) {
-        record_error(a.err, ERR_BAD_ARGUMENT);
-        sl = -1;
+  // all sequences by the last warp, 32 at a time, with the running number of units
+  if (warp == WARPS - 1) {
+    int run = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      const int b = b0 + lane;
+      Seq q = {0, 0, 0, 0};
+      int n = 0;
+      if (b < a.B) {
+        q.L = min(a.seq_lens[b], a.max_pages * a.page_size);
+        q.first = seq_prefix(a, b);
+        q.slots = seq_prefix_slots(a, b);
+        if (a.window > 0) q.first = max(q.first, q.L - a.T + 1 - a.window);
+        n = q.slices();
+        if (n > 0) n += PIECE_COST;
       }
+      int v = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int w = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += w;
+      }
+      q.before = run + v - n;
+      if (b < a.B) seqs[b] = q;
+      run += __shfl_sync(0xffffffffu, v, 31);
     }
-    row_slot[r] = sl;
-    row_pos[r] = r < rows ? L - a.T + t : -1;
-    row_q[r] = ((long)(seq * a.T + t) * hq + qh) * D;
+    if (lane == 0) seqs[a.B].before = run;
   }
   __syncthreads();
+  const int total = seqs[a.B].before * per_seq, workers = WARPS * (int)gridDim.x;
+  const int quota = max(MIN_QUOTA, (total + workers - 1) / workers);
+  if (blockIdx.x == 0) {  // for the combine kernel
+    for (int b = threadIdx.x; b <= a.B; b += blockDim.x) own_before(a)[b] = seqs[b].before;
+    if (threadIdx.x == 0) own_before(a)[a.B + 1] = quota;
+  }
+  const int worker = warp * (int)gridDim.x + blockIdx.x;  // few workers spread over the SMs
+  const int lo = min(total, worker * quota), hi = min(total, lo + quota);
 
-  if (warp == 4) {
-    if (lane == 0) {
-      tma_prefetch_desc(&tmK);
-      tma_prefetch_desc(&tmV);
-      const uint64_t pol = policy_evict_first();
-      const int* bt = a.block_tables + (long)seq * a.max_pages;
-      for (int i = 0; i < nst; ++i) {
-        const int s = i % STAGES;
-        if (!mbar_wait_bounded(&empty[s], ((i / STAGES) & 1) ^ 1, a.err, ERR_MBAR_TIMEOUT_PRODUCER, nullptr, WAIT_NS)) break;
-        const int n = min(KEYS / SLICE, ns - i * (KEYS / SLICE));
-        mbar_arrive_expect_tx(&full[s], (uint32_t)n * g::SLICE_BYTES);
-        for (int p = 0; p < n; ++p) {
-          const int sl = s0 + i * (KEYS / SLICE) + p;
-          const int pi = sl / a.slices_per_page;
-          const int y = (bt[pi] * a.hkv + h) * a.page_size + (sl - pi * a.slices_per_page) * SLICE;
-          uint8_t* pb = stages + s * g::STAGE_BYTES + p * g::SLICE_BYTES;
-#pragma unroll
-          for (int hf = 0; hf < g::HALVES; ++hf) {
-            tma_load_2d(pb + hf * g::BOX, &tmK, &full[s], hf * 64, y, pol);
-            tma_load_2d(pb + (g::HALVES + hf) * g::BOX, &tmV, &full[s], hf * 64, y, pol);
-          }
-        }
-      }
+  // a walk over the pieces of [lo, hi)
+  struct Piece {
+    int b, u, pos;  // sequence; its (KV head, tile); unit the piece starts at
+    int sl, n;      // first slice of the own ones, slices
+  };
+  auto fit = [&](Piece& p, int r) {  // r: units of (b, u) before pos
+    const int units = seqs[p.b + 1].before - seqs[p.b].before;
+    const int end = min(units, r + hi - p.pos);
+    p.sl = max(r, PIECE_COST) - PIECE_COST;
+    p.n = max(0, end - PIECE_COST - p.sl);
+    p.pos += end - r;  // where the next piece starts
+  };
+  auto begin = [&](Piece& p) {
+    int x = 0, y = a.B - 1;  // last sequence that starts at or before lo
+    while (x < y) {
+      const int mid = (x + y + 1) >> 1;
+      if (seqs[mid].before * per_seq <= lo)
+        x = mid;
+      else
+        y = mid - 1;
     }
-    if (a.n_prefix != 0) griddep_wait();
-    return;
-  }
-  const bool by_rows = rows > 16;
-  for (int i = threadIdx.x; i < (by_rows ? MAX_ROWS : 16) * (D / 8); i += 128) {
-    const int r = i / (D / 8), c = i - r * (D / 8);
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (r < rows) v = *reinterpret_cast<const uint4*>(a.q + row_q[r] + c * 8);
-    *reinterpret_cast<uint4*>(q_s + r * g::Q_LD + c * 8) = v;
-  }
-  named_bar_sync(1, 128);
-  const int wrow = by_rows ? warp * 16 : 0;  // first row of this warp
-  uint32_t qf[D / 16][4];
-#pragma unroll
-  for (int kk = 0; kk < D / 16; ++kk)
-    ldsm_x4(smem_u32(q_s + (wrow + (lane & 15)) * g::Q_LD + kk * 16 + (lane >> 4) * 8), qf[kk]);
-  const int rr[2] = {wrow + (lane >> 2), wrow + (lane >> 2) + 8};
-  int hi[2], lo[2];  // keys this lane's two rows may attend: [lo, hi)
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    hi[j] = rr[j] < rows ? min(k1, row_pos[rr[j]] + 1) : 0;
-    lo[j] = a.window > 0 ? max(k0, row_pos[rr[j]] + 1 - a.window) : k0;
-  }
-  float o[D / 8][4];
-#pragma unroll
-  for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  const bool live = !by_rows || wrow < rows;
-  for (int i = 0; i < nst; ++i) {
-    const int s = i % STAGES;
-    int okw = 1;
-    if (lane == 0) okw = mbar_wait_bounded(&full[s], (i / STAGES) & 1, a.err, ERR_MBAR_TIMEOUT_MMA, nullptr, WAIT_NS);
-    if (!__shfl_sync(0xffffffffu, okw, 0)) break;
-    const int n = min(KEYS / SLICE, ns - i * (KEYS / SLICE));
-    const int p0 = by_rows ? 0 : warp, p1 = !live ? 0 : by_rows ? n : min(n, warp + 1);
-    for (int p = p0; p < p1; ++p) {
-      const int key0 = (s0 + i * (KEYS / SLICE) + p) * SLICE;
-      uint8_t* base = stages + s * g::STAGE_BYTES + p * g::SLICE_BYTES;
-      const uint32_t kb = smem_u32(base), vb = kb + g::HALVES * g::BOX;
-      if (key0 + SLICE > k1) {
-        // keys past the range may hold anything (a page's unused tail): their values must not reach the
-        // products as NaN or infinity times a zero weight
-        for (int c = lane; c < SLICE * g::HALVES * 8; c += 32) {
-          const int r = c / (g::HALVES * 8), x = c - r * (g::HALVES * 8);
-          if (key0 + r >= k1) *reinterpret_cast<uint4*>(base + (g::HALVES + x / 8) * g::BOX + swz(r, x & 7)) = make_uint4(0, 0, 0, 0);
-        }
-        __syncwarp();
+    const int units = seqs[x + 1].before - seqs[x].before, off = lo - seqs[x].before * per_seq;
+    p.b = x;
+    p.u = off / units;
+    p.pos = lo;
+    fit(p, off - p.u * units);
+  };
+  auto next = [&](Piece& p) {  // false behind the last piece
+    do {
+      if (p.pos >= hi) return false;
+      if (++p.u == per_seq) {
+        p.u = 0;
+        do ++p.b;
+        while (seqs[p.b + 1].before == seqs[p.b].before);
       }
-      float sc[2][4];
+      fit(p, 0);
+    } while (p.n == 0);
+    return true;
+  };
+
+  if (lo < hi) {
+    const uint64_t pol = policy_evict_first();
+    // ---- requests: slice i of the walk's current piece goes to slot `rs`
+    Piece rp;
+    begin(rp);
+    bool more = rp.n > 0 || next(rp);
+    int ri = 0, rs = 0, row_y = 0;
+    // rows of the pool that hold the next 32 slices of the piece, one per lane
+    auto look_up = [&]() {
+      const int sl = seqs[rp.b].first / SLICE + rp.sl + ri + lane;
+      row_y = 0;
+      if (ri + lane < rp.n) {
+        const int pi = sl / a.slices_per_page;
+        row_y = (a.block_tables[(long)rp.b * a.max_pages + pi] * a.hkv + rp.u / tiles) * a.page_size +
+                (sl - pi * a.slices_per_page) * SLICE;
+      }
+    };
+    auto request = [&]() {
+      if (!more) return;
+      if ((ri & 31) == 0) look_up();
+      const int y = __shfl_sync(0xffffffffu, row_y, ri & 31);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&full[rs], g::SLICE_BYTES);
+        uint8_t* dst = ring + rs * g::SLICE_BYTES;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; kk += 2) {
-          uint32_t bb[4];
-          ldsm_x4(kb + (kk >> 2) * g::BOX + swz(t * 8 + (lane & 7), (kk & 3) * 2 + (lane >> 3)), bb);
-          mma(sc[t], qf[kk], bb[0], bb[1]);
-          mma(sc[t], qf[kk + 1], bb[2], bb[3]);
+        for (int hf = 0; hf < g::HALVES; ++hf) {
+          tma_load_2d(dst + hf * g::BOX, &tmK, &full[rs], hf * 64, y, pol);
+          tma_load_2d(dst + (g::HALVES + hf) * g::BOX, &tmV, &full[rs], hf * 64, y, pol);
         }
       }
-      float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = key0 + t * 8 + (lane & 3) * 2 + (e & 1), j = e >> 1;
-          sc[t][e] = (key < hi[j] && key >= lo[j]) ? sc[t][e] * a.scale_log2 : -INFINITY;
-          mx[j] = fmaxf(mx[j], sc[t][e]);
-        }
-      float pr[2][4];
+      if (++rs == SLOTS) rs = 0;
+      if (++ri == rp.n) {
+        ri = 0;
+        more = next(rp);
+      }
+    };
+#pragma unroll 1
+    for (int i = 0; i < SLOTS; ++i) request();
+
+    Piece p;
+    begin(p);
+    bool todo = p.n > 0 || next(p), ok = true;
+    int s = 0;
+    uint32_t ph = 0;
+    for (; todo; todo = next(p)) {
+      const Seq q = seqs[p.b];
+      const int h = p.u / tiles, row0 = (p.u - h * tiles) * TILE_ROWS, n_rows = min(TILE_ROWS, rows - row0);
+      const int s0 = q.first / SLICE + p.sl;
+      const int k0 = max(q.first, s0 * SLICE), k1 = min(q.L, (s0 + p.n) * SLICE);
+      // query fragments straight from memory: rows lane / 4 and 8 below it, columns (lane % 4) * 2 and 8 to the right
+      uint32_t qf[D / 16][4];
+      int hi_k[2], lo_k[2];  // keys this lane's two rows may attend: [lo_k, hi_k)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 1));
-        mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 2));
-        const float mn = fmaxf(m[j], mx[j]);
-        const float corr = mn == -INFINITY ? 1.f : exp2f(m[j] - mn);
-        float ps = 0.f;
+        const int r = (lane >> 2) + 8 * j, x = row0 + r, t = x / a.G;
+        const bool valid = j < HALF && r < n_rows;
+        const __nv_bfloat16* src = a.q + ((long)(p.b * a.T + t) * hq + h * a.G + x - t * a.G) * D + (lane & 3) * 2;
+        const int pos = q.L - a.T + t;
+        hi_k[j] = valid ? min(k1, pos + 1) : 0;
+        lo_k[j] = a.window > 0 ? max(k0, pos + 1 - a.window) : k0;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          qf[kk][j] = valid ? *reinterpret_cast<const uint32_t*>(src + kk * 16) : 0u;
+          qf[kk][2 + j] = valid ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8) : 0u;
+        }
+      }
+      float o[D / 8][4];
+#pragma unroll
+      for (int x = 0; x < D / 8; ++x) o[x][0] = o[x][1] = o[x][2] = o[x][3] = 0.f;
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll 1
+      for (int i = 0; i < p.n; ++i) {
+        int w = ok;
+        if (lane == 0 && ok) w = mbar_wait_bounded(&full[s], ph, a.err, ERR_MBAR_TIMEOUT_MMA, nullptr, WAIT_NS);
+        ok = __shfl_sync(0xffffffffu, w, 0) != 0;
+        if (!ok) break;
+        const int key0 = (s0 + i) * SLICE;
+        const uint32_t kb = smem_u32(ring + s * g::SLICE_BYTES), vb = kb + g::HALVES * g::BOX;
+        // Keys past the range may hold anything (a page's unused tail): their values must not reach the products as
+        // NaN or infinity times a zero weight. Clearing them in the fragments costs two masks; clearing them in shared
+        // memory needs a proxy fence, which waited for the loads in flight.
+        uint32_t keep[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int left = k1 - (key0 + x * 8 + (lane & 3) * 2);  // of this lane's two keys
+          keep[x] = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+        }
+        float sc[2][4], sd[2][4];  // two chains of products each
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[t][e] = sd[t][e] = 0.f;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; kk += 2) {
+            uint32_t bb[4];
+            ldsm_x4(kb + (kk >> 2) * g::BOX + swz(t * 8 + (lane & 7), (kk & 3) * 2 + (lane >> 3)), bb);
+            mma(sc[t], qf[kk], bb[0], bb[1]);
+            mma(sd[t], qf[kk + 1], bb[2], bb[3]);
+          }
+        }
+        float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float p = mn == -INFINITY ? 0.f : exp2f(sc[t][2 * j + e] - mn);
-            pr[t][2 * j + e] = p;
-            ps += p;
+          for (int e = 0; e < 2 * HALF; ++e) {
+            const int key = key0 + t * 8 + (lane & 3) * 2 + (e & 1), j = e >> 1;
+            sc[t][e] = (key < hi_k[j] && key >= lo_k[j]) ? (sc[t][e] + sd[t][e]) * a.scale_log2 : -INFINITY;
+            mx[j] = fmaxf(mx[j], sc[t][e]);
           }
-        l[j] = l[j] * corr + ps;
-        m[j] = mn;
+        float pr[2][4] = {};
 #pragma unroll
-        for (int x = 0; x < D / 8; ++x) {
-          o[x][2 * j] *= corr;
-          o[x][2 * j + 1] *= corr;
+        for (int j = 0; j < HALF; ++j) {
+          mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 1));
+          mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 2));
+          const float mn = fmaxf(m[j], mx[j]), mb = mn == -INFINITY ? 0.f : mn;
+          const float corr = ex2_ftz(m[j] - mb);
+          float ps = 0.f;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float x = ex2_ftz(sc[t][2 * j + e] - mb);
+              pr[t][2 * j + e] = x;
+              ps += x;
+            }
+          l[j] = l[j] * corr + ps;
+          m[j] = mn;
+#pragma unroll
+          for (int x = 0; x < D / 8; ++x) {
+            o[x][2 * j] *= corr;
+            o[x][2 * j + 1] *= corr;
+          }
+        }
+        // the weights are rounded to bf16 for the product (half a step of 2^-8 each); their sum keeps fp32
+        const uint32_t pa[4] = {pack_bf16x2(pr[0][0], pr[0][1]), pack_bf16x2(pr[0][2], pr[0][3]),
+                                pack_bf16x2(pr[1][0], pr[1][1]), pack_bf16x2(pr[1][2], pr[1][3])};
+#pragma unroll
+        for (int x = 0; x < D / 8; x += 2) {
+          uint32_t bb[4];
+          ldsm_x4_t(vb + (x >> 3) * g::BOX + swz((lane & 7) + ((lane >> 3) & 1) * 8, (x & 7) + (lane >> 4)), bb);
+          mma(o[x], pa, bb[0] & keep[0], bb[1] & keep[1]);
+          mma(o[x + 1], pa, bb[2] & keep[0], bb[3] & keep[1]);
+        }
+        // the products above have taken every fragment of this slot, so it may be filled again
+        __syncwarp();
+        request();
+        if (++s == SLOTS) {
+          s = 0;
+          ph ^= 1;
         }
       }
-      // the weights are rounded to bf16 for the product (half a step of 2^-8 each); their sum keeps fp32
-      const uint32_t pa[4] = {pack_bf16x2(pr[0][0], pr[0][1]), pack_bf16x2(pr[0][2], pr[0][3]),
-                              pack_bf16x2(pr[1][0], pr[1][1]), pack_bf16x2(pr[1][2], pr[1][3])};
 #pragma unroll
-      for (int x = 0; x < D / 8; x += 2) {
-        uint32_t bb[4];
-        ldsm_x4_t(vb + (x >> 3) * g::BOX + swz((lane & 7) + ((lane >> 3) & 1) * 8, (x & 7) + (lane >> 4)), bb);
-        mma(o[x], pa, bb[0], bb[1]);
-        mma(o[x + 1], pa, bb[2], bb[3]);
+      for (int j = 0; j < HALF; ++j) {
+        l[j] += __shfl_xor_sync(0xffffffffu, l[j], 1);
+        l[j] += __shfl_xor_sync(0xffffffffu, l[j], 2);
+      }
+      // a sequence without a prefix whose keys are all in this piece is done: its rows go out; else a partial
+      const bool whole = p.n == q.slices() && q.slots == 0;
+      const int stride = min(rows, TILE_ROWS);
+      const long part = a.own_at + (long)(worker + p.b * per_seq + p.u) * stride;
+      if (part + stride > a.slot_cap) {
+        if (lane == 0) record_error(a.err, ERR_BAD_ARGUMENT);
+        continue;
+      }
+#pragma unroll
+      for (int j = 0; j < HALF; ++j) {
+        const int r = (lane >> 2) + 8 * j;
+        if (r >= n_rows) continue;
+        const int x0 = row0 + r, t = x0 / a.G;
+        __nv_bfloat16* out = a.out + ((long)(p.b * a.T + t) * hq + h * a.G + x0 - t * a.G) * D;
+        const float inv = l[j] > 0.f ? 1.f / l[j] : 0.f;
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x) {
+          const int d = x * 8 + (lane & 3) * 2;
+          if (whole)
+            *reinterpret_cast<uint32_t*>(out + d) = pack_bf16x2(o[x][2 * j] * inv, o[x][2 * j + 1] * inv);
+          else
+            *reinterpret_cast<float2*>(a.po + (part + r) * D + d) = make_float2(o[x][2 * j], o[x][2 * j + 1]);
+        }
+        if (!whole && (lane & 3) == 0) a.pml[part + r] = make_float2(m[j], l[j]);
       }
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[s]);
-  }
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    l[j] += __shfl_xor_sync(0xffffffffu, l[j], 1);
-    l[j] += __shfl_xor_sync(0xffffffffu, l[j], 2);
-  }
-  if (by_rows) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const long sl = row_slot[rr[j]];
-      if (sl < 0) continue;
-#pragma unroll
-      for (int x = 0; x < D / 8; ++x)
-        *reinterpret_cast<float2*>(a.po + sl * D + x * 8 + (lane & 3) * 2) = make_float2(o[x][2 * j], o[x][2 * j + 1]);
-      if ((lane & 3) == 0) a.pml[sl] = make_float2(m[j], l[j]);
-    }
-    if (a.n_prefix != 0) griddep_wait();
-    return;
-  }
-  // merge the four warps' keys
-  if ((lane & 3) == 0)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      red_m[warp][rr[j]] = m[j];
-      red_l[warp][rr[j]] = l[j];
-    }
-  named_bar_sync(1, 128);  // every warp has left the ring
-  float* o_s = reinterpret_cast<float*>(stages);  // [4][16][D]
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-#pragma unroll
-    for (int x = 0; x < D / 8; ++x)
-      *reinterpret_cast<float2*>(o_s + (warp * 16 + rr[j]) * D + x * 8 + (lane & 3) * 2) = make_float2(o[x][2 * j], o[x][2 * j + 1]);
-  named_bar_sync(1, 128);
-  for (int i = threadIdx.x; i < rows * D; i += 128) {
-    const int r = i / D, d = i - r * D;
-    const long sl = row_slot[r];
-    if (sl < 0) continue;
-    float M = -INFINITY, ls = 0.f, ov = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, red_m[w][r]);
-    if (M != -INFINITY) {
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float f = exp2f(red_m[w][r] - M);
-        ls += red_l[w][r] * f;
-        ov += o_s[(w * 16 + r) * D + d] * f;
+    if (!ok) {
+      // the copies still in flight land before the warp goes (bounded)
+      const uint64_t t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 50000000ull) {
       }
     }
-    a.po[sl * D + d] = ov;
-    if (d == 0) a.pml[sl] = make_float2(M, ls);
   }
   if (a.n_prefix != 0) griddep_wait();  // this grid is complete only when the prefix grid is
 }
 
-// One warp per row (sequence, token, head): merge its partials in slot order. Lane i holds the (m, l) of slot i (of the
-// current 32), so the weights are known before the outputs arrive and eight of those are in flight at a time.
+// One warp per row (sequence, token, head): merge its partials, the prefix's first, in order. Lane i holds the (m, l) of
+// partial i (of the current 32), so the weights are known before the outputs arrive and eight of those are in flight
+// at a time.
 template <int D>
 __global__ void __launch_bounds__(128) combine_kernel(const Args a) {
   griddep_wait();
   griddep_launch_dependents();
   constexpr int V = D / 32, U = 8;
-  const int lane = threadIdx.x & 31, hq = a.hkv * a.G;
+  const int lane = threadIdx.x & 31, hq = a.hkv * a.G, rows = a.T * a.G;
   const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 5);  // (b * T + t) * hq + head
   if (row >= (long)a.B * a.T * hq) return;
   const int b = (int)(row / (a.T * hq));
-  const int x = (int)(row - (long)b * a.T * hq);
-  const long base = (long)seq_base(a, b) + (long)x * seq_slots(a, b);
-  int n = seq_prefix_slots(a, b) + a.own_splits;
-  if (base < 0 || base + n > a.slot_cap) {
+  const int x = (int)(row - (long)b * a.T * hq), t = x / hq, head = x - t * hq, h = head / a.G;
+  const int before = own_before(a)[b], units = own_before(a)[b + 1] - before, quota = own_before(a)[a.B + 1];
+  int n_prefix = seq_prefix_slots(a, b);
+  const long base = (long)seq_base(a, b) + (long)x * n_prefix;
+  // the workers whose quotas this row's slices fall into
+  const int r = t * a.G + (head - h * a.G), tile = r / TILE_ROWS, tiles = (rows + TILE_ROWS - 1) / TILE_ROWS;
+  const int u = h * tiles + tile, stride = min(rows, TILE_ROWS);
+  const int at = before * a.hkv * tiles + u * units + PIECE_COST;  // its first slice
+  const int w0 = at / quota;
+  int n_own = units > 0 ? (at + units - PIECE_COST - 1) / quota - w0 + 1 : 0;
+  if (n_prefix == 0 && n_own == 1) return;  // already written
+  const long own = a.own_at + (long)(w0 + b * a.hkv * tiles + u) * stride + (r - tile * TILE_ROWS);  // pieces are `stride` apart
+  if (base < 0 || base + n_prefix > a.own_at || (n_own > 0 && own + (long)(n_own - 1) * stride >= a.slot_cap)) {
     if (lane == 0) record_error(a.err, ERR_BAD_ARGUMENT);
-    n = 0;
+    n_prefix = n_own = 0;
   }
+  const int n = n_prefix + n_own;
+  auto slot = [&](int i) { return i < n_prefix ? base + i : own + (long)(i - n_prefix) * stride; };
   float acc[V] = {}, den = 0.f, M = -INFINITY;
-  for (int i = lane; i < n; i += 32) M = fmaxf(M, a.pml[base + i].x);
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, a.pml[slot(i)].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   for (int i0 = 0; i0 < n && M > -INFINITY; i0 += 32) {
-    const float2 ml = i0 + lane < n ? a.pml[base + i0 + lane] : make_float2(-INFINITY, 0.f);
-    const float f = exp2f(ml.x - M);  // 0 for a slot that saw nothing; its output was not written
+    const float2 ml = i0 + lane < n ? a.pml[slot(i0 + lane)] : make_float2(-INFINITY, 0.f);
+    const float f = ex2_ftz(ml.x - M);  // 0 for a partial that saw nothing; its output may not have been written
     den += ml.x > -INFINITY ? ml.y * f : 0.f;
     for (int i = i0; i < min(n, i0 + 32); i += U) {
       float p[U][V], w[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        w[u] = i + u < i0 + 32 ? __shfl_sync(0xffffffffu, f, (i + u) & 31) : 0.f;
+        w[u] = __shfl_sync(0xffffffffu, f, (i + u) & 31);
 #pragma unroll
         for (int v = 0; v < V; ++v) p[u][v] = 0.f;
         if (i + u < n && w[u] > 0.f) {
-          const float* src = a.po + (base + i + u) * D + lane * V;
+          const float* src = a.po + slot(i + u) * D + lane * V;
           if constexpr (V == 4)
             *reinterpret_cast<float4*>(p[u]) = *reinterpret_cast<const float4*>(src);
           else
@@ -359,12 +440,10 @@ static cudaError_t launch(const Args& a, cudaStream_t st) {
   const CUtensorMap tv = tma_map_2d_bf16(a.v, D, rows, D, 64, SLICE);
   cudaError_t e = cudaSuccess;
   if (a.n_prefix > 0 && (e = launch_prefix<D>(a, tk, tv, st)) != cudaSuccess) return e;
-  auto kern = own_kernel<D>;
-  // up to 16 rows need no more than 16 in shared memory: two CTAs fit an SM
-  const size_t smem = Geo<D>::smem(a.T * a.G <= 16 ? 16 : MAX_ROWS);
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<D>::smem(MAX_ROWS));
+  auto kern = a.T * a.G <= 8 ? own_kernel<D, 1> : own_kernel<D, 2>;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<D>::smem(SHARED_MAX_BATCH));
   if (e != cudaSuccess) return e;
-  e = launch_k(kern, dim3((unsigned)(a.B * a.hkv * a.own_splits)), dim3(160), smem, st, tk, tv, a);
+  e = launch_k(kern, dim3((unsigned)(2 * a.num_sms)), dim3(WARPS * 32), Geo<D>::smem(a.B), st, tk, tv, a);
   if (e != cudaSuccess) return e;
   const long out_rows = (long)a.B * a.T * a.hkv * a.G;
   return launch_k(combine_kernel<D>, dim3((unsigned)((out_rows + 3) / 4)), dim3(128), 0, st, a);

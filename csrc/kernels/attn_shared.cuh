@@ -20,9 +20,10 @@ struct Args : SharedAttnArgs {
 
 __device__ __forceinline__ int seq_prefix(const Args& a, int b) { return a.meta[HDR + b]; }
 __device__ __forceinline__ int seq_base(const Args& a, int b) { return a.meta[HDR + a.B + b]; }
-__device__ __forceinline__ int seq_slots(const Args& a, int b) { return a.meta[HDR + 2 * a.B + b]; }
-__device__ __forceinline__ int seq_prefix_slots(const Args& a, int b) { return a.meta[HDR + 3 * a.B + b]; }
-__device__ __forceinline__ const int* members(const Args& a) { return a.meta + HDR + 4 * a.B; }
+__device__ __forceinline__ int seq_prefix_slots(const Args& a, int b) { return a.meta[HDR + 2 * a.B + b]; }
+__device__ __forceinline__ const int* members(const Args& a) { return a.meta + HDR + 3 * a.B; }
+// slices of the keys behind the prefixes: those before each sequence [B + 1], then a CTA's quota; written by own_kernel
+__device__ __forceinline__ int* own_before(const Args& a) { return a.meta + HDR + 4 * a.B; }
 __device__ __forceinline__ const int* items(const Args& a) { return a.meta + shared_items_at(a.B); }
 
 // rows of a prefix item against its shared keys on tcgen05 (attn_shared_tc.cu)

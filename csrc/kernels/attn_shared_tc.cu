@@ -291,8 +291,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         src = ((long)(b * a.T + tok) * hq + head) * D;
         lim = min(it.k1, pos + 1);
         low = a.window > 0 ? pos + 1 - a.window : 0;
-        slot = (long)seq_base(a, b) + (long)(tok * hq + head) * seq_slots(a, b) + it.slot;
-        if (slot < 0 || slot >= a.slot_cap || it.slot >= seq_slots(a, b)) {
+        slot = (long)seq_base(a, b) + (long)(tok * hq + head) * seq_prefix_slots(a, b) + it.slot;
+        if (slot < 0 || slot >= a.own_at || it.slot >= seq_prefix_slots(a, b)) {
           record_error(a.err, ERR_BAD_ARGUMENT);
           slot = -1;
         }

@@ -4,6 +4,7 @@
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <algorithm>
 #include <climits>
 #include <string>
 
@@ -156,8 +157,8 @@ void verify_drafts(const at::Tensor& logits, const at::Tensor& ids, const at::Te
 }
 
 void attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor& vcache, const at::Tensor& block_tables,
-                 const at::Tensor& seq_lens, const at::Tensor& meta, at::Tensor& po, at::Tensor& pml, at::Tensor& out,
-                 at::Tensor& err, int64_t n_prefix, int64_t own_splits, double scale, int64_t window) {
+                 const at::Tensor& seq_lens, at::Tensor& meta, at::Tensor& po, at::Tensor& pml, at::Tensor& out,
+                 at::Tensor& err, int64_t n_prefix, int64_t own_at, double scale, int64_t window) {
   const char* what = "attn_shared_prefix";
   TORCH_CHECK(q.is_cuda() && q.scalar_type() == at::kBFloat16 && q.is_contiguous() && q.dim() == 2, what,
               ": q contiguous bf16 [B * T, hq * D] on a GPU");
@@ -185,6 +186,10 @@ void attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor
   TORCH_CHECK(po.scalar_type() == at::kFloat && pml.scalar_type() == at::kFloat && po.device() == q.device() &&
                   pml.device() == q.device() && po.numel() / D <= pml.numel() / 2,
               what, ": workspace");
+  TORCH_CHECK(B <= SHARED_MAX_BATCH, std::string(what) + ": a batch of " + num(B) + ", at most " + num(SHARED_MAX_BATCH));
+  const int64_t own_slots = (8 * at::cuda::getDeviceProperties(q.get_device())->multiProcessorCount + B * hkv * ((T * G + 15) / 16)) *
+                            std::min<int64_t>(16, T * G);
+  TORCH_CHECK(own_at >= 0 && (own_at + own_slots) * D <= po.numel(), what, ": workspace too small");
   TORCH_CHECK(kcache.size(0) * hkv * ps < (1ll << 31), what, ": KV pool too large for 32-bit TMA rows");
   TORCH_CHECK(block_tables.size(1) * ps < (1ll << 31), what, ": block tables too wide");
   const c10::cuda::CUDAGuard guard(q.device());
@@ -206,7 +211,7 @@ void attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor
   a.max_pages = (int)block_tables.size(1);
   a.page_size = (int)ps;
   a.n_prefix = (int)n_prefix;
-  a.own_splits = (int)own_splits;
+  a.own_at = own_at;
   a.window = (int)window;
   a.slot_cap = po.numel() / D;
   a.num_sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;

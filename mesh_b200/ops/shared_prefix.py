@@ -15,6 +15,7 @@ _HDR = 8      # header ints of the device table, [0] = number of prefix items
 _ITEM = 8     # ints per prefix item
 _ROWS = 64    # query rows of a sequence: new tokens x heads of a KV group
 _TILE = 256   # query rows per prefix item
+_MAX_BATCH = 1024
 _KEYS = 128   # key ranges of prefix items are multiples of this
 
 
@@ -28,8 +29,8 @@ class PrefixGroups:
     replay at the same time, need one each)."""
 
     def __init__(self, batch: int, hq: int, hkv: int, head_dim: int, q_len: int = 1, device=None):
-        if batch < 1 or q_len < 1:
-            raise ValueError("PrefixGroups needs at least one sequence and one new token each")
+        if not 1 <= batch <= _MAX_BATCH or q_len < 1:
+            raise ValueError(f"PrefixGroups serves 1 to {_MAX_BATCH} sequences and at least one new token each, got {batch} x {q_len}")
         if hkv < 1 or hq % hkv or head_dim not in (64, 128):
             raise ValueError(f"{hq} query heads over {hkv} KV heads of {head_dim}: need hq % hkv == 0 and head_dim 64 or 128")
         self.group = hq // hkv
@@ -41,17 +42,18 @@ class PrefixGroups:
             self.device = torch.device("cuda", torch.cuda.current_device())
         sms = torch.cuda.get_device_properties(self.device).multi_processor_count if self.device.type == "cuda" else 148
         self._sms = sms
-        # own items of a sequence split over its keys only while (sequence, KV head) pairs leave SMs idle
-        self.own_cap = max(1, min(32, (3 * sms + batch * hkv) // (2 * batch * hkv))) if 4 * batch * hkv < 3 * sms else 1
         rows = batch * q_len
         # one wave of prefix items, or one for each tile of rows where there are more of those
         self.item_cap = sms + hkv * (-(-rows * self.group // _TILE) + batch)
-        self._items_at = _HDR + (5 * batch + 3) // 4 * 4
-        slots = _TILE * sms + rows * hq * (1 + self.own_cap)
+        self._items_at = _HDR + (5 * batch + 2 + 3) // 4 * 4
+        # partial rows: of the prefix items (full ones, and one more wave for tiles that are not), then of the pieces
+        # that the keys behind the prefixes are cut into
+        self._own_at = _TILE * sms + rows * hq
+        own_rows = q_len * self.group
+        slots = self._own_at + (8 * sms + batch * hkv * -(-own_rows // 16)) * min(16, own_rows)
         self._po = torch.empty(slots * head_dim, dtype=torch.float32, device=self.device)
         self._pml = torch.empty(slots * 2, dtype=torch.float32, device=self.device)
         self._meta = torch.zeros(self._items_at + _ITEM * self.item_cap, dtype=torch.int32, device=self.device)
-        self.slot_cap = slots
         self.n_items = 0
         self.set([])
 
@@ -72,8 +74,7 @@ class PrefixGroups:
                 seen.add(int(b))
         groups = [([int(b) for b in seqs], int(n)) for seqs, n in groups if len(seqs) and n > 0]
         meta = np.zeros(self._meta.shape[0], dtype=np.int32)
-        prefix, base, slots, pslots = (meta[_HDR + i * B:_HDR + (i + 1) * B] for i in range(4))
-        member = meta[_HDR + 4 * B:_HDR + 5 * B]
+        prefix, base, slots, member = (meta[_HDR + i * B:_HDR + (i + 1) * B] for i in range(4))
         tiles = [-(-len(seqs) * T * G // _TILE) for seqs, _ in groups]
         # Every item takes the same number of 128-key blocks, the fewest with which the items make one wave: a
         # block costs the same whether it serves 256 rows (tensor cores) or few (memory).
@@ -88,7 +89,7 @@ class PrefixGroups:
             size = -(-(-(-n // splits)) // _KEYS) * _KEYS
             splits = -(-n // size)
             member[off:off + len(seqs)] = seqs
-            prefix[seqs], pslots[seqs] = n, splits
+            prefix[seqs], slots[seqs] = n, splits
             rows = len(seqs) * T * G
             h, i, s = np.meshgrid(np.arange(self.hkv), np.arange(t), np.arange(splits), indexing="ij")
             one = np.zeros((h.size, _ITEM), dtype=np.int32)
@@ -99,11 +100,10 @@ class PrefixGroups:
             one[:, 6], one[:, 7] = np.minimum(n, one[:, 5] + size), s.reshape(-1)
             items.append(one)
             off += len(seqs)
-        slots[:] = pslots + self.own_cap
         per_seq = slots.astype(np.int64) * (T * self.hq)
         base[:] = np.concatenate([[0], np.cumsum(per_seq)[:-1]])
         n_items = sum(len(x) for x in items)
-        assert n_items <= self.item_cap and int(per_seq.sum()) <= self.slot_cap, "prefix work list exceeds its workspace"
+        assert n_items <= self.item_cap and int(per_seq.sum()) <= self._own_at, "prefix work list exceeds its workspace"
         if items:
             meta[self._items_at:self._items_at + _ITEM * n_items] = np.concatenate(items).reshape(-1)
         meta[0] = n_items
@@ -114,19 +114,17 @@ class PrefixGroups:
         else:
             self._meta.copy_(host)
         self.n_items = n_items
-        self.min_prefix = min((n for _, n in groups), default=0) if len(seen) == B else 0
         return self
 
 
 def attn_shared_prefix(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_tables: torch.Tensor,
-                       seq_lens: torch.Tensor, groups: PrefixGroups, out: torch.Tensor, scale: float, window: int = 0,
-                       max_len_hint: int = 0) -> torch.Tensor:
+                       seq_lens: torch.Tensor, groups: PrefixGroups, out: torch.Tensor, scale: float,
+                       window: int = 0) -> torch.Tensor:
     """Causal paged GQA attention of the ``q_len`` newest tokens of every sequence, the shared prefixes of
     ``groups`` read once per group. q, out [B * q_len, hq * D] bf16 (the tokens of a sequence together);
     kcache, vcache [pages, hkv, page, D] bf16 (pages of a multiple of 16 tokens); block_tables [B, pages] and
     seq_lens [B] int32 as in ``attn_decode``, lengths including the new tokens. A token without any key gives
-    zeros. ``window``: attend the last ``window`` keys only. ``max_len_hint``: longest sequence (default: what
-    the tables can hold)."""
+    zeros. ``window``: attend the last ``window`` keys only."""
     from . import _count, ext, scratch
     B, T = groups.batch, groups.q_len
     if seq_lens.shape[0] != B or q.shape[0] != B * T or q.shape[1] != groups.hq * groups.head_dim:
@@ -136,12 +134,8 @@ def attn_shared_prefix(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tens
         raise ValueError(f"cache {tuple(kcache.shape)} does not fit groups of {groups.hkv} KV heads of {groups.head_dim}")
     if groups.device != q.device:
         raise ValueError(f"groups on {groups.device}, q on {q.device}")
-    own = max(1, (max_len_hint or block_tables.shape[1] * kcache.shape[2]) - groups.min_prefix)
-    splits = min(groups.own_cap, max(1, own // 128))
     capturing = torch.cuda.is_current_stream_capturing()
-    if capturing:
-        splits = groups.own_cap
     ext().attn_shared(q, kcache, vcache, block_tables, seq_lens, groups._meta, groups._po, groups._pml, out,
-                      scratch(q.device).err, groups.item_cap if capturing else groups.n_items, splits, scale, window)
+                      scratch(q.device).err, groups.item_cap if capturing else groups.n_items, groups._own_at, scale, window)
     _count(2 + (capturing or groups.n_items > 0))
     return out
