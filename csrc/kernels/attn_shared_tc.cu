@@ -1,19 +1,17 @@
 // Shared prefixes on the 5th-generation tensor cores (sm_100a): the rows of all sequences of a group (sequence, new
 // token, head of one KV group) against the keys they share, split over the keys so that one wave of CTAs takes it.
 //
-// An item is up to 256 rows x a range of keys, walked in blocks of 128 keys by two streams of 128 rows x 128 keys that
-// keep the tensor cores busy in turn: while one stream's softmax runs, the other's products do.
-//   more than 128 rows   stream t takes rows 128 t .. of every block, so each block serves 256 rows: 16.8 MFLOP for
-//                        64 KB, where tensor cores (11.6 TFLOP/s an SM) and HBM (43 GB/s an SM) take the same 1.5 us;
-//   at most 128          stream t takes every other block with the same rows; bound by reading the keys. The streams'
-//                        results are merged in shared memory at the end.
+// An item is up to 256 rows x a range of keys, in two streams of 128 rows that walk the keys in blocks of 64. 64 keys for
+// 256 rows are 8.4 MFLOP and 32 KB: tensor cores (11.6 TFLOP/s an SM) and HBM (43 GB/s an SM) take the same 0.73 us.
 // Roles (320 threads): warp 0 loads K and V (16-key slices of pages, [16 x 64] boxes, 128-byte swizzle) into separate
 // rings, so a K block makes room as soon as its scores are done; warp 1 issues tcgen05.mma (one thread): S = Q K^T into
 // TMEM, then O += P V with the bf16 weights P read from TMEM (over the first half of S) and V read MN-major from the page
 // layout; warps 2..5 and 6..9 run the softmax of stream 0 and 1, a row per thread, and gather the query rows, which lie
-// wherever their sequences do. The running maximum only moves (and O is rescaled in TMEM) when it grows by more than
-// 2^8; sum and output share it, so the result stays exact.
-// TMEM columns (512): S0 [0,128) S1 [128,256) O0 [256,256+D) O1 [384,384+D).
+// wherever their sequences do. A stream has two score buffers: the scores of a block are made while the softmax
+// of the one before runs, which therefore never waits for a product (with one buffer and blocks of 128 the way from
+// weights to the next scores, 1.5 us, stood beside 1.1 us of softmax). The running maximum only moves (and O is rescaled in
+// TMEM) when it grows by more than 2^8; sum and output share it, so the result stays exact.
+// TMEM columns (512): S of stream t, buffer b at t * 128 + b * 64; O_t at 256 + t * 128.
 // Every wait is bounded; on a timeout an error is recorded, copies and products in flight are drained, TMEM is freed.
 #include "attn_shared.cuh"
 
@@ -21,51 +19,39 @@ namespace mesh {
 namespace shared_attn {
 namespace {
 
-constexpr int BM = 128, BK = 128, NS = 2;  // rows and keys of a stream's block, streams
+constexpr int BM = 128, BK = 64, NS = 2;  // rows and keys of a stream's block, streams
 constexpr int SLICES = BK / SLICE;
 constexpr int THREADS = 64 + NS * BM;
 constexpr uint32_t TMEM_COLS = 512;
-constexpr uint32_t O_COL = NS * BK;
+constexpr uint32_t S_COLS = 128, O_COL = NS * S_COLS, O_COLS = 128;
 constexpr float RESCALE = 8.0f;  // log2 units
 
 template <int D>
 struct Cfg {
   static constexpr int HALVES = D / 64;
-  static constexpr uint32_t ATOM = BM * 128;           // 128 rows x 64 elements
-  static constexpr uint32_t TILE = HALVES * ATOM;      // 128 rows x D
-  static constexpr int STAGES = 2 * (128 / D);         // blocks of K, and of V: 128 KB of rings
+  static constexpr uint32_t Q_ATOM = BM * 128;            // 128 rows x 64 elements
+  static constexpr uint32_t Q_TILE = HALVES * Q_ATOM;     // 128 rows x D
+  static constexpr uint32_t ATOM = BK * 128;              // 64 keys x 64 elements
+  static constexpr uint32_t TILE = HALVES * ATOM;         // 64 keys x D
+  static constexpr int STAGES = 4 * (128 / D);            // blocks of K, and of V: 128 KB of rings
   static constexpr uint32_t BOX = SLICE * 128;
+  static constexpr int STAGED = D * 4 + 16;               // a row of the result on its way out: padded against bank conflicts
 };
 
 template <int D>
 struct Bars {
   uint64_t q_full;
   uint64_t k_full[Cfg<D>::STAGES], v_full[Cfg<D>::STAGES], k_empty[Cfg<D>::STAGES], v_empty[Cfg<D>::STAGES];
-  uint64_t s_full[NS], p_full[NS], o_done[NS];
+  uint64_t s_full[NS][2], p_full[NS][2], o_done[NS];
   uint64_t mma_done;
   uint32_t tmem_base;
   int abort;
 };
 
-static_assert(BM * (128 * 4 + 16) <= (NS + Cfg<128>::STAGES) * Cfg<128>::TILE && BM * (64 * 4 + 16) <= (NS + Cfg<64>::STAGES) * Cfg<64>::TILE &&
-                  NS * BM * (128 * 4 + 16) <= (NS + 2 * Cfg<128>::STAGES) * Cfg<128>::TILE,
-              "staged rows fit");
-
 template <int D>
 constexpr size_t smem_bytes() {
-  return 1024 + (NS + 2 * Cfg<D>::STAGES) * Cfg<D>::TILE + BM * 8 + NS * BM * 8 + sizeof(Bars<D>);
-}
-
-// One contiguous copy shared -> global (16-byte aligned, a multiple of 16 bytes).
-__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(reinterpret_cast<uint64_t>(dst)),
-               "r"(smem_u32(src)), "r"(bytes)
-               : "memory");
-}
-// This thread's bulk copies have read their sources (the shared memory may be used again).
-__device__ __forceinline__ void bulk_commit_wait_read() {
-  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  static_assert(NS * BM * Cfg<D>::STAGED <= NS * Cfg<D>::Q_TILE + 2 * Cfg<D>::STAGES * Cfg<D>::TILE, "staged rows fit");
+  return 1024 + NS * Cfg<D>::Q_TILE + 2 * Cfg<D>::STAGES * Cfg<D>::TILE + sizeof(Bars<D>);
 }
 
 struct Item {
@@ -77,7 +63,7 @@ struct Item {
     h = y.x, k0 = y.y, k1 = min(y.z, a.max_pages * a.page_size), slot = y.w;
   }
   __device__ __forceinline__ int blocks() const { return k1 > k0 ? (k1 - k0 + BK - 1) / BK : 0; }
-  __device__ __forceinline__ bool two_tiles() const { return rows > BM; }
+  __device__ __forceinline__ int streams() const { return rows > BM ? 2 : 1; }
 };
 
 template <int D>
@@ -88,11 +74,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* q_sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
-  uint8_t* k_sm = q_sm + NS * C::TILE;
+  uint8_t* k_sm = q_sm + NS * C::Q_TILE;
   uint8_t* v_sm = k_sm + STAGES * C::TILE;
-  float2* ml_sm = reinterpret_cast<float2*>(v_sm + STAGES * C::TILE);
-  long* row_sm = reinterpret_cast<long*>(ml_sm + BM);  // offsets of the query rows, then partial slots
-  Bars<D>* bars = reinterpret_cast<Bars<D>*>(row_sm + NS * BM);
+  Bars<D>* bars = reinterpret_cast<Bars<D>*>(v_sm + STAGES * C::TILE);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -104,8 +88,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&bars->v_empty[i], 1);
     }
     for (int t = 0; t < NS; ++t) {
-      mbar_init(&bars->s_full[t], 1);
-      mbar_init(&bars->p_full[t], BM);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&bars->s_full[t][b], 1);
+        mbar_init(&bars->p_full[t][b], BM);
+      }
       mbar_init(&bars->o_done[t], 1);
     }
     mbar_init(&bars->mma_done, 1);
@@ -123,19 +109,29 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
   volatile int* abort_flag = &bars->abort;
+  // The items and members are written by the host alone, never by a kernel that this grid may overlap.
+  const int n_items = min(a.meta[0], a.n_prefix);
+  const int TG = a.T * a.G, hq = a.hkv * a.G;
+  // softmax threads: stream, TMEM lane (a warp may access those of warp % 4 only), row of the item
+  const int st = (warp - 2) >> 2, r = (warp & 3) * 32 + lane, x = st * BM + r;
+  int first_b = 0;
+  if (warp >= 2 && (int)blockIdx.x < n_items) {
+    const Item it(a, blockIdx.x);
+    if (x < it.rows) first_b = members(a)[it.moff + (it.row0 + x) / TG];
+  }
   griddep_wait();
   // The kernel of the sequences' own keys needs what precedes this grid (complete now) and, at its end only, this
   // grid's partials: it may start as SMs fall free.
   griddep_launch_dependents();
-  const int n_items = min(a.meta[0], a.n_prefix);
 
-  uint32_t kvc = 0;               // blocks loaded by this CTA (ring position)
-  uint32_t cnt[NS] = {0, 0};      // MMA warp: blocks each stream has gone through; softmax warps: their own in cnt[0]
-  uint32_t ic = 0;                // items
+  uint32_t kvc = 0;  // blocks this CTA has gone through (ring position)
+  uint32_t cnt = 0;  // blocks: of both streams (MMA warp: of stream 0, stream 1 in cnt1), of this stream (softmax)
+  uint32_t cnt1 = 0;
+  uint32_t ic = 0;   // items
   for (int i = blockIdx.x; i < n_items; i += gridDim.x, ++ic) {
     const Item it(a, i);
     const int nblk = it.blocks();
-    const bool two = it.two_tiles();
+    const int ns = it.streams();
     if (warp == 0) {
       // ------------------------------------ TMA producer ------------------------------------
       if (lane == 0) {
@@ -204,28 +200,28 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       auto stage = [&](int j) { return (int)((kvc + j) % STAGES); };
       auto parity = [&](int j) { return ((kvc + j) / STAGES) & 1u; };
-      // scores of block j for stream t; `last` = no other stream reads this K block
-      auto issue_qk = [&](int t, int j, bool last) {
+      // scores of block j for stream t, whose g-th block it is
+      auto issue_qk = [&](int t, int j, uint32_t g) {
         if (lane == 0) {
-          const uint32_t qa = q_addr + (two ? t : 0) * C::TILE, ka = k_addr + stage(j) * C::TILE;
+          const uint32_t qa = q_addr + t * C::Q_TILE, ka = k_addr + stage(j) * C::TILE;
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
-            umma_bf16(tmem + (uint32_t)(t * BK), make_sdesc_sw128(qa + (kk >> 2) * C::ATOM) + 2 * (kk & 3),
+            umma_bf16(tmem + t * S_COLS + (g & 1) * BK, make_sdesc_sw128(qa + (kk >> 2) * C::Q_ATOM) + 2 * (kk & 3),
                       make_sdesc_sw128(ka + (kk >> 2) * C::ATOM) + 2 * (kk & 3), IDESC_QK, kk > 0 ? 1u : 0u);
-          umma_commit(&bars->s_full[t]);
-          if (last) umma_commit(&bars->k_empty[stage(j)]);
+          umma_commit(&bars->s_full[t][g & 1]);
+          if (t == ns - 1) umma_commit(&bars->k_empty[stage(j)]);
         }
         __syncwarp();
       };
-      auto issue_pv = [&](int t, int j, bool first, bool last) {
+      auto issue_pv = [&](int t, int j, uint32_t g) {
         if (lane == 0) {
           const uint32_t va = v_addr + stage(j) * C::TILE;
 #pragma unroll
           for (int kk = 0; kk < BK / 16; ++kk)
-            umma_bf16_ts(tmem + O_COL + (uint32_t)(t * BK), tmem + (uint32_t)(t * BK + kk * 8),
-                         make_sdesc_sw128_mn(va + kk * 2048, C::ATOM, 1024), IDESC_PV, (!first || kk > 0) ? 1u : 0u);
+            umma_bf16_ts(tmem + O_COL + t * O_COLS, tmem + t * S_COLS + (g & 1) * BK + kk * 8,
+                         make_sdesc_sw128_mn(va + kk * 2048, C::ATOM, 1024), IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
           umma_commit(&bars->o_done[t]);
-          if (last) umma_commit(&bars->v_empty[stage(j)]);
+          if (t == ns - 1) umma_commit(&bars->v_empty[stage(j)]);
         }
         __syncwarp();
       };
@@ -243,52 +239,60 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
       };
       bool ok = nblk == 0 || wait(&bars->q_full, ic & 1u);
-      tc_fence_after();
-      // the first scores of both streams
-      for (int t = 0; t < NS && ok; ++t) {
-        const int j = two ? 0 : t;
-        if (j >= nblk) break;
+      // both score buffers of every stream
+      for (int j = 0; j < min(2, nblk) && ok; ++j) {
         ok = wait(&bars->k_full[stage(j)], parity(j));
+        if (!ok) break;
         tc_fence_after();
-        if (ok) issue_qk(t, j, !two || t == NS - 1);
+        issue_qk(0, j, cnt + j);
+        if (ns == 2) issue_qk(1, j, cnt1 + j);
       }
-      const int step = two ? 1 : NS;
       for (int j = 0; j < nblk && ok; ++j) {
         ok = wait(&bars->v_full[stage(j)], parity(j));
         if (!ok) break;
         if (j == nblk - 1) clear_tail(j);
 #pragma unroll
         for (int t = 0; t < NS; ++t) {
-          if (!ok || (!two && t != (j & 1))) continue;
-          ok = wait(&bars->p_full[t], cnt[t] & 1u);  // the softmax wrote P and rescaled O
+          if (t >= ns || !ok) continue;
+          const uint32_t g = (t == 0 ? cnt : cnt1) + j;
+          ok = wait(&bars->p_full[t][g & 1], (g >> 1) & 1u);  // the softmax wrote P and rescaled O
           if (!ok) continue;
           tc_fence_after();
-          issue_pv(t, j, j < step, !two || t == NS - 1);
-          ++cnt[t];
-          if (j + step < nblk) {
+          issue_pv(t, j, g);
+          if (j + 2 < nblk) {
             // these scores overwrite the columns P was in: one thread's products run in the order of issue
-            ok = wait(&bars->k_full[stage(j + step)], parity(j + step));
+            ok = wait(&bars->k_full[stage(j + 2)], parity(j + 2));
             tc_fence_after();
-            if (ok) issue_qk(t, j + step, !two || t == NS - 1);
+            if (ok) issue_qk(t, j + 2, g + 2);
           }
         }
       }
+      cnt += nblk;
+      if (ns == 2) cnt1 += nblk;
     } else {
       // ------------------------------------ softmax (warps 2..9) ------------------------------------
-      const int t = (warp - 2) >> 2;  // stream
-      const int quarter = warp & 3;   // TMEM lanes this warp may access
-      const int r = quarter * 32 + lane;
-      const int x = (two ? t * BM : 0) + r;  // row of the item
+      const int t = st;
       const bool valid = x < it.rows;
-      const int TG = a.T * a.G, hq = a.hkv * a.G;
-      long slot = -1, src = -1;
+      int b = 0;
+      if (valid) b = ic == 0 ? first_b : members(a)[it.moff + (it.row0 + x) / TG];
+      const int y = it.row0 + x, tok = (y / a.G) % a.T, head = it.h * a.G + y % a.G;
+      // this thread's query row into the tile, all its loads in flight at once
+      if (t < ns) {
+        constexpr int CH = D / 8;
+        uint4 v[CH];
+        const uint4* src = reinterpret_cast<const uint4*>(a.q + ((long)(b * a.T + tok) * hq + head) * D);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) v[c] = valid ? src[c] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+          *reinterpret_cast<uint4*>(q_sm + t * C::Q_TILE + (c >> 3) * C::Q_ATOM + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[c];
+        fence_proxy_async();
+      }
+      mbar_arrive(&bars->q_full);
+      long slot = -1;
       int lim = 0, low = 0;  // keys [low, lim) of the range are this row's
       if (valid) {
-        const int y = it.row0 + x;
-        const int b = members(a)[it.moff + y / TG];
-        const int tok = (y / a.G) % a.T, head = it.h * a.G + y % a.G;
         const int pos = a.seq_lens[b] - a.T + tok;
-        src = ((long)(b * a.T + tok) * hq + head) * D;
         lim = min(it.k1, pos + 1);
         low = a.window > 0 ? pos + 1 - a.window : 0;
         slot = (long)seq_base(a, b) + (long)(tok * hq + head) * seq_prefix_slots(a, b) + it.slot;
@@ -297,47 +301,22 @@ __global__ void __launch_bounds__(THREADS, 1)
           slot = -1;
         }
       }
-      row_sm[t * BM + r] = src;
-      named_bar_sync(1, NS * BM);
-      // gather the query rows (one tile, or one per stream): a row's 16-byte pieces by consecutive lanes, eight loads
-      // in flight per thread
-      {
-        constexpr int CH = D / 8, U = 8;
-        const int total = (two ? NS * BM : BM) * CH;
-        for (int c0 = threadIdx.x - 64; c0 < total; c0 += U * NS * BM) {
-          uint4 v[U];
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int c = c0 + u * NS * BM;
-            const long from = c < total ? row_sm[c / CH] : -1;
-            v[u] = from >= 0 ? *reinterpret_cast<const uint4*>(a.q + from + (c % CH) * 8) : make_uint4(0, 0, 0, 0);
-          }
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int c = c0 + u * NS * BM, rr = c / CH, ch = c % CH, tr = rr & (BM - 1);
-            if (c < total)
-              *reinterpret_cast<uint4*>(q_sm + (rr / BM) * C::TILE + (ch >> 3) * C::ATOM + tr * 128 + (((ch & 7) ^ (tr & 7)) << 4)) = v[u];
-          }
-        }
-        fence_proxy_async();
-        mbar_arrive(&bars->q_full);
-      }
-      const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
-      const uint32_t s_addr = tmem + lane_off + (uint32_t)(t * BK);
-      const uint32_t o_addr = tmem + lane_off + O_COL + (uint32_t)(t * BK);
+      const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+      const uint32_t o_addr = tmem + lane_off + O_COL + t * O_COLS;
       const bool warp_live = __any_sync(0xffffffffu, valid);
       float m_used = -INFINITY, l = 0.f;
-      bool ok = true, any = false;
-      for (int j = two ? 0 : t; j < nblk; j += two ? 1 : NS, ++cnt[0]) {
-        int okw = 1;
-        if (lane == 0)
-          okw = mbar_wait_bounded(&bars->s_full[t], cnt[0] & 1u, a.err, ERR_MBAR_TIMEOUT_EPILOGUE, abort_flag, WAIT_NS);
-        if (!__shfl_sync(0xffffffffu, okw, 0)) {
-          ok = false;
-          break;
-        }
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        int w = 1;
+        if (lane == 0) w = mbar_wait_bounded(bar, parity, a.err, ERR_MBAR_TIMEOUT_EPILOGUE, abort_flag, WAIT_NS);
+        return __shfl_sync(0xffffffffu, w, 0) != 0;
+      };
+      for (int j = 0; j < nblk && t < ns; ++j) {
+        const uint32_t g = cnt + j;
+        if (!(ok = wait(&bars->s_full[t][g & 1], (g >> 1) & 1u))) break;
         tc_fence_after();
         if (warp_live) {
+          const uint32_t s_addr = tmem + lane_off + t * S_COLS + (g & 1) * BK;
           uint32_t sv[BK];
 #pragma unroll
           for (int c = 0; c < BK / 16; ++c)
@@ -349,13 +328,12 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int c = 0; c < BK; ++c)
               if (key0 + c >= lim || key0 + c < low) sv[c] = __float_as_uint(-INFINITY);
           }
-          float mx[8];
+          float mx[4];
 #pragma unroll
-          for (int c = 0; c < 8; ++c) mx[c] = __uint_as_float(sv[c]);
+          for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(sv[c]);
 #pragma unroll
-          for (int c = 8; c < BK; ++c) mx[c & 7] = fmaxf(mx[c & 7], __uint_as_float(sv[c]));
-          const float mraw =
-              fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+          for (int c = 4; c < BK; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(sv[c]));
+          const float mraw = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           const float m_new = fmaxf(m_used, mraw * a.scale_log2);
           const bool resc = m_new > m_used + RESCALE;
           float alpha = 1.f;
@@ -379,8 +357,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             tmem_st16(s_addr + (uint32_t)(16 * c), pk);
           }
           l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-          // the product before this block's scores is complete, so O is stable
-          if (any && __any_sync(0xffffffffu, resc)) {
+          if (j > 0 && __any_sync(0xffffffffu, resc)) {
+            // the product before is complete (the one before that was when these scores were): O is stable
+            if (!(ok = wait(&bars->o_done[t], (g - 1) & 1u))) break;
+            tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
               uint32_t ov[16];
@@ -393,83 +373,48 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           tmem_st_wait();
         }
-        any = true;
         tc_fence_before();
-        mbar_arrive(&bars->p_full[t]);
+        mbar_arrive(&bars->p_full[t][g & 1]);
       }
-      if (ok && any) {
-        int okw = 1;
-        if (lane == 0)
-          okw = mbar_wait_bounded(&bars->o_done[t], (cnt[0] - 1) & 1u, a.err, ERR_MBAR_TIMEOUT_EPILOGUE, abort_flag, WAIT_NS);
-        ok = __shfl_sync(0xffffffffu, okw, 0) != 0;
+      if (t < ns) {
+        cnt += nblk;
+        // the last two products, one after the other: the parity alone tells only neighbouring phases apart
+        if (ok && nblk > 1) ok = wait(&bars->o_done[t], (cnt - 2) & 1u);
+        if (ok && nblk > 0) ok = wait(&bars->o_done[t], (cnt - 1) & 1u);
         tc_fence_after();
-      }
-      // one row: 16 columns at a time, 16-byte pieces rotated by the row so that a warp's rows fall on all banks
-      auto piece = [&](int p) {
-        return reinterpret_cast<float4*>(v_sm) + r * (D / 4) + ((p + r) & (D / 4 - 1));
-      };
-      const bool merge = !two && nblk > 1;
-      named_bar_sync(1, NS * BM);  // both streams are done with the rings and the query tiles
-      if (ok && merge) {
-        if (t == 1) {
-          if (warp_live) {
+        named_bar_sync(1, ns * BM);  // every stream is done with the query tiles and the rings
+        if (ok && warp_live) {
+          if (slot >= 0) a.pml[slot] = make_float2(m_used, l);
+          const long to = slot >= 0 && l > 0.f ? slot : -1;
+          if (nblk > 0 && __any_sync(0xffffffffu, to >= 0)) {
+            // A row is one TMEM lane: the warp lays its 32 rows out in shared memory and writes them row by row.
+            uint8_t* rows_sm = q_sm + (x - lane) * C::STAGED;
 #pragma unroll 1
-            for (int c = 0; c < D / 16; ++c) {
-              uint32_t ov[16];
-              tmem_ld16(o_addr + 16 * c, ov);
+            for (int c = 0; c < D / 64; ++c) {
+              uint32_t ov[64];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                tmem_ld16(o_addr + 64 * c + 16 * e, *reinterpret_cast<uint32_t(*)[16]>(&ov[16 * e]));
               tmem_ld_wait_tied(ov);
 #pragma unroll
-              for (int p = 0; p < 4; ++p)
-                *piece(c * 4 + p) = make_float4(__uint_as_float(ov[4 * p]), __uint_as_float(ov[4 * p + 1]),
-                                                __uint_as_float(ov[4 * p + 2]), __uint_as_float(ov[4 * p + 3]));
+              for (int e = 0; e < 16; ++e)
+                *reinterpret_cast<uint4*>(rows_sm + lane * C::STAGED + c * 256 + e * 16) =
+                    make_uint4(ov[4 * e], ov[4 * e + 1], ov[4 * e + 2], ov[4 * e + 3]);
             }
-          }
-          ml_sm[r] = make_float2(m_used, l);
-        }
-      }
-      if (merge) named_bar_sync(1, NS * BM);
-      if (ok && (two || t == 0) && warp_live) {
-        float f0 = 1.f, f1 = 0.f, mo = m_used;
-        if (merge) {
-          const float2 o = ml_sm[r];
-          mo = fmaxf(m_used, o.x);
-          if (mo > -INFINITY) {
-            f0 = ex2_ftz(m_used - mo);
-            f1 = ex2_ftz(o.x - mo);
-          }
-          l = l * f0 + o.y * f1;
-        }
-        if (slot >= 0) a.pml[slot] = make_float2(mo, l);
-        if (any) {
-          // A row is 4 D consecutive bytes in memory but one lane here: it is laid out in shared memory (16 bytes of
-          // padding a row keep the lanes on different banks) and leaves in one bulk copy. 256 rows reach into the V
-          // ring, one stream's 128 end before it, where the other stream's rows wait to be merged.
-          float4* mine = reinterpret_cast<float4*>(q_sm + x * (D * 4 + 16));
-#pragma unroll 1
-          for (int c = 0; c < D / 16; ++c) {
-            uint32_t ov[16];
-            tmem_ld16(o_addr + 16 * c, ov);
-            tmem_ld_wait_tied(ov);
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-              float4 v = make_float4(__uint_as_float(ov[4 * p]), __uint_as_float(ov[4 * p + 1]),
-                                     __uint_as_float(ov[4 * p + 2]), __uint_as_float(ov[4 * p + 3]));
-              if (merge) {
-                const float4 w = *piece(c * 4 + p);
-                v = make_float4(v.x * f0 + w.x * f1, v.y * f0 + w.y * f1, v.z * f0 + w.z * f1, v.w * f0 + w.w * f1);
-              }
-              mine[c * 4 + p] = v;
+            __syncwarp();
+            constexpr int LANES = D / 4, AT_ONCE = 32 / LANES;  // lanes of a row, rows at once
+#pragma unroll 8
+            for (int k = 0; k < 32 / AT_ONCE; ++k) {
+              const int row = k * AT_ONCE + lane / LANES;
+              const long dst = __shfl_sync(0xffffffffu, to, row);
+              const float4 v = *reinterpret_cast<const float4*>(rows_sm + row * C::STAGED + (lane % LANES) * 16);
+              if (dst >= 0) *reinterpret_cast<float4*>(a.po + dst * D + (lane % LANES) * 4) = v;
             }
-          }
-          fence_proxy_async();
-          if (slot >= 0 && l > 0.f) {
-            bulk_store(a.po + slot * D, mine, D * 4);
-            bulk_commit_wait_read();
           }
         }
       }
       tc_fence_before();
-      fence_proxy_async();  // the rings are written by TMA again
+      if (i + (int)gridDim.x < n_items) fence_proxy_async();  // the shared memory is written by TMA again
     }
     kvc += nblk;
     __syncthreads();

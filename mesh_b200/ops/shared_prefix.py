@@ -16,7 +16,7 @@ _ITEM = 8     # ints per prefix item
 _ROWS = 64    # query rows of a sequence: new tokens x heads of a KV group
 _TILE = 256   # query rows per prefix item
 _MAX_BATCH = 1024
-_KEYS = 128   # key ranges of prefix items are multiples of this
+_KEYS = 64    # key ranges of prefix items are multiples of this
 
 
 class PrefixGroups:
@@ -76,7 +76,7 @@ class PrefixGroups:
         meta = np.zeros(self._meta.shape[0], dtype=np.int32)
         prefix, base, slots, member = (meta[_HDR + i * B:_HDR + (i + 1) * B] for i in range(4))
         tiles = [-(-len(seqs) * T * G // _TILE) for seqs, _ in groups]
-        # Every item takes the same number of 128-key blocks, the fewest with which the items make one wave: a
+        # Every item takes the same number of 64-key blocks, the fewest with which the items make one wave: a
         # block costs the same whether it serves 256 rows (tensor cores) or few (memory).
         blocks = [-(-n // _KEYS) for _, n in groups]
         per = max(1, -(-sum(t * self.hkv * k for t, k in zip(tiles, blocks)) // self._sms))
