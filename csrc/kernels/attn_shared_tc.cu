@@ -3,8 +3,9 @@
 //
 // An item is up to 256 rows x a range of keys, in two streams of 128 rows that walk the keys in blocks of 64. 64 keys for
 // 256 rows are 8.4 MFLOP and 32 KB: tensor cores (11.6 TFLOP/s an SM) and HBM (43 GB/s an SM) take the same 0.73 us.
-// Roles (320 threads): warp 0 loads K and V (16-key slices of pages, [16 x 64] boxes, 128-byte swizzle) into separate
-// rings, so a K block makes room as soon as its scores are done; warp 1 issues tcgen05.mma (one thread): S = Q K^T into
+// Roles (352 threads): warp 0 loads K and warp 10 V (16-key slices of pages, [16 x 64] boxes, 128-byte swizzle) into
+// separate rings, so a K block makes room as soon as its scores are done, and because one thread takes 90 ns a box, which
+// alone made a block take 1.5 us; warp 1 issues tcgen05.mma (one thread): S = Q K^T into
 // TMEM, then O += P V with the bf16 weights P read from TMEM (over the first half of S) and V read MN-major from the page
 // layout; warps 2..5 and 6..9 run the softmax of stream 0 and 1, a row per thread, and gather the query rows, which lie
 // wherever their sequences do. A stream has two score buffers: the scores of a block are made while the softmax
@@ -21,7 +22,8 @@ namespace {
 
 constexpr int BM = 128, BK = 64, NS = 2;  // rows and keys of a stream's block, streams
 constexpr int SLICES = BK / SLICE;
-constexpr int THREADS = 64 + NS * BM;
+constexpr int THREADS = 96 + NS * BM;
+constexpr int PRODUCER_V = 10;  // warp
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t S_COLS = 128, O_COL = NS * S_COLS, O_COLS = 128;
 constexpr float RESCALE = 8.0f;  // log2 units
@@ -77,7 +79,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint8_t* k_sm = q_sm + NS * C::Q_TILE;
   uint8_t* v_sm = k_sm + STAGES * C::TILE;
   Bars<D>* bars = reinterpret_cast<Bars<D>*>(v_sm + STAGES * C::TILE);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // broadcast values are known to be the same for the whole warp, so the address arithmetic of the issuing warps stays in
+  // uniform registers (a product took 60 ns to issue otherwise, a TMA box 108 instead of 75)
+  auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, NS * BM);
@@ -107,16 +112,16 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars->tmem_base;
+  const uint32_t tmem = (uint32_t)uniform((int)bars->tmem_base);
   volatile int* abort_flag = &bars->abort;
   // The items and members are written by the host alone, never by a kernel that this grid may overlap.
-  const int n_items = min(a.meta[0], a.n_prefix);
+  const int n_items = uniform(min(a.meta[0], a.n_prefix));
   const int TG = a.T * a.G, hq = a.hkv * a.G;
   // softmax threads: stream, TMEM lane (a warp may access those of warp % 4 only), row of the item
   const int st = (warp - 2) >> 2, r = (warp & 3) * 32 + lane, x = st * BM + r;
   int first_b = 0;
-  if (warp >= 2 && (int)blockIdx.x < n_items) {
-    const Item it(a, blockIdx.x);
+  Item it(a, min((int)blockIdx.x, max(0, n_items - 1)));
+  if (warp >= 2 && warp < PRODUCER_V && (int)blockIdx.x < n_items) {
     if (x < it.rows) first_b = members(a)[it.moff + (it.row0 + x) / TG];
   }
   griddep_wait();
@@ -129,61 +134,50 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint32_t cnt1 = 0;
   uint32_t ic = 0;   // items
   for (int i = blockIdx.x; i < n_items; i += gridDim.x, ++ic) {
-    const Item it(a, i);
-    const int nblk = it.blocks();
-    const int ns = it.streams();
-    if (warp == 0) {
-      // ------------------------------------ TMA producer ------------------------------------
-      if (lane == 0) {
-        const uint64_t pol = policy_evict_last();  // other tiles of rows read the same keys
-        const int* bt = a.block_tables + (long)it.table_row * a.max_pages;
-        bool ok = true;
-        int j = 0;
-        for (; j < nblk && ok; ++j) {
-          const uint32_t c = kvc + j;
-          const int s = c % STAGES;
-          const uint32_t ph = ((c / STAGES) & 1u) ^ 1u;
-          const int key0 = it.k0 + j * BK;
-          const int n = min(SLICES, (it.k1 - key0 + SLICE - 1) / SLICE);
-          int y[SLICES];
-#pragma unroll
-          for (int p = 0; p < SLICES; ++p) {
-            if (p < n) {
-              const int sl = key0 / SLICE + p, pi = sl / a.slices_per_page;
-              y[p] = (bt[pi] * a.hkv + it.h) * a.page_size + (sl - pi * a.slices_per_page) * SLICE;
-            }
+    if (ic > 0) it = Item(a, i);
+    const int nblk = uniform(it.blocks());
+    const int ns = uniform(it.streams());
+    if (warp == 0 || warp == PRODUCER_V) {
+      // ------------------------------------ TMA producers: K, V ------------------------------------
+      const uint64_t pol = policy_evict_first();
+      const int* bt = a.block_tables + (long)it.table_row * a.max_pages;
+      const CUtensorMap* tm = warp == 0 ? &tmK : &tmV;
+      uint8_t* ring = warp == 0 ? k_sm : v_sm;
+      uint64_t* full = warp == 0 ? bars->k_full : bars->v_full;
+      uint64_t* empty = warp == 0 ? bars->k_empty : bars->v_empty;
+      const int first = it.k0 / SLICE, slices = nblk > 0 ? (it.k1 + SLICE - 1) / SLICE - first : 0;
+      int row_y = 0, ok = 1, j = 0;
+      for (; j < nblk && ok; ++j) {
+        if ((j & (32 / SLICES - 1)) == 0) {  // rows of the pool that hold the next 32 slices, one per lane
+          const int c = j * SLICES + lane;
+          if (c < slices) {
+            const int pi = (first + c) / a.slices_per_page;
+            row_y = (bt[pi] * a.hkv + it.h) * a.page_size + (first + c - pi * a.slices_per_page) * SLICE;
           }
-          if (!(ok = mbar_wait_bounded(&bars->k_empty[s], ph, a.err, ERR_MBAR_TIMEOUT_PRODUCER, abort_flag, WAIT_NS))) break;
-          mbar_arrive_expect_tx(&bars->k_full[s], (uint32_t)n * C::HALVES * C::BOX);
-#pragma unroll
-          for (int p = 0; p < SLICES; ++p)
-            if (p < n)
-#pragma unroll
-              for (int hf = 0; hf < C::HALVES; ++hf)
-                tma_load_2d(k_sm + s * C::TILE + hf * C::ATOM + p * C::BOX, &tmK, &bars->k_full[s], hf * 64, y[p], pol);
-          if (!(ok = mbar_wait_bounded(&bars->v_empty[s], ph, a.err, ERR_MBAR_TIMEOUT_PRODUCER, abort_flag, WAIT_NS))) {
-            // the K block just requested lands before the CTA goes on (bounded)
-            const uint64_t t0 = globaltimer_ns();
-            while (!mbar_try_wait(&bars->k_full[s], ph ^ 1u) && globaltimer_ns() - t0 < 50000000ull) {
-            }
-            break;
-          }
-          mbar_arrive_expect_tx(&bars->v_full[s], (uint32_t)n * C::HALVES * C::BOX);
-#pragma unroll
-          for (int p = 0; p < SLICES; ++p)
-            if (p < n)
-#pragma unroll
-              for (int hf = 0; hf < C::HALVES; ++hf)
-                tma_load_2d(v_sm + s * C::TILE + hf * C::ATOM + p * C::BOX, &tmV, &bars->v_full[s], hf * 64, y[p], pol);
         }
-        if (!ok) {
-          const uint64_t t0 = globaltimer_ns();
-          for (int x = max(0, j - STAGES); x < j; ++x) {
-            const uint32_t c = kvc + x;
-            while (!(mbar_try_wait(&bars->k_full[c % STAGES], (c / STAGES) & 1u) &&
-                     mbar_try_wait(&bars->v_full[c % STAGES], (c / STAGES) & 1u)) &&
-                   globaltimer_ns() - t0 < 50000000ull) {
-            }
+        const uint32_t c = kvc + j;
+        const int s = c % STAGES, n = uniform(min(SLICES, slices - j * SLICES));
+        int y[SLICES];
+#pragma unroll
+        for (int p = 0; p < SLICES; ++p) y[p] = __shfl_sync(0xffffffffu, row_y, (j * SLICES + p) & 31);
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], ((c / STAGES) & 1u) ^ 1u, a.err, ERR_MBAR_TIMEOUT_PRODUCER,
+                                                       abort_flag, WAIT_NS));
+        if (ok && elect_one()) {
+          mbar_arrive_expect_tx(&full[s], (uint32_t)n * C::HALVES * C::BOX);
+#pragma unroll
+          for (int p = 0; p < SLICES; ++p)
+            if (p < n)
+#pragma unroll
+              for (int hf = 0; hf < C::HALVES; ++hf)
+                tma_load_2d(ring + s * C::TILE + hf * C::ATOM + p * C::BOX, tm, &full[s], hf * 64, y[p], pol);
+        }
+        __syncwarp();
+      }
+      if (!ok && lane == 0) {  // copies already in flight land before the CTA goes on (bounded)
+        const uint64_t t0 = globaltimer_ns();
+        for (int x = max(0, j - 1 - STAGES); x < j - 1; ++x) {
+          const uint32_t c = kvc + x;
+          while (!mbar_try_wait(&full[c % STAGES], (c / STAGES) & 1u) && globaltimer_ns() - t0 < 50000000ull) {
           }
         }
       }
@@ -192,34 +186,35 @@ __global__ void __launch_bounds__(THREADS, 1)
       // ------------------------------------ MMA issuer ------------------------------------
       constexpr uint32_t IDESC_QK = make_idesc_bf16(BM, BK);
       constexpr uint32_t IDESC_PV = make_idesc_bf16(BM, D) | IDESC_B_MN_MAJOR;
-      const uint32_t q_addr = smem_u32(q_sm), k_addr = smem_u32(k_sm), v_addr = smem_u32(v_sm);
+      // descriptors of the first tile; addresses count in 16 bytes and stay below 2^18, so offsets just add up
+      const uint64_t q_desc = make_sdesc_sw128(smem_u32(q_sm)), k_desc = make_sdesc_sw128(smem_u32(k_sm));
+      const uint64_t v_desc = make_sdesc_sw128_mn(smem_u32(v_sm), C::ATOM, 1024);
       auto wait = [&](uint64_t* bar, uint32_t parity) {
-        int ok = 1;
-        if (lane == 0) ok = mbar_wait_bounded(bar, parity, a.err, ERR_MBAR_TIMEOUT_MMA, abort_flag, WAIT_NS);
-        return __shfl_sync(0xffffffffu, ok, 0) != 0;
+        return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, a.err, ERR_MBAR_TIMEOUT_MMA, abort_flag, WAIT_NS)) != 0;
       };
       auto stage = [&](int j) { return (int)((kvc + j) % STAGES); };
       auto parity = [&](int j) { return ((kvc + j) / STAGES) & 1u; };
       // scores of block j for stream t, whose g-th block it is
       auto issue_qk = [&](int t, int j, uint32_t g) {
-        if (lane == 0) {
-          const uint32_t qa = q_addr + t * C::Q_TILE, ka = k_addr + stage(j) * C::TILE;
+        const uint64_t qd = q_desc + t * (C::Q_TILE >> 4), kd = k_desc + stage(j) * (C::TILE >> 4);
+        const uint32_t st = tmem + t * S_COLS + (g & 1) * BK;
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
-            umma_bf16(tmem + t * S_COLS + (g & 1) * BK, make_sdesc_sw128(qa + (kk >> 2) * C::Q_ATOM) + 2 * (kk & 3),
-                      make_sdesc_sw128(ka + (kk >> 2) * C::ATOM) + 2 * (kk & 3), IDESC_QK, kk > 0 ? 1u : 0u);
+            umma_bf16(st, qd + (kk >> 2) * (C::Q_ATOM >> 4) + 2 * (kk & 3), kd + (kk >> 2) * (C::ATOM >> 4) + 2 * (kk & 3), IDESC_QK,
+                      kk > 0 ? 1u : 0u);
           umma_commit(&bars->s_full[t][g & 1]);
           if (t == ns - 1) umma_commit(&bars->k_empty[stage(j)]);
         }
         __syncwarp();
       };
       auto issue_pv = [&](int t, int j, uint32_t g) {
-        if (lane == 0) {
-          const uint32_t va = v_addr + stage(j) * C::TILE;
+        const uint64_t vd = v_desc + stage(j) * (C::TILE >> 4);
+        const uint32_t ot = tmem + O_COL + t * O_COLS, pt = tmem + t * S_COLS + (g & 1) * BK;
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < BK / 16; ++kk)
-            umma_bf16_ts(tmem + O_COL + t * O_COLS, tmem + t * S_COLS + (g & 1) * BK + kk * 8,
-                         make_sdesc_sw128_mn(va + kk * 2048, C::ATOM, 1024), IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
+            umma_bf16_ts(ot, pt + kk * 8, vd + kk * (2048 >> 4), IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
           umma_commit(&bars->o_done[t]);
           if (t == ns - 1) umma_commit(&bars->v_empty[stage(j)]);
         }
