@@ -3,9 +3,9 @@
 //
 // An item is up to 256 rows x a range of keys, in two streams of 128 rows that walk the keys in blocks of 64. 64 keys for
 // 256 rows are 8.4 MFLOP and 32 KB: tensor cores (11.6 TFLOP/s an SM) and HBM (43 GB/s an SM) take the same 0.73 us.
-// Roles (352 threads): warp 0 loads K and warp 10 V (16-key slices of pages, [16 x 64] boxes, 128-byte swizzle) into
+// Roles (384 threads): warp 0 loads K and warp 10 V (16-key slices of pages, [16 x 64] boxes, 128-byte swizzle) into
 // separate rings, so a K block makes room as soon as its scores are done, and because one thread takes 90 ns a box, which
-// alone made a block take 1.5 us; warp 1 issues tcgen05.mma (one thread): S = Q K^T into
+// alone made a block take 1.5 us; warps 1 and 11 issue tcgen05.mma (one thread each) for stream 0 and 1: S = Q K^T into
 // TMEM, then O += P V with the bf16 weights P read from TMEM (over the first half of S) and V read MN-major from the page
 // layout; warps 2..5 and 6..9 run the softmax of stream 0 and 1, a row per thread, and gather the query rows, which lie
 // wherever their sequences do. A stream has two score buffers: the scores of a block are made while the softmax
@@ -22,8 +22,8 @@ namespace {
 
 constexpr int BM = 128, BK = 64, NS = 2;  // rows and keys of a stream's block, streams
 constexpr int SLICES = BK / SLICE;
-constexpr int THREADS = 96 + NS * BM;
-constexpr int PRODUCER_V = 10;  // warp
+constexpr int THREADS = 128 + NS * BM;
+constexpr int PRODUCER_V = 10, MMA0 = 1, MMA1 = 11;  // warps
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t S_COLS = 128, O_COL = NS * S_COLS, O_COLS = 128;
 constexpr float RESCALE = 8.0f;  // log2 units
@@ -89,8 +89,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&bars->k_full[i], 1);
       mbar_init(&bars->v_full[i], 1);
-      mbar_init(&bars->k_empty[i], 1);
-      mbar_init(&bars->v_empty[i], 1);
+      mbar_init(&bars->k_empty[i], NS);
+      mbar_init(&bars->v_empty[i], NS);
     }
     for (int t = 0; t < NS; ++t) {
       for (int b = 0; b < 2; ++b) {
@@ -99,13 +99,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       mbar_init(&bars->o_done[t], 1);
     }
-    mbar_init(&bars->mma_done, 1);
+    mbar_init(&bars->mma_done, NS);
     bars->abort = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
-  if (warp == 1) {
+  if (warp == MMA0) {
     tmem_alloc(&bars->tmem_base, TMEM_COLS);
     tmem_relinquish();
   }
@@ -130,8 +130,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   griddep_launch_dependents();
 
   uint32_t kvc = 0;  // blocks this CTA has gone through (ring position)
-  uint32_t cnt = 0;  // blocks: of both streams (MMA warp: of stream 0, stream 1 in cnt1), of this stream (softmax)
-  uint32_t cnt1 = 0;
+  uint32_t cnt = 0;  // blocks this warp's stream has gone through (MMA, softmax)
   uint32_t ic = 0;   // items
   for (int i = blockIdx.x; i < n_items; i += gridDim.x, ++ic) {
     if (ic > 0) it = Item(a, i);
@@ -182,8 +181,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       __syncwarp();
-    } else if (warp == 1) {
-      // ------------------------------------ MMA issuer ------------------------------------
+    } else if (warp == MMA0 || warp == MMA1) {
+      // ------------------------------------ MMA issuers: stream 0, 1 ------------------------------------
+      // two, because a wait costs the issuing warp about 200 cycles even when it is over, in which the tensor core runs dry
+      const int t = warp == MMA0 ? 0 : 1;
       constexpr uint32_t IDESC_QK = make_idesc_bf16(BM, BK);
       constexpr uint32_t IDESC_PV = make_idesc_bf16(BM, D) | IDESC_B_MN_MAJOR;
       // descriptors of the first tile; addresses count in 16 bytes and stay below 2^18, so offsets just add up
@@ -194,8 +195,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       auto stage = [&](int j) { return (int)((kvc + j) % STAGES); };
       auto parity = [&](int j) { return ((kvc + j) / STAGES) & 1u; };
-      // scores of block j for stream t, whose g-th block it is
-      auto issue_qk = [&](int t, int j, uint32_t g) {
+      // a block of K or V is free when every stream has given it back
+      auto give_back = [&](uint64_t* bar) {
+        umma_commit(bar);
+        if (ns == 1) umma_commit(bar);
+      };
+      // scores of block j, the stream's g-th
+      auto issue_qk = [&](int j, uint32_t g) {
         const uint64_t qd = q_desc + t * (C::Q_TILE >> 4), kd = k_desc + stage(j) * (C::TILE >> 4);
         const uint32_t st = tmem + t * S_COLS + (g & 1) * BK;
         if (elect_one()) {
@@ -204,11 +210,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             umma_bf16(st, qd + (kk >> 2) * (C::Q_ATOM >> 4) + 2 * (kk & 3), kd + (kk >> 2) * (C::ATOM >> 4) + 2 * (kk & 3), IDESC_QK,
                       kk > 0 ? 1u : 0u);
           umma_commit(&bars->s_full[t][g & 1]);
-          if (t == ns - 1) umma_commit(&bars->k_empty[stage(j)]);
+          give_back(&bars->k_empty[stage(j)]);
         }
         __syncwarp();
       };
-      auto issue_pv = [&](int t, int j, uint32_t g) {
+      auto issue_pv = [&](int j, uint32_t g) {
         const uint64_t vd = v_desc + stage(j) * (C::TILE >> 4);
         const uint32_t ot = tmem + O_COL + t * O_COLS, pt = tmem + t * S_COLS + (g & 1) * BK;
         if (elect_one()) {
@@ -216,7 +222,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int kk = 0; kk < BK / 16; ++kk)
             umma_bf16_ts(ot, pt + kk * 8, vd + kk * (2048 >> 4), IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
           umma_commit(&bars->o_done[t]);
-          if (t == ns - 1) umma_commit(&bars->v_empty[stage(j)]);
+          give_back(&bars->v_empty[stage(j)]);
         }
         __syncwarp();
       };
@@ -234,36 +240,32 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
       };
       bool ok = nblk == 0 || wait(&bars->q_full, ic & 1u);
-      // both score buffers of every stream
-      for (int j = 0; j < min(2, nblk) && ok; ++j) {
-        ok = wait(&bars->k_full[stage(j)], parity(j));
-        if (!ok) break;
-        tc_fence_after();
-        issue_qk(0, j, cnt + j);
-        if (ns == 2) issue_qk(1, j, cnt1 + j);
-      }
-      for (int j = 0; j < nblk && ok; ++j) {
-        ok = wait(&bars->v_full[stage(j)], parity(j));
-        if (!ok) break;
-        if (j == nblk - 1) clear_tail(j);
-#pragma unroll
-        for (int t = 0; t < NS; ++t) {
-          if (t >= ns || !ok) continue;
-          const uint32_t g = (t == 0 ? cnt : cnt1) + j;
-          ok = wait(&bars->p_full[t][g & 1], (g >> 1) & 1u);  // the softmax wrote P and rescaled O
-          if (!ok) continue;
+      if (t < ns) {
+        // both score buffers
+        for (int j = 0; j < min(2, nblk) && ok; ++j) {
+          ok = wait(&bars->k_full[stage(j)], parity(j));
           tc_fence_after();
-          issue_pv(t, j, g);
+          if (ok) issue_qk(j, cnt + j);
+        }
+        for (int j = 0; j < nblk && ok; ++j) {
+          const uint32_t g = cnt + j;
+          // V of this block, the softmax's P (and its rescaling of O), K of the next scores
+          ok = wait(&bars->v_full[stage(j)], parity(j));
+          if (!ok) break;
+          if (j == nblk - 1) clear_tail(j);
+          ok = wait(&bars->p_full[t][g & 1], (g >> 1) & 1u);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(j, g);
           if (j + 2 < nblk) {
             // these scores overwrite the columns P was in: one thread's products run in the order of issue
             ok = wait(&bars->k_full[stage(j + 2)], parity(j + 2));
             tc_fence_after();
-            if (ok) issue_qk(t, j + 2, g + 2);
+            if (ok) issue_qk(j + 2, g + 2);
           }
         }
+        cnt += nblk;
       }
-      cnt += nblk;
-      if (ns == 2) cnt1 += nblk;
     } else {
       // ------------------------------------ softmax (warps 2..9) ------------------------------------
       const int t = st;
@@ -417,7 +419,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (bars->abort) break;
   }
   // every product issued above has completed before TMEM is released
-  if (warp == 1 && lane == 0) {
+  if ((warp == MMA0 || warp == MMA1) && lane == 0) {
     umma_commit(&bars->mma_done);
     const uint64_t t0 = globaltimer_ns();
     while (!mbar_try_wait(&bars->mma_done, 0) && globaltimer_ns() - t0 < 50000000ull) {
@@ -426,7 +428,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, TMEM_COLS);
+  if (warp == MMA0) tmem_dealloc(tmem, TMEM_COLS);
 }
 
 }  // namespace
