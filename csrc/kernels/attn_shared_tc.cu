@@ -14,7 +14,7 @@
 // TMEM) when it grows by more than 2^8; sum and output share it, so the result stays exact.
 // TMEM columns (512): S of stream t, buffer b at t * 128 + b * 64; O_t at 256 + t * 128.
 // Every wait is bounded; on a timeout an error is recorded, copies and products in flight are drained, TMEM is freed.
-#include "attn_shared.cuh"
+#include "attn_shared_own.cuh"
 
 namespace mesh {
 namespace shared_attn {
@@ -22,8 +22,9 @@ namespace {
 
 constexpr int BM = 128, BK = 64, NS = 2;  // rows and keys of a stream's block, streams
 constexpr int SLICES = BK / SLICE;
-constexpr int THREADS = 128 + NS * BM;
-constexpr int PRODUCER_V = 10, MMA0 = 1, MMA1 = 11;  // warps
+constexpr int P_THREADS = 128 + NS * BM;             // of the prefix items
+constexpr int THREADS = P_THREADS + WARPS * 32;       // and of the sequences' own keys
+constexpr int PRODUCER_V = 10, MMA0 = 1, MMA1 = 11, OWN = 12;  // warps
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t S_COLS = 128, O_COL = NS * S_COLS, O_COLS = 128;
 constexpr float RESCALE = 8.0f;  // log2 units
@@ -35,7 +36,8 @@ struct Cfg {
   static constexpr uint32_t Q_TILE = HALVES * Q_ATOM;     // 128 rows x D
   static constexpr uint32_t ATOM = BK * 128;              // 64 keys x 64 elements
   static constexpr uint32_t TILE = HALVES * ATOM;         // 64 keys x D
-  static constexpr int STAGES = 4 * (128 / D);            // blocks of K, and of V: 128 KB of rings
+  // blocks of K and of V in flight: 80 KB of rings, beside 64 KB of those of the sequences' own keys
+  static constexpr int K_STAGES = 3 * (128 / D), V_STAGES = 2 * (128 / D);
   static constexpr uint32_t BOX = SLICE * 128;
   static constexpr int STAGED = D * 4 + 16;               // a row of the result on its way out: padded against bank conflicts
 };
@@ -43,17 +45,19 @@ struct Cfg {
 template <int D>
 struct Bars {
   uint64_t q_full;
-  uint64_t k_full[Cfg<D>::STAGES], v_full[Cfg<D>::STAGES], k_empty[Cfg<D>::STAGES], v_empty[Cfg<D>::STAGES];
+  uint64_t k_full[Cfg<D>::K_STAGES], k_empty[Cfg<D>::K_STAGES], v_full[Cfg<D>::V_STAGES], v_empty[Cfg<D>::V_STAGES];
   uint64_t s_full[NS][2], p_full[NS][2], o_done[NS];
   uint64_t mma_done;
+  uint64_t own_full[WARPS][Geo<D>::SLOTS];
   uint32_t tmem_base;
   int abort;
 };
 
 template <int D>
-constexpr size_t smem_bytes() {
-  static_assert(NS * BM * Cfg<D>::STAGED <= NS * Cfg<D>::Q_TILE + 2 * Cfg<D>::STAGES * Cfg<D>::TILE, "staged rows fit");
-  return 1024 + NS * Cfg<D>::Q_TILE + 2 * Cfg<D>::STAGES * Cfg<D>::TILE + sizeof(Bars<D>);
+constexpr size_t smem_bytes(int B) {
+  static_assert(NS * BM * Cfg<D>::STAGED <= NS * Cfg<D>::Q_TILE + (Cfg<D>::K_STAGES + Cfg<D>::V_STAGES) * Cfg<D>::TILE, "staged rows fit");
+  return 1024 + NS * Cfg<D>::Q_TILE + (Cfg<D>::K_STAGES + Cfg<D>::V_STAGES) * Cfg<D>::TILE + sizeof(Bars<D>) +
+         WARPS * Geo<D>::SLOTS * Geo<D>::SLICE_BYTES + 16 * (B + 1);
 }
 
 struct Item {
@@ -68,17 +72,19 @@ struct Item {
   __device__ __forceinline__ int streams() const { return rows > BM ? 2 : 1; }
 };
 
-template <int D>
+template <int D, int HALF>
 __global__ void __launch_bounds__(THREADS, 1)
     prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Args a) {
   using C = Cfg<D>;
-  constexpr int STAGES = C::STAGES;
+  constexpr int K_STAGES = C::K_STAGES, V_STAGES = C::V_STAGES;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* q_sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   uint8_t* k_sm = q_sm + NS * C::Q_TILE;
-  uint8_t* v_sm = k_sm + STAGES * C::TILE;
-  Bars<D>* bars = reinterpret_cast<Bars<D>*>(v_sm + STAGES * C::TILE);
+  uint8_t* v_sm = k_sm + K_STAGES * C::TILE;
+  uint8_t* own_sm = v_sm + V_STAGES * C::TILE;
+  Seq* seqs = reinterpret_cast<Seq*>(own_sm + WARPS * Geo<D>::SLOTS * Geo<D>::SLICE_BYTES);  // [B + 1]
+  Bars<D>* bars = reinterpret_cast<Bars<D>*>(seqs + a.B + 1);
   // broadcast values are known to be the same for the whole warp, so the address arithmetic of the issuing warps stays in
   // uniform registers (a product took 60 ns to issue otherwise, a TMA box 108 instead of 75)
   auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
@@ -86,10 +92,12 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, NS * BM);
-    for (int i = 0; i < STAGES; ++i) {
+    for (int i = 0; i < K_STAGES; ++i) {
       mbar_init(&bars->k_full[i], 1);
-      mbar_init(&bars->v_full[i], 1);
       mbar_init(&bars->k_empty[i], NS);
+    }
+    for (int i = 0; i < V_STAGES; ++i) {
+      mbar_init(&bars->v_full[i], 1);
       mbar_init(&bars->v_empty[i], NS);
     }
     for (int t = 0; t < NS; ++t) {
@@ -100,6 +108,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&bars->o_done[t], 1);
     }
     mbar_init(&bars->mma_done, NS);
+    for (int i = 0; i < WARPS * Geo<D>::SLOTS; ++i) mbar_init(&bars->own_full[0][0] + i, 1);
     bars->abort = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmK);
@@ -125,11 +134,27 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (x < it.rows) first_b = members(a)[it.moff + (it.row0 + x) / TG];
   }
   griddep_wait();
-  // The kernel of the sequences' own keys needs what precedes this grid (complete now) and, at its end only, this
-  // grid's partials: it may start as SMs fall free.
   griddep_launch_dependents();
+  if (warp >= OWN) {
+    // The sequences' own keys, read beside the products: these warps wait for memory while the others keep the tensor
+    // cores busy (as a kernel of its own behind this one, 64 sessions behind 8k took 42 us).
+    if (warp == OWN) own_sequences(a, seqs, lane);
+    named_bar_sync(2, WARPS * 32);
+    const int w = warp - OWN;
+    own_worker<D, HALF>(tmK, tmV, a, seqs, own_sm + w * Geo<D>::SLOTS * Geo<D>::SLICE_BYTES, bars->own_full[w], lane,
+                        w * (int)gridDim.x + (int)blockIdx.x, WARPS * (int)gridDim.x);
+    return;
+  }
 
-  uint32_t kvc = 0;  // blocks this CTA has gone through (ring position)
+  // ring positions of this warp's role: the next block of K (MMA: to score; producer of K) and of V
+  int pos = 0, v_pos = 0;
+  uint32_t phase = 0, v_phase = 0;
+  auto advance = [](int& at, uint32_t& ph, int stages) {
+    if (++at == stages) {
+      at = 0;
+      ph ^= 1u;
+    }
+  };
   uint32_t cnt = 0;  // blocks this warp's stream has gone through (MMA, softmax)
   uint32_t ic = 0;   // items
   for (int i = blockIdx.x; i < n_items; i += gridDim.x, ++ic) {
@@ -144,6 +169,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint8_t* ring = warp == 0 ? k_sm : v_sm;
       uint64_t* full = warp == 0 ? bars->k_full : bars->v_full;
       uint64_t* empty = warp == 0 ? bars->k_empty : bars->v_empty;
+      const int stages = warp == 0 ? K_STAGES : V_STAGES;
       const int first = it.k0 / SLICE, slices = nblk > 0 ? (it.k1 + SLICE - 1) / SLICE - first : 0;
       int row_y = 0, ok = 1, j = 0;
       for (; j < nblk && ok; ++j) {
@@ -154,12 +180,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             row_y = (bt[pi] * a.hkv + it.h) * a.page_size + (first + c - pi * a.slices_per_page) * SLICE;
           }
         }
-        const uint32_t c = kvc + j;
-        const int s = c % STAGES, n = uniform(min(SLICES, slices - j * SLICES));
+        const int s = pos, n = uniform(min(SLICES, slices - j * SLICES));
         int y[SLICES];
 #pragma unroll
         for (int p = 0; p < SLICES; ++p) y[p] = __shfl_sync(0xffffffffu, row_y, (j * SLICES + p) & 31);
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], ((c / STAGES) & 1u) ^ 1u, a.err, ERR_MBAR_TIMEOUT_PRODUCER,
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], phase ^ 1u, a.err, ERR_MBAR_TIMEOUT_PRODUCER,
                                                        abort_flag, WAIT_NS));
         if (ok && elect_one()) {
           mbar_arrive_expect_tx(&full[s], (uint32_t)n * C::HALVES * C::BOX);
@@ -171,13 +196,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                 tma_load_2d(ring + s * C::TILE + hf * C::ATOM + p * C::BOX, tm, &full[s], hf * 64, y[p], pol);
         }
         __syncwarp();
+        if (ok) advance(pos, phase, stages);
       }
       if (!ok && lane == 0) {  // copies already in flight land before the CTA goes on (bounded)
         const uint64_t t0 = globaltimer_ns();
-        for (int x = max(0, j - 1 - STAGES); x < j - 1; ++x) {
-          const uint32_t c = kvc + x;
-          while (!mbar_try_wait(&full[c % STAGES], (c / STAGES) & 1u) && globaltimer_ns() - t0 < 50000000ull) {
-          }
+        while (globaltimer_ns() - t0 < 1000000ull) {
         }
       }
       __syncwarp();
@@ -193,16 +216,14 @@ __global__ void __launch_bounds__(THREADS, 1)
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, a.err, ERR_MBAR_TIMEOUT_MMA, abort_flag, WAIT_NS)) != 0;
       };
-      auto stage = [&](int j) { return (int)((kvc + j) % STAGES); };
-      auto parity = [&](int j) { return ((kvc + j) / STAGES) & 1u; };
       // a block of K or V is free when every stream has given it back
       auto give_back = [&](uint64_t* bar) {
         umma_commit(bar);
         if (ns == 1) umma_commit(bar);
       };
-      // scores of block j, the stream's g-th
-      auto issue_qk = [&](int j, uint32_t g) {
-        const uint64_t qd = q_desc + t * (C::Q_TILE >> 4), kd = k_desc + stage(j) * (C::TILE >> 4);
+      // scores of the next block of K, the stream's g-th
+      auto issue_qk = [&](uint32_t g) {
+        const uint64_t qd = q_desc + t * (C::Q_TILE >> 4), kd = k_desc + pos * (C::TILE >> 4);
         const uint32_t st = tmem + t * S_COLS + (g & 1) * BK;
         if (elect_one()) {
 #pragma unroll
@@ -210,28 +231,30 @@ __global__ void __launch_bounds__(THREADS, 1)
             umma_bf16(st, qd + (kk >> 2) * (C::Q_ATOM >> 4) + 2 * (kk & 3), kd + (kk >> 2) * (C::ATOM >> 4) + 2 * (kk & 3), IDESC_QK,
                       kk > 0 ? 1u : 0u);
           umma_commit(&bars->s_full[t][g & 1]);
-          give_back(&bars->k_empty[stage(j)]);
+          give_back(&bars->k_empty[pos]);
         }
         __syncwarp();
+        advance(pos, phase, K_STAGES);
       };
       auto issue_pv = [&](int j, uint32_t g) {
-        const uint64_t vd = v_desc + stage(j) * (C::TILE >> 4);
+        const uint64_t vd = v_desc + v_pos * (C::TILE >> 4);
         const uint32_t ot = tmem + O_COL + t * O_COLS, pt = tmem + t * S_COLS + (g & 1) * BK;
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < BK / 16; ++kk)
             umma_bf16_ts(ot, pt + kk * 8, vd + kk * (2048 >> 4), IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
           umma_commit(&bars->o_done[t]);
-          give_back(&bars->v_empty[stage(j)]);
+          give_back(&bars->v_empty[v_pos]);
         }
         __syncwarp();
+        advance(v_pos, v_phase, V_STAGES);
       };
       // V rows past the range (a page's tail, or a slice that was not loaded) may hold anything; a zero weight times
       // NaN would reach the output, so they are cleared
       auto clear_tail = [&](int j) {
         const int valid = it.k1 - (it.k0 + j * BK);
         if (valid >= BK) return;
-        uint8_t* v = v_sm + stage(j) * C::TILE;
+        uint8_t* v = v_sm + v_pos * C::TILE;
         for (int c = lane; c < (BK - valid) * C::HALVES * 8; c += 32) {
           const int r = valid + c / (C::HALVES * 8), x = c % (C::HALVES * 8);
           *reinterpret_cast<uint4*>(v + (x >> 3) * C::ATOM + r * 128 + ((x & 7) << 4)) = make_uint4(0, 0, 0, 0);
@@ -243,14 +266,14 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (t < ns) {
         // both score buffers
         for (int j = 0; j < min(2, nblk) && ok; ++j) {
-          ok = wait(&bars->k_full[stage(j)], parity(j));
+          ok = wait(&bars->k_full[pos], phase);
           tc_fence_after();
-          if (ok) issue_qk(j, cnt + j);
+          if (ok) issue_qk(cnt + j);
         }
         for (int j = 0; j < nblk && ok; ++j) {
           const uint32_t g = cnt + j;
           // V of this block, the softmax's P (and its rescaling of O), K of the next scores
-          ok = wait(&bars->v_full[stage(j)], parity(j));
+          ok = wait(&bars->v_full[v_pos], v_phase);
           if (!ok) break;
           if (j == nblk - 1) clear_tail(j);
           ok = wait(&bars->p_full[t][g & 1], (g >> 1) & 1u);
@@ -259,12 +282,17 @@ __global__ void __launch_bounds__(THREADS, 1)
           issue_pv(j, g);
           if (j + 2 < nblk) {
             // these scores overwrite the columns P was in: one thread's products run in the order of issue
-            ok = wait(&bars->k_full[stage(j + 2)], parity(j + 2));
+            ok = wait(&bars->k_full[pos], phase);
             tc_fence_after();
-            if (ok) issue_qk(j + 2, g + 2);
+            if (ok) issue_qk(g + 2);
           }
         }
         cnt += nblk;
+      } else {  // the ring moves on without this stream
+        for (int j = 0; j < nblk; ++j) {
+          advance(pos, phase, K_STAGES);
+          advance(v_pos, v_phase, V_STAGES);
+        }
       }
     } else {
       // ------------------------------------ softmax (warps 2..9) ------------------------------------
@@ -413,8 +441,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       tc_fence_before();
       if (i + (int)gridDim.x < n_items) fence_proxy_async();  // the shared memory is written by TMA again
     }
-    kvc += nblk;
-    __syncthreads();
+    named_bar_sync(3, P_THREADS);
     tc_fence_after();
     if (bars->abort) break;
   }
@@ -426,7 +453,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   }
   tc_fence_before();
-  __syncthreads();
+  named_bar_sync(3, P_THREADS);
   tc_fence_after();
   if (warp == MMA0) tmem_dealloc(tmem, TMEM_COLS);
 }
@@ -435,10 +462,11 @@ __global__ void __launch_bounds__(THREADS, 1)
 
 template <int D>
 cudaError_t launch_prefix(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
-  auto kern = prefix_kernel<D>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<D>());
+  auto kern = a.T * a.G <= 8 ? prefix_kernel<D, 1> : prefix_kernel<D, 2>;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<D>(SHARED_MAX_BATCH));
   if (e != cudaSuccess) return e;
-  return launch_k(kern, dim3((unsigned)min(a.n_prefix, a.num_sms)), dim3(THREADS), smem_bytes<D>(), st, tk, tv, a);
+  return launch_k(kern, dim3((unsigned)a.num_sms), dim3(THREADS), smem_bytes<D>(a.B), st, tk, tv, a);
 }
 template cudaError_t launch_prefix<64>(const Args&, const CUtensorMap&, const CUtensorMap&, cudaStream_t);
 template cudaError_t launch_prefix<128>(const Args&, const CUtensorMap&, const CUtensorMap&, cudaStream_t);

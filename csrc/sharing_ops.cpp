@@ -187,7 +187,7 @@ void attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor
                   pml.device() == q.device() && po.numel() / D <= pml.numel() / 2,
               what, ": workspace");
   TORCH_CHECK(B <= SHARED_MAX_BATCH, std::string(what) + ": a batch of " + num(B) + ", at most " + num(SHARED_MAX_BATCH));
-  const int64_t own_slots = (8 * at::cuda::getDeviceProperties(q.get_device())->multiProcessorCount + B * hkv * ((T * G + 15) / 16)) *
+  const int64_t own_slots = (12 * at::cuda::getDeviceProperties(q.get_device())->multiProcessorCount + B * hkv * ((T * G + 15) / 16)) *
                             std::min<int64_t>(16, T * G);
   TORCH_CHECK(own_at >= 0 && (own_at + own_slots) * D <= po.numel(), what, ": workspace too small");
   TORCH_CHECK(kcache.size(0) * hkv * ps < (1ll << 31), what, ": KV pool too large for 32-bit TMA rows");

@@ -50,7 +50,7 @@ class PrefixGroups:
         # that the keys behind the prefixes are cut into
         self._own_at = _TILE * sms + rows * hq
         own_rows = q_len * self.group
-        slots = self._own_at + (8 * sms + batch * hkv * -(-own_rows // 16)) * min(16, own_rows)
+        slots = self._own_at + (12 * sms + batch * hkv * -(-own_rows // 16)) * min(16, own_rows)
         self._po = torch.empty(slots * head_dim, dtype=torch.float32, device=self.device)
         self._pml = torch.empty(slots * 2, dtype=torch.float32, device=self.device)
         self._meta = torch.zeros(self._items_at + _ITEM * self.item_cap, dtype=torch.int32, device=self.device)
@@ -137,5 +137,5 @@ def attn_shared_prefix(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tens
     capturing = torch.cuda.is_current_stream_capturing()
     ext().attn_shared(q, kcache, vcache, block_tables, seq_lens, groups._meta, groups._po, groups._pml, out,
                       scratch(q.device).err, groups.item_cap if capturing else groups.n_items, groups._own_at, scale, window)
-    _count(2 + (capturing or groups.n_items > 0))
+    _count(2)
     return out
