@@ -37,8 +37,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) own_kernel(const __grid_cons
   }
   griddep_wait();
   griddep_launch_dependents();
-  if (warp == WARPS - 1) own_sequences(a, seqs, lane);
-  __syncthreads();
+  own_sequences(a, seqs, threadIdx.x, [] { __syncthreads(); });
   // few workers spread over the SMs
   own_worker<D, HALF>(tmK, tmV, a, seqs, base + warp * g::SLOTS * g::SLICE_BYTES, bars[warp], lane,
                       warp * (int)gridDim.x + (int)blockIdx.x, WARPS * (int)gridDim.x);
@@ -118,14 +117,17 @@ static cudaError_t launch(const Args& a, cudaStream_t st) {
   const uint64_t rows = (uint64_t)a.pool_pages * a.hkv * a.page_size;
   const CUtensorMap tk = tma_map_2d_bf16(a.k, D, rows, D, 64, SLICE);
   const CUtensorMap tv = tma_map_2d_bf16(a.v, D, rows, D, 64, SLICE);
+  // a slice of 128 columns in one box: two halves of 64 columns, 16 rows each
+  auto map3 = [&](const void* p) { return tma_map_3d_bf16(p, 64, rows, 2, D * 2, 128, 64, SLICE, 2); };
+  const CUtensorMap ok = D == 128 ? map3(a.k) : tk, ov = D == 128 ? map3(a.v) : tv;
   cudaError_t e;
   if (a.n_prefix > 0) {
-    e = launch_prefix<D>(a, tk, tv, st);
+    e = launch_prefix<D>(a, tk, tv, ok, ov, st);
   } else {
     auto kern = a.T * a.G <= 8 ? own_kernel<D, 1> : own_kernel<D, 2>;
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<D>::smem(SHARED_MAX_BATCH));
     if (e != cudaSuccess) return e;
-    e = launch_k(kern, dim3((unsigned)(CTAS * a.num_sms)), dim3(WARPS * 32), Geo<D>::smem(a.B), st, tk, tv, a);
+    e = launch_k(kern, dim3((unsigned)(CTAS * a.num_sms)), dim3(WARPS * 32), Geo<D>::smem(a.B), st, ok, ov, a);
   }
   if (e != cudaSuccess) return e;
   const long out_rows = (long)a.B * a.T * a.hkv * a.G;

@@ -51,32 +51,41 @@ struct Seq {
   __device__ __forceinline__ int slices() const { return L > first ? (L + SLICE - 1) / SLICE - first / SLICE : 0; }
 };
 
-// All sequences by one warp, 32 at a time, with the running number of units; seqs [B + 1].
-__device__ __forceinline__ void own_sequences(const Args& a, Seq* seqs, int lane) {
-  int run = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 32) {
-    const int b = b0 + lane;
-    Seq q = {0, 0, 0, 0};
-    int n = 0;
-    if (b < a.B) {
-      q.L = min(a.seq_lens[b], a.max_pages * a.page_size);
-      q.first = seq_prefix(a, b);
-      q.slots = seq_prefix_slots(a, b);
-      if (a.window > 0) q.first = max(q.first, q.L - a.T + 1 - a.window);
-      n = q.slices();
-      if (n > 0) n += PIECE_COST;
-    }
-    int v = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int w = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += w;
-    }
-    q.before = run + v - n;
-    if (b < a.B) seqs[b] = q;
-    run += __shfl_sync(0xffffffffu, v, 31);
+// A value that is the same in all lanes, known to be so (it may live in a uniform register)
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ int uniform_at(int v, int lane) { return __shfl_sync(0xffffffffu, v, lane); }
+
+// All sequences by the WARPS * 32 threads of the workers (tid among them), with the running number of units; seqs [B + 1].
+// The loads of all sequences are in flight at once; `sync` is a barrier of these threads.
+template <typename Sync>
+__device__ __forceinline__ void own_sequences(const Args& a, Seq* seqs, int tid, Sync sync) {
+  for (int b = tid; b < a.B; b += WARPS * 32) {
+    Seq q;
+    q.L = min(a.seq_lens[b], a.max_pages * a.page_size);
+    q.first = seq_prefix(a, b);
+    q.slots = seq_prefix_slots(a, b);
+    if (a.window > 0) q.first = max(q.first, q.L - a.T + 1 - a.window);
+    const int n = q.slices();
+    q.before = n > 0 ? n + PIECE_COST : 0;
+    seqs[b] = q;
   }
-  if (lane == 0) seqs[a.B].before = run;
+  sync();
+  if (tid < 32) {
+    int run = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      const int b = b0 + tid, n = b < a.B ? seqs[b].before : 0;
+      int v = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int w = __shfl_up_sync(0xffffffffu, v, o);
+        if (tid >= o) v += w;
+      }
+      if (b < a.B) seqs[b].before = run + v - n;
+      run += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (tid == 0) seqs[a.B].before = run;
+  }
+  sync();
 }
 
 // The keys behind the shared prefixes: 16 rows (new tokens x heads of a KV group) of one sequence against that sequence's
@@ -101,7 +110,7 @@ __device__ __forceinline__ void own_worker(const CUtensorMap& tmK, const CUtenso
     for (int b = lane; b <= a.B; b += 32) own_before(a)[b] = seqs[b].before;
     if (lane == 0) own_before(a)[a.B + 1] = quota;
   }
-  const int lo = min(total, worker * quota), hi = min(total, lo + quota);
+  const int lo = uniform(min(total, worker * quota)), hi = uniform(min(total, lo + quota));
 
   // a walk over the pieces of [lo, hi)
   struct Piece {
@@ -145,38 +154,49 @@ __device__ __forceinline__ void own_worker(const CUtensorMap& tmK, const CUtenso
 
   if (lo < hi) {
     const uint64_t pol = policy_evict_first();
-    // ---- requests: slice i of the walk's current piece goes to slot `rs`
-    Piece rp;
+    // ---- requests: slice ri of the walk's current piece goes to slot rs
+    Piece rp, np;  // the piece being requested, the one behind it
     begin(rp);
-    bool more = rp.n > 0 || next(rp);
-    int ri = 0, rs = 0, row_y = 0;
-    // rows of the pool that hold the next 32 slices of the piece, one per lane
-    auto look_up = [&]() {
-      const int sl = seqs[rp.b].first / SLICE + rp.sl + ri + lane;
-      row_y = 0;
-      if (ri + lane < rp.n) {
-        const int pi = sl / a.slices_per_page;
-        row_y = (a.block_tables[(long)rp.b * a.max_pages + pi] * a.hkv + rp.u / tiles) * a.page_size +
-                (sl - pi * a.slices_per_page) * SLICE;
-      }
+    bool more = uniform(rp.n > 0 || next(rp)), more2;
+    int ri = 0, rs = 0, page = 0, next_page = 0;
+    // page that holds slice i0 + lane of a piece; nothing is computed from it here, so the load stays in flight
+    auto look_up = [&](const Piece& x, int i0) {
+      const int sl = seqs[x.b].first / SLICE + x.sl + i0 + lane;
+      return i0 + lane < x.n ? a.block_tables[(long)x.b * a.max_pages + sl / a.slices_per_page] : 0;
     };
+    auto look_ahead = [&]() {  // the next piece's first pages are read long before they are needed
+      np = rp;
+      more2 = uniform(more && next(np));
+      if (more2) next_page = look_up(np, 0);
+    };
+    if (more) page = look_up(rp, 0);
+    look_ahead();
     auto request = [&]() {
       if (!more) return;
-      if ((ri & 31) == 0) look_up();
-      const int y = __shfl_sync(0xffffffffu, row_y, ri & 31);
-      if (lane == 0) {
+      const int sl = seqs[rp.b].first / SLICE + rp.sl + ri;
+      const int y = uniform((uniform_at(page, ri & 31) * a.hkv + rp.u / tiles) * a.page_size + sl % a.slices_per_page * SLICE);
+      if (elect_one()) {
         mbar_arrive_expect_tx(&full[rs], g::SLICE_BYTES);
         uint8_t* dst = ring + rs * g::SLICE_BYTES;
-#pragma unroll
-        for (int hf = 0; hf < g::HALVES; ++hf) {
-          tma_load_2d(dst + hf * g::BOX, &tmK, &full[rs], hf * 64, y, pol);
-          tma_load_2d(dst + (g::HALVES + hf) * g::BOX, &tmV, &full[rs], hf * 64, y, pol);
+        // both 64-column halves of the 16 rows in one box each of K and V
+        if constexpr (g::HALVES == 2) {
+          tma_load_3d(dst, &tmK, &full[rs], 0, y, 0, pol);
+          tma_load_3d(dst + 2 * g::BOX, &tmV, &full[rs], 0, y, 0, pol);
+        } else {
+          tma_load_2d(dst, &tmK, &full[rs], 0, y, pol);
+          tma_load_2d(dst + g::BOX, &tmV, &full[rs], 0, y, pol);
         }
       }
+      __syncwarp();
       if (++rs == SLOTS) rs = 0;
-      if (++ri == rp.n) {
+      if (++ri == uniform(rp.n)) {
         ri = 0;
-        more = next(rp);
+        rp = np;
+        page = next_page;
+        more = more2;
+        look_ahead();
+      } else if ((ri & 31) == 0) {
+        page = look_up(rp, ri);
       }
     };
 #pragma unroll 1
@@ -215,9 +235,7 @@ __device__ __forceinline__ void own_worker(const CUtensorMap& tmK, const CUtenso
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll 1
       for (int i = 0; i < p.n; ++i) {
-        int w = ok;
-        if (lane == 0 && ok) w = mbar_wait_bounded(&full[s], ph, a.err, ERR_MBAR_TIMEOUT_MMA, nullptr, WAIT_NS);
-        ok = __shfl_sync(0xffffffffu, w, 0) != 0;
+        ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(&full[s], ph, a.err, ERR_MBAR_TIMEOUT_MMA, nullptr, WAIT_NS));
         if (!ok) break;
         const int key0 = (s0 + i) * SLICE;
         const uint32_t kb = smem_u32(ring + s * g::SLICE_BYTES), vb = kb + g::HALVES * g::BOX;

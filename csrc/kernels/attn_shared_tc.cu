@@ -24,6 +24,9 @@ constexpr int BM = 128, BK = 64, NS = 2;  // rows and keys of a stream's block, 
 constexpr int SLICES = BK / SLICE;
 constexpr int P_THREADS = 128 + NS * BM;             // of the prefix items
 constexpr int THREADS = P_THREADS + WARPS * 32;       // and of the sequences' own keys
+// registers a thread: the workers' accumulators need more than the softmax; the sum is what the CTA is launched with
+constexpr int P_REGS = 120, OWN_REGS = 152;
+static_assert(P_THREADS * P_REGS + WARPS * 32 * OWN_REGS <= THREADS * 128, "register split");
 constexpr int PRODUCER_V = 10, MMA0 = 1, MMA1 = 11, OWN = 12;  // warps
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t S_COLS = 128, O_COL = NS * S_COLS, O_COLS = 128;
@@ -74,7 +77,8 @@ struct Item {
 
 template <int D, int HALF>
 __global__ void __launch_bounds__(THREADS, 1)
-    prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Args a) {
+    prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                  const __grid_constant__ CUtensorMap ownK, const __grid_constant__ CUtensorMap ownV, const Args a) {
   using C = Cfg<D>;
   constexpr int K_STAGES = C::K_STAGES, V_STAGES = C::V_STAGES;
   extern __shared__ uint8_t smem_raw[];
@@ -87,7 +91,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   Bars<D>* bars = reinterpret_cast<Bars<D>*>(seqs + a.B + 1);
   // broadcast values are known to be the same for the whole warp, so the address arithmetic of the issuing warps stays in
   // uniform registers (a product took 60 ns to issue otherwise, a TMA box 108 instead of 75)
-  auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -138,14 +141,15 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp >= OWN) {
     // The sequences' own keys, read beside the products: these warps wait for memory while the others keep the tensor
     // cores busy (as a kernel of its own behind this one, 64 sessions behind 8k took 42 us).
-    if (warp == OWN) own_sequences(a, seqs, lane);
-    named_bar_sync(2, WARPS * 32);
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(OWN_REGS));
+    own_sequences(a, seqs, threadIdx.x - OWN * 32, [] { named_bar_sync(2, WARPS * 32); });
     const int w = warp - OWN;
-    own_worker<D, HALF>(tmK, tmV, a, seqs, own_sm + w * Geo<D>::SLOTS * Geo<D>::SLICE_BYTES, bars->own_full[w], lane,
+    own_worker<D, HALF>(ownK, ownV, a, seqs, own_sm + w * Geo<D>::SLOTS * Geo<D>::SLICE_BYTES, bars->own_full[w], lane,
                         w * (int)gridDim.x + (int)blockIdx.x, WARPS * (int)gridDim.x);
     return;
   }
 
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P_REGS));
   // ring positions of this warp's role: the next block of K (MMA: to score; producer of K) and of V
   int pos = 0, v_pos = 0;
   uint32_t phase = 0, v_phase = 0;
@@ -461,15 +465,16 @@ __global__ void __launch_bounds__(THREADS, 1)
 }  // namespace
 
 template <int D>
-cudaError_t launch_prefix(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
+cudaError_t launch_prefix(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& ok, const CUtensorMap& ov,
+                          cudaStream_t st) {
   auto kern = a.T * a.G <= 8 ? prefix_kernel<D, 1> : prefix_kernel<D, 2>;
   const cudaError_t e =
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<D>(SHARED_MAX_BATCH));
   if (e != cudaSuccess) return e;
-  return launch_k(kern, dim3((unsigned)a.num_sms), dim3(THREADS), smem_bytes<D>(a.B), st, tk, tv, a);
+  return launch_k(kern, dim3((unsigned)a.num_sms), dim3(THREADS), smem_bytes<D>(a.B), st, tk, tv, ok, ov, a);
 }
-template cudaError_t launch_prefix<64>(const Args&, const CUtensorMap&, const CUtensorMap&, cudaStream_t);
-template cudaError_t launch_prefix<128>(const Args&, const CUtensorMap&, const CUtensorMap&, cudaStream_t);
+template cudaError_t launch_prefix<64>(const Args&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, cudaStream_t);
+template cudaError_t launch_prefix<128>(const Args&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, cudaStream_t);
 
 }  // namespace shared_attn
 }  // namespace mesh
