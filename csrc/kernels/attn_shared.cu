@@ -13,19 +13,381 @@
 //
 // The item list is made on the host when the groups change (PrefixGroups) and lives in device memory, so a
 // captured step follows later changes of groups, lengths and tables.
-#include "attn_shared_own.cuh"
+#include "attn_shared.cuh"
 
 namespace mesh {
 namespace shared_attn {
 namespace {
 
-// Where no sequence shares a prefix: three CTAs of four workers an SM.
-template <int D, int HALF>
-__global__ void __launch_bounds__(WARPS * 32, CTAS) own_kernel(const __grid_constant__ CUtensorMap tmK,
-                                                               const __grid_constant__ CUtensorMap tmV, const Args a) {
+constexpr int WARPS = 4;         // workers of a CTA
+constexpr int CTAS = 3;          // per SM; one beside a CTA of the prefix kernel
+constexpr int TILE_ROWS = 16;    // query rows of a worker
+constexpr int PIECE_COST = 2;    // what a piece costs besides its slices, in slices
+constexpr int MIN_QUOTA = 4;     // units (slices and piece costs) a worker takes at least
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1));
+}
+// transpose of an 8 x 8 matrix of 16-bit values held by the warp
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// byte offset of (row, 16-byte chunk) inside a [16 x 64] box written with the 128-byte swizzle
+__device__ __forceinline__ uint32_t swz(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
+
+template <int D>
+struct Geo {
+  static constexpr int HALVES = D / 64;
+  static constexpr uint32_t BOX = SLICE * 64 * 2;           // one [16 x 64] box
+  static constexpr uint32_t SLICE_BYTES = 2 * HALVES * BOX; // K halves then V halves
+  static constexpr int SLOTS = 16 * 1024 / SLICE_BYTES;     // slices in flight per worker: 64 KB per CTA
+  // rings | what is known of each sequence
+  static size_t smem(int B) { return 1024 + WARPS * SLOTS * SLICE_BYTES + 16 * (B + 1); }
+};
+
+// A sequence's keys behind its shared prefix (and inside the window).
+struct Seq {
+  int before;  // units of the sequences before it, for one KV head and tile of rows
+  int first;   // first key
+  int L;       // end
+  int slots;   // partials of its shared prefix per row
+  __device__ __forceinline__ int slices() const { return L > first ? (L + SLICE - 1) / SLICE - first / SLICE : 0; }
+};
+
+// A value that is the same in all lanes, known to be so (it may live in a uniform register)
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ int uniform_at(int v, int lane) { return __shfl_sync(0xffffffffu, v, lane); }
+
+// All sequences by the WARPS * 32 threads of the workers (tid among them), with the running number of units; seqs [B + 1].
+// The loads of all sequences are in flight at once; `sync` is a barrier of these threads.
+template <typename Sync>
+__device__ __forceinline__ void own_sequences(const Args& a, Seq* seqs, int tid, Sync sync) {
+  for (int b = tid; b < a.B; b += WARPS * 32) {
+    Seq q;
+    q.L = min(a.seq_lens[b], a.max_pages * a.page_size);
+    q.first = seq_prefix(a, b);
+    q.slots = seq_prefix_slots(a, b);
+    if (a.window > 0) q.first = max(q.first, q.L - a.T + 1 - a.window);
+    const int n = q.slices();
+    q.before = n > 0 ? n + PIECE_COST : 0;
+    seqs[b] = q;
+  }
+  sync();
+  if (tid < 32) {
+    int run = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      const int b = b0 + tid, n = b < a.B ? seqs[b].before : 0;
+      int v = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int w = __shfl_up_sync(0xffffffffu, v, o);
+        if (tid >= o) v += w;
+      }
+      if (b < a.B) seqs[b].before = run + v - n;
+      run += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (tid == 0) seqs[a.B].before = run;
+  }
+  sync();
+}
+
+// The keys behind the shared prefixes: 16 rows (new tokens x heads of a KV group) of one sequence against that sequence's
+// own slices of 16 keys. All of them, in the order (sequence, KV head, tile of rows, slice), are cut into equal quotas,
+// one per warp: lengths from one token to long ones then keep every SM as busy. A quota is a run of
+// pieces, one for each (sequence, head, tile) it touches; a piece counts as PIECE_COST slices besides its own, about
+// what loading its queries and writing its result take. Piece number = worker + (sequence, head, tile), which no other
+// piece has. A warp works by itself: it requests slices SLOTS ahead (TMA, 128-byte swizzle), without a barrier between
+// warps; four warps that split each piece and merged it took twice as long (64 sessions of up to 512 keys). Bound by
+// reading K and V.
+// The products run transposed, S^T = K Q^T and O^T = V^T P^T on m16n8k16 fragments, so that the few query rows are the
+// narrow side: NT tiles of 8 rows. With the rows on the 16-wide side half of every product and of the accumulators
+// would be padding (168 registers, so no CTA fitted beside the prefix kernel's).
+template <int D, int NT>
+__device__ __forceinline__ void own_worker(const CUtensorMap& tmK, const CUtensorMap& tmV, const Args& a, const Seq* seqs,
+                                           uint8_t* ring, uint64_t* full, int lane, int worker, int workers) {
+  using g = Geo<D>;
+  constexpr int SLOTS = g::SLOTS;
+  const int rows = a.T * a.G, hq = a.hkv * a.G, tiles = (rows + TILE_ROWS - 1) / TILE_ROWS;
+  const int per_seq = a.hkv * tiles;
+  const int total = seqs[a.B].before * per_seq;
+  const int quota = max(MIN_QUOTA, (total + workers - 1) / workers);
+  if (worker == 0) {  // for the combine kernel
+    for (int b = lane; b <= a.B; b += 32) own_before(a)[b] = seqs[b].before;
+    if (lane == 0) own_before(a)[a.B + 1] = quota;
+  }
+  const int lo = uniform(min(total, worker * quota)), hi = uniform(min(total, lo + quota));
+
+  // a walk over the pieces of [lo, hi)
+  struct Piece {
+    int b, u, pos;  // sequence; its (KV head, tile); unit the piece starts at
+    int sl, n;      // first slice of the own ones, slices
+  };
+  auto fit = [&](Piece& p, int r) {  // r: units of (b, u) before pos
+    const int units = seqs[p.b + 1].before - seqs[p.b].before;
+    const int end = min(units, r + hi - p.pos);
+    p.sl = max(r, PIECE_COST) - PIECE_COST;
+    p.n = max(0, end - PIECE_COST - p.sl);
+    p.pos += end - r;  // where the next piece starts
+  };
+  auto begin = [&](Piece& p) {
+    int x = 0, y = a.B - 1;  // last sequence that starts at or before lo
+    while (x < y) {
+      const int mid = (x + y + 1) >> 1;
+      if (seqs[mid].before * per_seq <= lo)
+        x = mid;
+      else
+        y = mid - 1;
+    }
+    const int units = seqs[x + 1].before - seqs[x].before, off = lo - seqs[x].before * per_seq;
+    p.b = x;
+    p.u = off / units;
+    p.pos = lo;
+    fit(p, off - p.u * units);
+  };
+  auto next = [&](Piece& p) {  // false behind the last piece
+    do {
+      if (p.pos >= hi) return false;
+      if (++p.u == per_seq) {
+        p.u = 0;
+        do ++p.b;
+        while (seqs[p.b + 1].before == seqs[p.b].before);
+      }
+      fit(p, 0);
+    } while (p.n == 0);
+    return true;
+  };
+
+  if (lo < hi) {
+    const uint64_t pol = policy_evict_first();
+    // ---- requests: slice ri of the walk's current piece goes to slot rs
+    Piece rp, np;  // the piece being requested, the one behind it
+    begin(rp);
+    bool more = uniform(rp.n > 0 || next(rp)), more2;
+    int ri = 0, rs = 0, page = 0, next_page = 0;
+    // page that holds slice i0 + lane of a piece; nothing is computed from it here, so the load stays in flight
+    auto look_up = [&](const Piece& x, int i0) {
+      const int sl = seqs[x.b].first / SLICE + x.sl + i0 + lane;
+      return i0 + lane < x.n ? a.block_tables[(long)x.b * a.max_pages + sl / a.slices_per_page] : 0;
+    };
+    auto look_ahead = [&]() {  // the next piece's first pages are read long before they are needed
+      np = rp;
+      more2 = uniform(more && next(np));
+      if (more2) next_page = look_up(np, 0);
+    };
+    if (more) page = look_up(rp, 0);
+    look_ahead();
+    auto request = [&]() {
+      if (!more) return;
+      const int sl = seqs[rp.b].first / SLICE + rp.sl + ri;
+      const int y = uniform((uniform_at(page, ri & 31) * a.hkv + rp.u / tiles) * a.page_size + sl % a.slices_per_page * SLICE);
+      if (elect_one()) {
+        mbar_arrive_expect_tx(&full[rs], g::SLICE_BYTES);
+        uint8_t* dst = ring + rs * g::SLICE_BYTES;
+        // both 64-column halves of the 16 rows in one box each of K and V
+        if constexpr (g::HALVES == 2) {
+          tma_load_3d(dst, &tmK, &full[rs], 0, y, 0, pol);
+          tma_load_3d(dst + 2 * g::BOX, &tmV, &full[rs], 0, y, 0, pol);
+        } else {
+          tma_load_2d(dst, &tmK, &full[rs], 0, y, pol);
+          tma_load_2d(dst + g::BOX, &tmV, &full[rs], 0, y, pol);
+        }
+      }
+      __syncwarp();
+      if (++rs == SLOTS) rs = 0;
+      if (++ri == uniform(rp.n)) {
+        ri = 0;
+        rp = np;
+        page = next_page;
+        more = more2;
+        look_ahead();
+      } else if ((ri & 31) == 0) {
+        page = look_up(rp, ri);
+      }
+    };
+#pragma unroll 1
+    for (int i = 0; i < SLOTS; ++i) request();
+
+    Piece p;
+    begin(p);
+    bool todo = p.n > 0 || next(p), ok = true;
+    int s = 0;
+    uint32_t ph = 0;
+    for (; todo; todo = next(p)) {
+      const Seq q = seqs[p.b];
+      const int h = p.u / tiles, row0 = (p.u - h * tiles) * TILE_ROWS, n_rows = min(TILE_ROWS, rows - row0);
+      const int s0 = q.first / SLICE + p.sl;
+      const int k0 = max(q.first, s0 * SLICE), k1 = min(q.L, (s0 + p.n) * SLICE);
+      // query fragments straight from memory: row lane / 4 of each tile, columns (lane % 4) * 2 and 8 to the right
+      uint32_t qf[NT][D / 16][2];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int r = (lane >> 2) + 8 * j, x = row0 + min(r, n_rows - 1), t = x / a.G;
+        const __nv_bfloat16* src = a.q + ((long)(p.b * a.T + t) * hq + h * a.G + x - t * a.G) * D + (lane & 3) * 2;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          qf[j][kk][0] = r < n_rows ? *reinterpret_cast<const uint32_t*>(src + kk * 16) : 0u;
+          qf[j][kk][1] = r < n_rows ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8) : 0u;
+        }
+      }
+      int hi_k[NT][2], lo_k[NT][2];  // keys that this lane's rows (lane % 4) * 2 + i of each tile may attend: [lo_k, hi_k)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = (lane & 3) * 2 + i + 8 * j, pos = q.L - a.T + (row0 + r) / a.G;
+          hi_k[j][i] = r < n_rows ? min(k1, pos + 1) : 0;
+          lo_k[j][i] = a.window > 0 ? max(k0, pos + 1 - a.window) : k0;
+        }
+      float o[NT][D / 16][4];  // [tile][16 columns of the head]: columns lane / 4 and 8 below, rows (lane % 4) * 2 + {0, 1}
+      float m[NT][2], l[NT][2];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x) o[j][x][0] = o[j][x][1] = o[j][x][2] = o[j][x][3] = 0.f;
+        m[j][0] = m[j][1] = -INFINITY;
+        l[j][0] = l[j][1] = 0.f;
+      }
+#pragma unroll 1
+      for (int i = 0; i < p.n; ++i) {
+        ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(&full[s], ph, a.err, ERR_MBAR_TIMEOUT_MMA, nullptr, WAIT_NS));
+        if (!ok) break;
+        const int key0 = (s0 + i) * SLICE;
+        const uint32_t kb = smem_u32(ring + s * g::SLICE_BYTES), vb = kb + g::HALVES * g::BOX;
+        // Keys past the range may hold anything (a page's unused tail): their values must not reach the products as
+        // NaN or infinity times a zero weight. Clearing them in the fragments costs two masks; clearing them in shared
+        // memory needs a proxy fence, which waited for the loads in flight.
+        uint32_t keep[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int left = k1 - (key0 + x * 8 + (lane & 3) * 2);  // of this lane's two keys
+          keep[x] = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+        }
+        float sc[NT][4], sd[NT][4];  // keys lane / 4 and 8 below; two chains of products each
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[j][e] = sd[j][e] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          uint32_t kf[4];
+          ldsm_x4(kb + (kk >> 2) * g::BOX + swz((lane & 7) + ((lane >> 3) & 1) * 8, (kk & 3) * 2 + (lane >> 4)), kf);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) mma((kk & 1) ? sd[j] : sc[j], kf, qf[j][kk][0], qf[j][kk][1]);
+        }
+        uint32_t pf[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int key = key0 + (lane >> 2);
+            const bool in0 = key < hi_k[j][i] && key >= lo_k[j][i], in1 = key + 8 < hi_k[j][i] && key + 8 >= lo_k[j][i];
+            const float s0v = in0 ? (sc[j][i] + sd[j][i]) * a.scale_log2 : -INFINITY;
+            const float s1v = in1 ? (sc[j][2 + i] + sd[j][2 + i]) * a.scale_log2 : -INFINITY;
+            float mx = fmaxf(s0v, s1v);
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+            const float mn = fmaxf(m[j][i], mx), mb = mn == -INFINITY ? 0.f : mn;
+            const float corr = ex2_ftz(m[j][i] - mb);
+            sc[j][i] = ex2_ftz(s0v - mb);
+            sc[j][2 + i] = ex2_ftz(s1v - mb);
+            l[j][i] = l[j][i] * corr + (sc[j][i] + sc[j][2 + i]);
+            m[j][i] = mn;
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x) {
+              o[j][x][i] *= corr;
+              o[j][x][2 + i] *= corr;
+            }
+          }
+          // the weights are rounded to bf16 for the product (half a step of 2^-8 each); their sum keeps fp32
+          pf[j][0] = transposed(pack_bf16x2(sc[j][0], sc[j][1]));
+          pf[j][1] = transposed(pack_bf16x2(sc[j][2], sc[j][3]));
+        }
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x) {
+          uint32_t vf[4];
+          ldsm_x4_t(vb + (x >> 2) * g::BOX + swz((lane & 7) + (lane >> 4) * 8, (x & 3) * 2 + ((lane >> 3) & 1)), vf);
+          vf[0] &= keep[0];
+          vf[1] &= keep[0];
+          vf[2] &= keep[1];
+          vf[3] &= keep[1];
+#pragma unroll
+          for (int j = 0; j < NT; ++j) mma(o[j][x], vf, pf[j][0], pf[j][1]);
+        }
+        // the products above have taken every fragment of this slot, so it may be filled again
+        __syncwarp();
+        request();
+        if (++s == SLOTS) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) l[j][i] += __shfl_xor_sync(0xffffffffu, l[j][i], x);
+      // a sequence without a prefix whose keys are all in this piece is done: its rows go out; else a partial
+      const bool whole = p.n == q.slices() && q.slots == 0;
+      const int stride = min(rows, TILE_ROWS);
+      const long part = a.own_at + (long)(worker + p.b * per_seq + p.u) * stride;
+      if (part + stride > a.slot_cap) {
+        if (lane == 0) record_error(a.err, ERR_BAD_ARGUMENT);
+        continue;
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = (lane & 3) * 2 + i + 8 * j;
+          if (r >= n_rows) continue;
+          const int x0 = row0 + r, t = x0 / a.G;
+          __nv_bfloat16* out = a.out + ((long)(p.b * a.T + t) * hq + h * a.G + x0 - t * a.G) * D + (lane >> 2);
+          float* po = a.po + (part + r) * D + (lane >> 2);
+          const float inv = l[j][i] > 0.f ? 1.f / l[j][i] : 0.f;
+#pragma unroll
+          for (int x = 0; x < D / 16; ++x)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if (whole)
+                out[x * 16 + e * 8] = f2bf(o[j][x][2 * e + i] * inv);
+              else
+                po[x * 16 + e * 8] = o[j][x][2 * e + i];
+            }
+          if (!whole && lane < 4) a.pml[part + r] = make_float2(m[j][i], l[j][i]);
+        }
+    }
+    if (!ok) {
+      // the copies still in flight land before the warp goes (bounded)
+      const uint64_t t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 50000000ull) {
+      }
+    }
+  }
+}
+
+// Three CTAs an SM; for up to 8 rows, whose registers (128) allow it, also one beside a CTA of the prefix kernel.
+template <int D, int NT>
+__global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : CTAS) own_kernel(const __grid_constant__ CUtensorMap tmK,
+                                                            const __grid_constant__ CUtensorMap tmV, const Args a) {
   using g = Geo<D>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Seq* seqs = reinterpret_cast<Seq*>(base + WARPS * g::SLOTS * g::SLICE_BYTES);  // [B + 1]
   __shared__ uint64_t bars[WARPS][g::SLOTS];
@@ -35,12 +397,15 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) own_kernel(const __grid_cons
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
-  griddep_wait();
   griddep_launch_dependents();
+  // behind a prefix kernel, whose own inputs are complete when it lets this one start, only the end has to wait
+  if (a.n_prefix == 0) griddep_wait();
   own_sequences(a, seqs, threadIdx.x, [] { __syncthreads(); });
   // few workers spread over the SMs
-  own_worker<D, HALF>(tmK, tmV, a, seqs, base + warp * g::SLOTS * g::SLICE_BYTES, bars[warp], lane,
+  own_worker<D, NT>(tmK, tmV, a, seqs, base + warp * g::SLOTS * g::SLICE_BYTES, bars[warp], lane,
                       warp * (int)gridDim.x + (int)blockIdx.x, WARPS * (int)gridDim.x);
+  // this grid is complete only when the prefix grid is; one CTA sees to that, the others make room for the next
+  if (a.n_prefix != 0 && blockIdx.x == gridDim.x - 1) griddep_wait();
 }
 
 // One warp per row (sequence, token, head): merge its partials, the prefix's first, in order. Lane i holds the (m, l) of
@@ -120,15 +485,14 @@ static cudaError_t launch(const Args& a, cudaStream_t st) {
   // a slice of 128 columns in one box: two halves of 64 columns, 16 rows each
   auto map3 = [&](const void* p) { return tma_map_3d_bf16(p, 64, rows, 2, D * 2, 128, 64, SLICE, 2); };
   const CUtensorMap ok = D == 128 ? map3(a.k) : tk, ov = D == 128 ? map3(a.v) : tv;
-  cudaError_t e;
-  if (a.n_prefix > 0) {
-    e = launch_prefix<D>(a, tk, tv, ok, ov, st);
-  } else {
-    auto kern = a.T * a.G <= 8 ? own_kernel<D, 1> : own_kernel<D, 2>;
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<D>::smem(SHARED_MAX_BATCH));
-    if (e != cudaSuccess) return e;
-    e = launch_k(kern, dim3((unsigned)(CTAS * a.num_sms)), dim3(WARPS * 32), Geo<D>::smem(a.B), st, ok, ov, a);
-  }
+  cudaError_t e = cudaSuccess;
+  if (a.n_prefix > 0 && (e = launch_prefix<D>(a, tk, tv, st)) != cudaSuccess) return e;
+  auto kern = a.T * a.G <= 8 ? own_kernel<D, 1> : own_kernel<D, 2>;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<D>::smem(SHARED_MAX_BATCH));
+  if (e != cudaSuccess) return e;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  if (e != cudaSuccess) return e;
+  e = launch_k(kern, dim3((unsigned)(CTAS * a.num_sms)), dim3(WARPS * 32), Geo<D>::smem(a.B), st, ok, ov, a);
   if (e != cudaSuccess) return e;
   const long out_rows = (long)a.B * a.T * a.hkv * a.G;
   return launch_k(combine_kernel<D>, dim3((unsigned)((out_rows + 3) / 4)), dim3(128), 0, st, a);

@@ -28,8 +28,7 @@ __device__ __forceinline__ const int* items(const Args& a) { return a.meta + sha
 
 // rows of a prefix item against its shared keys on tcgen05 (attn_shared_tc.cu)
 template <int D>
-cudaError_t launch_prefix(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& ok, const CUtensorMap& ov,
-                          cudaStream_t st);
+cudaError_t launch_prefix(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st);
 
 }  // namespace shared_attn
 }  // namespace mesh

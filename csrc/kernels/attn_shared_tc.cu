@@ -14,7 +14,7 @@
 // TMEM) when it grows by more than 2^8; sum and output share it, so the result stays exact.
 // TMEM columns (512): S of stream t, buffer b at t * 128 + b * 64; O_t at 256 + t * 128.
 // Every wait is bounded; on a timeout an error is recorded, copies and products in flight are drained, TMEM is freed.
-#include "attn_shared_own.cuh"
+#include "attn_shared.cuh"
 
 namespace mesh {
 namespace shared_attn {
@@ -22,12 +22,9 @@ namespace {
 
 constexpr int BM = 128, BK = 64, NS = 2;  // rows and keys of a stream's block, streams
 constexpr int SLICES = BK / SLICE;
-constexpr int P_THREADS = 128 + NS * BM;             // of the prefix items
-constexpr int THREADS = P_THREADS + WARPS * 32;       // and of the sequences' own keys
-// registers a thread: the workers' accumulators need more than the softmax; the sum is what the CTA is launched with
-constexpr int P_REGS = 120, OWN_REGS = 152;
-static_assert(P_THREADS * P_REGS + WARPS * 32 * OWN_REGS <= THREADS * 128, "register split");
-constexpr int PRODUCER_V = 10, MMA0 = 1, MMA1 = 11, OWN = 12;  // warps
+constexpr int THREADS = 128 + NS * BM;
+constexpr int MAX_REGS = 128;  // a thread: 12 warps leave room for the 4 of an own_kernel CTA
+constexpr int PRODUCER_V = 10, MMA0 = 1, MMA1 = 11;  // warps
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t S_COLS = 128, O_COL = NS * S_COLS, O_COLS = 128;
 constexpr float RESCALE = 8.0f;  // log2 units
@@ -39,7 +36,8 @@ struct Cfg {
   static constexpr uint32_t Q_TILE = HALVES * Q_ATOM;     // 128 rows x D
   static constexpr uint32_t ATOM = BK * 128;              // 64 keys x 64 elements
   static constexpr uint32_t TILE = HALVES * ATOM;         // 64 keys x D
-  // blocks of K and of V in flight: 80 KB of rings, beside 64 KB of those of the sequences' own keys
+  // blocks of K and of V in flight: 80 KB of rings. With the query tiles that leaves room for a CTA of the sequences' own
+  // keys on the same SM, which reads while this kernel multiplies.
   static constexpr int K_STAGES = 3 * (128 / D), V_STAGES = 2 * (128 / D);
   static constexpr uint32_t BOX = SLICE * 128;
   static constexpr int STAGED = D * 4 + 16;               // a row of the result on its way out: padded against bank conflicts
@@ -49,18 +47,16 @@ template <int D>
 struct Bars {
   uint64_t q_full;
   uint64_t k_full[Cfg<D>::K_STAGES], k_empty[Cfg<D>::K_STAGES], v_full[Cfg<D>::V_STAGES], v_empty[Cfg<D>::V_STAGES];
-  uint64_t s_full[NS][2], p_full[NS][2], o_done[NS];
+  uint64_t s_full[NS][2], p_full[NS][2], o_done[NS], o_last[NS];  // o_last: the item's last product
   uint64_t mma_done;
-  uint64_t own_full[WARPS][Geo<D>::SLOTS];
   uint32_t tmem_base;
   int abort;
 };
 
 template <int D>
-constexpr size_t smem_bytes(int B) {
+constexpr size_t smem_bytes() {
   static_assert(NS * BM * Cfg<D>::STAGED <= NS * Cfg<D>::Q_TILE + (Cfg<D>::K_STAGES + Cfg<D>::V_STAGES) * Cfg<D>::TILE, "staged rows fit");
-  return 1024 + NS * Cfg<D>::Q_TILE + (Cfg<D>::K_STAGES + Cfg<D>::V_STAGES) * Cfg<D>::TILE + sizeof(Bars<D>) +
-         WARPS * Geo<D>::SLOTS * Geo<D>::SLICE_BYTES + 16 * (B + 1);
+  return 1024 + NS * Cfg<D>::Q_TILE + (Cfg<D>::K_STAGES + Cfg<D>::V_STAGES) * Cfg<D>::TILE + sizeof(Bars<D>);
 }
 
 struct Item {
@@ -75,10 +71,9 @@ struct Item {
   __device__ __forceinline__ int streams() const { return rows > BM ? 2 : 1; }
 };
 
-template <int D, int HALF>
-__global__ void __launch_bounds__(THREADS, 1)
-    prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                  const __grid_constant__ CUtensorMap ownK, const __grid_constant__ CUtensorMap ownV, const Args a) {
+template <int D>
+__global__ void __maxnreg__(MAX_REGS)
+    prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Args a) {
   using C = Cfg<D>;
   constexpr int K_STAGES = C::K_STAGES, V_STAGES = C::V_STAGES;
   extern __shared__ uint8_t smem_raw[];
@@ -86,11 +81,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint8_t* q_sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   uint8_t* k_sm = q_sm + NS * C::Q_TILE;
   uint8_t* v_sm = k_sm + K_STAGES * C::TILE;
-  uint8_t* own_sm = v_sm + V_STAGES * C::TILE;
-  Seq* seqs = reinterpret_cast<Seq*>(own_sm + WARPS * Geo<D>::SLOTS * Geo<D>::SLICE_BYTES);  // [B + 1]
-  Bars<D>* bars = reinterpret_cast<Bars<D>*>(seqs + a.B + 1);
+  Bars<D>* bars = reinterpret_cast<Bars<D>*>(v_sm + V_STAGES * C::TILE);
   // broadcast values are known to be the same for the whole warp, so the address arithmetic of the issuing warps stays in
   // uniform registers (a product took 60 ns to issue otherwise, a TMA box 108 instead of 75)
+  auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -109,9 +103,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         mbar_init(&bars->p_full[t][b], BM);
       }
       mbar_init(&bars->o_done[t], 1);
+      mbar_init(&bars->o_last[t], 1);
     }
     mbar_init(&bars->mma_done, NS);
-    for (int i = 0; i < WARPS * Geo<D>::SLOTS; ++i) mbar_init(&bars->own_full[0][0] + i, 1);
     bars->abort = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmK);
@@ -137,19 +131,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (x < it.rows) first_b = members(a)[it.moff + (it.row0 + x) / TG];
   }
   griddep_wait();
+  // The kernel of the sequences' own keys needs what precedes this grid (complete now) and, at its end only, this
+  // grid's partials: it starts beside it.
   griddep_launch_dependents();
-  if (warp >= OWN) {
-    // The sequences' own keys, read beside the products: these warps wait for memory while the others keep the tensor
-    // cores busy (as a kernel of its own behind this one, 64 sessions behind 8k took 42 us).
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(OWN_REGS));
-    own_sequences(a, seqs, threadIdx.x - OWN * 32, [] { named_bar_sync(2, WARPS * 32); });
-    const int w = warp - OWN;
-    own_worker<D, HALF>(ownK, ownV, a, seqs, own_sm + w * Geo<D>::SLOTS * Geo<D>::SLICE_BYTES, bars->own_full[w], lane,
-                        w * (int)gridDim.x + (int)blockIdx.x, WARPS * (int)gridDim.x);
-    return;
-  }
 
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P_REGS));
   // ring positions of this warp's role: the next block of K (MMA: to score; producer of K) and of V
   int pos = 0, v_pos = 0;
   uint32_t phase = 0, v_phase = 0;
@@ -161,6 +146,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   };
   uint32_t cnt = 0;  // blocks this warp's stream has gone through (MMA, softmax)
   uint32_t ic = 0;   // items
+  uint32_t lasts = 0;  // items this softmax warp's stream took part in
   for (int i = blockIdx.x; i < n_items; i += gridDim.x, ++ic) {
     if (ic > 0) it = Item(a, i);
     const int nblk = uniform(it.blocks());
@@ -248,6 +234,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int kk = 0; kk < BK / 16; ++kk)
             umma_bf16_ts(ot, pt + kk * 8, vd + kk * (2048 >> 4), IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
           umma_commit(&bars->o_done[t]);
+          if (j == nblk - 1) umma_commit(&bars->o_last[t]);
           give_back(&bars->v_empty[v_pos]);
         }
         __syncwarp();
@@ -407,9 +394,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (t < ns) {
         cnt += nblk;
-        // the last two products, one after the other: the parity alone tells only neighbouring phases apart
-        if (ok && nblk > 1) ok = wait(&bars->o_done[t], (cnt - 2) & 1u);
-        if (ok && nblk > 0) ok = wait(&bars->o_done[t], (cnt - 1) & 1u);
+        // A barrier of its own: o_done may be one or two products behind, which its parity does not tell apart.
+        if (nblk > 0) ok = ok && wait(&bars->o_last[t], lasts++ & 1u);
         tc_fence_after();
         named_bar_sync(1, ns * BM);  // every stream is done with the query tiles and the rings
         if (ok && warp_live) {
@@ -445,7 +431,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       tc_fence_before();
       if (i + (int)gridDim.x < n_items) fence_proxy_async();  // the shared memory is written by TMA again
     }
-    named_bar_sync(3, P_THREADS);
+    __syncthreads();
     tc_fence_after();
     if (bars->abort) break;
   }
@@ -457,7 +443,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   }
   tc_fence_before();
-  named_bar_sync(3, P_THREADS);
+  __syncthreads();
   tc_fence_after();
   if (warp == MMA0) tmem_dealloc(tmem, TMEM_COLS);
 }
@@ -465,16 +451,17 @@ __global__ void __launch_bounds__(THREADS, 1)
 }  // namespace
 
 template <int D>
-cudaError_t launch_prefix(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& ok, const CUtensorMap& ov,
-                          cudaStream_t st) {
-  auto kern = a.T * a.G <= 8 ? prefix_kernel<D, 1> : prefix_kernel<D, 2>;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<D>(SHARED_MAX_BATCH));
+cudaError_t launch_prefix(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
+  auto kern = prefix_kernel<D>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<D>());
   if (e != cudaSuccess) return e;
-  return launch_k(kern, dim3((unsigned)a.num_sms), dim3(THREADS), smem_bytes<D>(a.B), st, tk, tv, ok, ov, a);
+  // the SM keeps all its shared memory, also what this kernel does not use: the other kernel's CTA starts beside it
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  if (e != cudaSuccess) return e;
+  return launch_k(kern, dim3((unsigned)min(a.n_prefix, a.num_sms)), dim3(THREADS), smem_bytes<D>(), st, tk, tv, a);
 }
-template cudaError_t launch_prefix<64>(const Args&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, cudaStream_t);
-template cudaError_t launch_prefix<128>(const Args&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, cudaStream_t);
+template cudaError_t launch_prefix<64>(const Args&, const CUtensorMap&, const CUtensorMap&, cudaStream_t);
+template cudaError_t launch_prefix<128>(const Args&, const CUtensorMap&, const CUtensorMap&, cudaStream_t);
 
 }  // namespace shared_attn
 }  // namespace mesh

@@ -137,5 +137,5 @@ def attn_shared_prefix(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tens
     capturing = torch.cuda.is_current_stream_capturing()
     ext().attn_shared(q, kcache, vcache, block_tables, seq_lens, groups._meta, groups._po, groups._pml, out,
                       scratch(q.device).err, groups.item_cap if capturing else groups.n_items, groups._own_at, scale, window)
-    _count(2)
+    _count(2 + (capturing or groups.n_items > 0))
     return out
