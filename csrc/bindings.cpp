@@ -58,11 +58,11 @@ void kv_pages_move(at::Tensor& k_pool, at::Tensor& v_pool, const at::Tensor& src
                    const c10::optional<at::Tensor>& tokens, at::Tensor& err);
 void kv_pages_compact(at::Tensor& k_pool, at::Tensor& v_pool, const at::Tensor& tables, const at::Tensor& counts,
                       at::Tensor& out_tables, at::Tensor& ws, int64_t reserved, int64_t num_sms, at::Tensor& err);
-int64_t verify_parts_bytes(int64_t B, int64_t K, int64_t V);
-void verify_drafts(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& uniforms,
-                   const c10::optional<at::Tensor>& inv_t, const c10::optional<at::Tensor>& probs,
-                   const c10::optional<at::Tensor>& lens, at::Tensor& parts, at::Tensor& tokens, at::Tensor& accepted,
-                   at::Tensor& draft_p);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> verify_drafts(const at::Tensor& logits, const at::Tensor& ids,
+                                                             const at::Tensor& uniforms,
+                                                             const c10::optional<at::Tensor>& inv_t,
+                                                             const c10::optional<at::Tensor>& probs,
+                                                             const c10::optional<at::Tensor>& lens);
 void attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor& vcache, const at::Tensor& block_tables,
                  const at::Tensor& seq_lens, at::Tensor& meta, at::Tensor& po, at::Tensor& pml, at::Tensor& out,
                  at::Tensor& err, int64_t n_prefix, int64_t own_at, double scale, int64_t window);
@@ -123,7 +123,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "gather a session's KV pages (every layer) into a contiguous buffer, or scatter one into pages");
   m.def("kv_pages_move", &mesh::kv_pages_move, "copy pages (or their first tokens) inside the pools, every layer");
   m.def("kv_pages_compact", &mesh::kv_pages_compact, "move live pages to the front of the pools, rewrite block tables");
-  m.def("verify_parts_bytes", &mesh::verify_parts_bytes, "workspace bytes of verify_drafts");
   m.def("verify_drafts", &mesh::verify_drafts, "accept or replace drafted tokens against the target's probabilities");
   m.def("attn_shared", &mesh::attn_shared, "paged GQA decode attention with prefixes shared by groups of sequences");
   m.def("ar_fused_norm", &mesh::ar_fused_norm, "peer-memory all-reduce + residual + RMSNorm");

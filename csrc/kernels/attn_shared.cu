@@ -487,10 +487,10 @@ static cudaError_t launch(const Args& a, cudaStream_t st) {
   const CUtensorMap ok = D == 128 ? map3(a.k) : tk, ov = D == 128 ? map3(a.v) : tv;
   cudaError_t e = cudaSuccess;
   if (a.n_prefix > 0 && (e = launch_prefix<D>(a, tk, tv, st)) != cudaSuccess) return e;
-  auto kern = a.T * a.G <= 8 ? own_kernel<D, 1> : own_kernel<D, 2>;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<D>::smem(SHARED_MAX_BATCH));
-  if (e != cudaSuccess) return e;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  const bool narrow = a.T * a.G <= 8;
+  auto kern = narrow ? own_kernel<D, 1> : own_kernel<D, 2>;
+  static bool done[2][MAX_DEVICES] = {};
+  e = prepare_kernel(kern, (int)Geo<D>::smem(SHARED_MAX_BATCH), done[narrow]);
   if (e != cudaSuccess) return e;
   e = launch_k(kern, dim3((unsigned)(CTAS * a.num_sms)), dim3(WARPS * 32), Geo<D>::smem(a.B), st, ok, ov, a);
   if (e != cudaSuccess) return e;

@@ -26,6 +26,21 @@ __device__ __forceinline__ const int* members(const Args& a) { return a.meta + H
 __device__ __forceinline__ int* own_before(const Args& a) { return a.meta + HDR + 4 * a.B; }
 __device__ __forceinline__ const int* items(const Args& a) { return a.meta + shared_items_at(a.B); }
 
+// Once per device: the kernel's dynamic shared memory, and that the SM keeps all its shared memory, also what the kernel
+// itself does not use, so that a CTA of the other kernel can start beside it.
+constexpr int MAX_DEVICES = 64;
+template <typename Kern>
+inline cudaError_t prepare_kernel(Kern kern, int smem, bool (&done)[MAX_DEVICES]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < MAX_DEVICES && done[dev])) return e;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  if (e == cudaSuccess && dev < MAX_DEVICES) done[dev] = true;
+  return e;
+}
+
 // rows of a prefix item against its shared keys on tcgen05 (attn_shared_tc.cu)
 template <int D>
 cudaError_t launch_prefix(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st);

@@ -453,10 +453,8 @@ __global__ void __maxnreg__(MAX_REGS)
 template <int D>
 cudaError_t launch_prefix(const Args& a, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
   auto kern = prefix_kernel<D>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<D>());
-  if (e != cudaSuccess) return e;
-  // the SM keeps all its shared memory, also what this kernel does not use: the other kernel's CTA starts beside it
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  static bool done[MAX_DEVICES] = {};
+  const cudaError_t e = prepare_kernel(kern, (int)smem_bytes<D>(), done);
   if (e != cudaSuccess) return e;
   return launch_k(kern, dim3((unsigned)min(a.n_prefix, a.num_sms)), dim3(THREADS), smem_bytes<D>(), st, tk, tv, a);
 }

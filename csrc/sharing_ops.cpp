@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <climits>
 #include <string>
+#include <tuple>
 
 #include "include/sharing.h"
 
@@ -101,10 +102,12 @@ void kv_pages_compact(at::Tensor& k_pool, at::Tensor& v_pool, const at::Tensor& 
   C10_CUDA_CHECK(launch_kv_compact(a, at::cuda::getCurrentCUDAStream()));
 }
 
-void verify_drafts(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& uniforms,
-                   const c10::optional<at::Tensor>& inv_t, const c10::optional<at::Tensor>& probs,
-                   const c10::optional<at::Tensor>& lens, at::Tensor& parts, at::Tensor& tokens, at::Tensor& accepted,
-                   at::Tensor& draft_p) {
+// Returns (tokens [B, K+1] int32, accepted [B] int32, probs [B, K] fp32).
+std::tuple<at::Tensor, at::Tensor, at::Tensor> verify_drafts(const at::Tensor& logits, const at::Tensor& ids,
+                                                             const at::Tensor& uniforms,
+                                                             const c10::optional<at::Tensor>& inv_t,
+                                                             const c10::optional<at::Tensor>& probs,
+                                                             const c10::optional<at::Tensor>& lens) {
   const char* what = "verify_drafts";
   const at::Tensor& x = logits;
   TORCH_CHECK(x.is_cuda() && x.dim() == 3 && x.size(1) >= 1 && x.size(2) >= 1 && x.stride(2) == 1 &&
@@ -116,22 +119,20 @@ void verify_drafts(const at::Tensor& logits, const at::Tensor& ids, const at::Te
   check_tensor(what, "uniforms", uniforms, x, at::kFloat, {B, K + 1});
   if (inv_t.has_value()) check_tensor(what, "inv_t", *inv_t, x, at::kFloat, {B});
   if (lens.has_value()) check_tensor(what, "draft_lens", *lens, x, at::kInt, {B});
-  check_tensor(what, "tokens", tokens, x, at::kInt, {B, K + 1});
-  check_tensor(what, "accepted", accepted, x, at::kInt, {B});
-  check_tensor(what, "probs", draft_p, x, at::kFloat, {B, K});
   if (probs.has_value())
     TORCH_CHECK(probs->device() == x.device() && probs->dim() == 3 && probs->size(0) == B && probs->size(1) == K &&
                     probs->size(2) == V && probs->stride(2) == 1 &&
                     (probs->scalar_type() == at::kFloat || probs->scalar_type() == at::kBFloat16),
                 what, ": draft_probs [B, K, V] fp32 or bf16 on the logits' device, vocabulary contiguous");
-  if (B == 0) return;
   const bool qs = probs.has_value() && K > 0;
   TORCH_CHECK(V <= verify_max_vocab(), std::string(what) + ": a vocabulary of " + num(V) + ", at most " + num(verify_max_vocab()));
   TORCH_CHECK(B * (K + 1) <= 65535, std::string(what) + ": " + num(B * (K + 1)) + " rows, at most 65535");
-  TORCH_CHECK(parts.device() == x.device() && parts.is_contiguous() && (uintptr_t)parts.data_ptr() % 16 == 0 &&
-                  (int64_t)parts.nbytes() >= verify_parts_bytes(B, K, V),
-              what, ": workspace too small");
   const c10::cuda::CUDAGuard guard(x.device());
+  const auto ints = x.options().dtype(at::kInt);
+  at::Tensor tokens = at::empty({B, K + 1}, ints), accepted = at::empty({B}, ints);
+  at::Tensor draft_p = at::empty({B, K}, x.options().dtype(at::kFloat));
+  if (B == 0) return {tokens, accepted, draft_p};
+  at::Tensor parts = at::empty({verify_parts_bytes(B, K, V)}, x.options().dtype(at::kByte));
   VerifyArgs a;
   a.logits = x.data_ptr();
   a.ids = ids.data_ptr<int>();
@@ -154,6 +155,7 @@ void verify_drafts(const at::Tensor& logits, const at::Tensor& ids, const at::Te
   a.logits_bf16 = x.scalar_type() == at::kBFloat16;
   a.probs_bf16 = qs && probs->scalar_type() == at::kBFloat16;
   C10_CUDA_CHECK(launch_verify(a, at::cuda::getCurrentCUDAStream()));
+  return {tokens, accepted, draft_p};
 }
 
 void attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor& vcache, const at::Tensor& block_tables,

@@ -54,6 +54,8 @@ class PrefixGroups:
         self._po = torch.empty(slots * head_dim, dtype=torch.float32, device=self.device)
         self._pml = torch.empty(slots * 2, dtype=torch.float32, device=self.device)
         self._meta = torch.zeros(self._items_at + _ITEM * self.item_cap, dtype=torch.int32, device=self.device)
+        from . import scratch
+        self._err = scratch(self.device).err if self.device.type == "cuda" else None
         self.n_items = 0
         self.set([])
 
@@ -125,7 +127,7 @@ def attn_shared_prefix(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tens
     kcache, vcache [pages, hkv, page, D] bf16 (pages of a multiple of 16 tokens); block_tables [B, pages] and
     seq_lens [B] int32 as in ``attn_decode``, lengths including the new tokens. A token without any key gives
     zeros. ``window``: attend the last ``window`` keys only."""
-    from . import _count, ext, scratch
+    from . import _count, ext
     B, T = groups.batch, groups.q_len
     if seq_lens.shape[0] != B or q.shape[0] != B * T or q.shape[1] != groups.hq * groups.head_dim:
         raise ValueError(f"q {tuple(q.shape)} and {seq_lens.shape[0]} lengths do not fit groups of {B} sequences x {T} "
@@ -136,6 +138,6 @@ def attn_shared_prefix(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tens
         raise ValueError(f"groups on {groups.device}, q on {q.device}")
     capturing = torch.cuda.is_current_stream_capturing()
     ext().attn_shared(q, kcache, vcache, block_tables, seq_lens, groups._meta, groups._po, groups._pml, out,
-                      scratch(q.device).err, groups.item_cap if capturing else groups.n_items, groups._own_at, scale, window)
+                      groups._err, groups.item_cap if capturing else groups.n_items, groups._own_at, scale, window)
     _count(2 + (capturing or groups.n_items > 0))
     return out

@@ -26,15 +26,8 @@ def verify_drafts(logits: torch.Tensor, draft_ids: torch.Tensor, uniforms: torch
     Returns (tokens [B, K+1] int32: accepted drafts, the new token, then -1; accepted [B] int32; probs [B, K] fp32:
     the target's probability of each draft, 0 past a session's drafts)."""
     from . import _count, ext
-    E = ext()
     if logits.dim() != 3 or logits.shape[1] < 1:
         raise ValueError(f"logits [B, K+1, V] expected, got {tuple(logits.shape)}")
-    B, K1, V = logits.shape
-    dev = logits.device
-    tokens = torch.empty(B, K1, dtype=torch.int32, device=dev)
-    accepted = torch.empty(B, dtype=torch.int32, device=dev)
-    probs = torch.empty(B, K1 - 1, dtype=torch.float32, device=dev)
-    parts = torch.empty(E.verify_parts_bytes(B, K1 - 1, V), dtype=torch.uint8, device=dev)
-    E.verify_drafts(logits, draft_ids, uniforms, inv_t, draft_probs, draft_lens, parts, tokens, accepted, probs)
+    out = ext().verify_drafts(logits, draft_ids, uniforms, inv_t, draft_probs, draft_lens)
     _count(2)
-    return tokens, accepted, probs
+    return out
