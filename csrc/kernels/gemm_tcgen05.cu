@@ -1250,9 +1250,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       while (ok && itr.next(p, sg)) {
         int kb_start = sg.kb0;
         if (first_seg) {
-          // Operand A of the first stages (weights in decode) does not depend on the previous
-          // kernel: fetch it before waiting for that kernel's results, then fetch B.
+          // Operand A of the first stages, where it is the weights (TRANS), does not depend on the previous
+          // kernel: fetch it before waiting for that kernel's results, then fetch B. Otherwise A is what that
+          // kernel wrote, and waits.
           first_seg = false;
+          if (!TRANS) griddep_wait();
           const int npre = min(p.stages, sg.kb1 - sg.kb0);
           for (int i = 0; i < npre; ++i) {
             mbar_arrive_expect_tx(&s.full[i], a_stage_bytes + b_stage_bytes);
@@ -1260,7 +1262,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               tma_load_2d(s.a + (size_t)i * a_stage_bytes + j * a_box_bytes, &tmA, &s.full[i],
                           (sg.kb0 + i) * bk_eff + j * BK, sg.tm * BM, pol_a);
           }
-          griddep_wait();
+          if (TRANS) griddep_wait();
           if (trace) trace[1] = globaltimer_ns();
           for (int i = 0; i < npre; ++i)
             for (int j = 0; j < kbox; ++j)
