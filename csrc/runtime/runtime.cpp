@@ -1,6 +1,6 @@
 // Native host runtime of mesh_b200 (module mesh_b200._runtime, pybind11).
 //
-// * PageAllocator   - KV page pool free list (lowest ids first, double-free detection).
+// * PageAllocator   - KV page pool free list (lowest ids first, holder counts, double-free detection).
 // * DecodeScheduler - the fair decode queue and microbatch builder of the serving engine: tasks
 //   ordered by (decode_steps_served, fairness_epoch, session id); a batch starts from an optional
 //   primary session, then admits queued sessions that share the primary's execution class, stay
@@ -48,7 +48,7 @@ class PageAllocator {
     for (int64_t i = 0; i < n; ++i) {
       int64_t p = free_.top();
       free_.pop();
-      used_.insert(p);
+      used_.emplace(p, 1);
       out.push_back(p);
     }
     return py::cast(out);
@@ -57,9 +57,34 @@ class PageAllocator {
     for (int64_t p : pages) {
       auto it = used_.find(p);
       if (it == used_.end()) throw std::invalid_argument("double free or foreign page " + std::to_string(p));
+      if (--it->second > 0) continue;  // another holder keeps it
       used_.erase(it);
       free_.push(p);
     }
+  }
+  // One more holder for each of these pages (a forked session's); every holder frees them once.
+  void share(const std::vector<int64_t>& pages) {
+    for (int64_t p : pages)
+      if (!used_.count(p)) throw std::invalid_argument("page " + std::to_string(p) + " is not in use");
+    for (int64_t p : pages) ++used_[p];
+  }
+  int64_t refs(int64_t page) const {
+    auto it = used_.find(page);
+    return it == used_.end() ? 0 : it->second;
+  }
+  // After a compaction of the pool: page p is now remap[p]. Holders keep their counts; all other pages are free.
+  void remap(const std::vector<int64_t>& remap) {
+    if ((int64_t)remap.size() != num_pages_) throw std::invalid_argument("remap must cover the pool");
+    std::unordered_map<int64_t, int64_t> moved;
+    for (const auto& [p, n] : used_) {
+      const int64_t q = remap[p];
+      if (q < reserved_ || q >= num_pages_) throw std::invalid_argument("page " + std::to_string(p) + " is in use but has no new place");
+      if (!moved.emplace(q, n).second) throw std::invalid_argument("two pages moved to " + std::to_string(q));
+    }
+    used_.swap(moved);
+    free_ = {};
+    for (int64_t p = reserved_; p < num_pages_; ++p)
+      if (!used_.count(p)) free_.push(p);
   }
   int64_t num_free() const { return (int64_t)free_.size(); }
   int64_t num_used() const { return (int64_t)used_.size(); }
@@ -68,7 +93,7 @@ class PageAllocator {
  private:
   int64_t num_pages_, reserved_;
   std::priority_queue<int64_t, std::vector<int64_t>, std::greater<int64_t>> free_;
-  std::unordered_set<int64_t> used_;
+  std::unordered_map<int64_t, int64_t> used_;  // page -> holders
 };
 
 // ------------------------------------------------------------------------------------------------
@@ -318,6 +343,9 @@ PYBIND11_MODULE(_runtime, m) {
       .def(py::init<int64_t, int64_t>(), py::arg("num_pages"), py::arg("reserved") = 0)
       .def("alloc", &PageAllocator::alloc)
       .def("free", &PageAllocator::free)
+      .def("share", &PageAllocator::share)
+      .def("refs", &PageAllocator::refs)
+      .def("remap", &PageAllocator::remap)
       .def_property_readonly("num_free", &PageAllocator::num_free)
       .def_property_readonly("num_used", &PageAllocator::num_used)
       .def_property_readonly("capacity", &PageAllocator::capacity);

@@ -5,7 +5,8 @@ Per layer (reference ``forward_layer``, ``agent/src/inference/forward_pass.rs:19
     qkv   = tcgen05 GEMM(normed, wqkv)                    (swap-AB for decode-sized T)
     q     = RoPE(q); k,v -> paged KV pool                 (decode: in the qkv GEMM epilogue;
                                                           prefill: rope_kv_write)
-    attn  = paged GQA attention                           (decode: split-KV; prefill: flash)
+    attn  = paged GQA attention                           (decode: split-KV; prefill: flash; sessions that
+                                                          share pages or verify drafts: attn_shared_prefix)
     part  = tcgen05 GEMM(attn, wo)                        -> own slot of the symmetric workspace
     resid, normed = AR(part) + resid, RMSNorm(mlp_norm)   (ar_fused_norm over NVLink; TP=1: add_rmsnorm;
                                                           opt-in at decode: one launch, gemm_allreduce_norm)
@@ -86,6 +87,8 @@ class StepMeta:
     thr: Optional[torch.Tensor] = None
     nucleus: bool = True   # some row has 0 < top_p < 1 (the sampler's radix passes are needed)
     cu_host: Optional[List[int]] = None  # host copy of cu_q (prefill): lets the runner split the chunk
+    # sequences that share a prefix, and several new tokens a sequence (ops.PrefixGroups); None = ops.attn_decode
+    groups: Optional["ops.PrefixGroups"] = None
 
 
 class LlamaRunner:
@@ -264,7 +267,9 @@ class LlamaRunner:
         qkv, q, attn, h = scr
         kc, vc = self.kv.k[li], self.kv.v[li]
         ops.qkv_rope(normed, L.wqkv, m.pos, m.slot, self.cos, self.sin, q, kc, vc, self.hq, self.hkv, qkv_buf=qkv)
-        if m.decode:
+        if m.groups is not None:
+            ops.attn_shared_prefix(q, kc, vc, m.block_tables, m.seq_lens, m.groups, attn, self.scale, self.window)
+        elif m.decode:
             ops.attn_decode(q, kc, vc, m.block_tables, m.seq_lens, attn, self.scale, self.window,
                             max_len_hint=m.max_q_len)
         else:

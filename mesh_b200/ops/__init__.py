@@ -415,4 +415,4 @@ def rope_tables(head_dim: int, base: float, max_pos: int, device) -> tuple:
 
 
 from .shared_prefix import PrefixGroups, attn_shared_prefix  # noqa: E402,F401
-from .speculative import verify_drafts  # noqa: E402,F401
+from .speculative import VERIFY_MAX_DRAFTS, verify_drafts  # noqa: E402,F401

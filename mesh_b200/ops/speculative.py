@@ -5,6 +5,8 @@ from typing import Optional, Tuple
 
 import torch
 
+VERIFY_MAX_DRAFTS = 31  # drafts a session, as in the kernel
+
 
 def verify_drafts(logits: torch.Tensor, draft_ids: torch.Tensor, uniforms: torch.Tensor,
                   inv_t: Optional[torch.Tensor] = None, draft_probs: Optional[torch.Tensor] = None,
