@@ -56,8 +56,10 @@ void embed_peer_norm(const at::Tensor& bases, const at::Tensor& ids, int64_t V, 
 void kv_pages_copy(at::Tensor& k_pool, at::Tensor& v_pool, at::Tensor& buf, const at::Tensor& pages, bool to_buf);
 void kv_pages_move(at::Tensor& k_pool, at::Tensor& v_pool, const at::Tensor& src, const at::Tensor& dst,
                    const c10::optional<at::Tensor>& tokens, at::Tensor& err);
-void kv_pages_compact(at::Tensor& k_pool, at::Tensor& v_pool, const at::Tensor& tables, const at::Tensor& counts,
-                      at::Tensor& out_tables, at::Tensor& ws, int64_t reserved, int64_t num_sms, at::Tensor& err);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> kv_pages_compact(at::Tensor& k_pool, at::Tensor& v_pool,
+                                                                const at::Tensor& tables, const at::Tensor& counts,
+                                                                const c10::optional<at::Tensor>& out, int64_t reserved,
+                                                                at::Tensor& err);
 std::tuple<at::Tensor, at::Tensor, at::Tensor> verify_drafts(const at::Tensor& logits, const at::Tensor& ids,
                                                              const at::Tensor& uniforms,
                                                              const c10::optional<at::Tensor>& inv_t,

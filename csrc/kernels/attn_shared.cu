@@ -13,6 +13,9 @@
 //
 // The item list is made on the host when the groups change (PrefixGroups) and lives in device memory, so a
 // captured step follows later changes of groups, lengths and tables.
+#include <cstdlib>
+#include <type_traits>
+
 #include "attn_shared.cuh"
 
 namespace mesh {
@@ -21,7 +24,6 @@ namespace {
 
 constexpr int WARPS = 4;         // workers of a CTA
 constexpr int CTAS = 3;          // per SM; one beside a CTA of the prefix kernel
-constexpr int TILE_ROWS = 16;    // query rows of a worker
 constexpr int PIECE_COST = 2;    // what a piece costs besides its slices, in slices
 constexpr int MIN_QUOTA = 4;     // units (slices and piece costs) a worker takes at least
 
@@ -122,6 +124,7 @@ __device__ __forceinline__ void own_worker(const CUtensorMap& tmK, const CUtenso
                                            uint8_t* ring, uint64_t* full, int lane, int worker, int workers) {
   using g = Geo<D>;
   constexpr int SLOTS = g::SLOTS;
+  constexpr int TILE_ROWS = 8 * NT;
   const int rows = a.T * a.G, hq = a.hkv * a.G, tiles = (rows + TILE_ROWS - 1) / TILE_ROWS;
   const int per_seq = a.hkv * tiles;
   const int total = seqs[a.B].before * per_seq;
@@ -408,69 +411,72 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : CTAS) own_kernel(con
   if (a.n_prefix != 0 && blockIdx.x == gridDim.x - 1) griddep_wait();
 }
 
-// One warp per row (sequence, token, head): merge its partials, the prefix's first, in order. Lane i holds the (m, l) of
-// partial i (of the current 32), so the weights are known before the outputs arrive and eight of those are in flight
-// at a time.
+// One warp per row (sequence, token, head): merge its partials, the prefix's first, in order. Bound by latency, not by the
+// bytes: lane i asks for the (m, l) of partial i and the warp for all of its first 16 outputs at once, weights follow.
 template <int D>
 __global__ void __launch_bounds__(128) combine_kernel(const Args a) {
+  constexpr int V = D / 32, U = 16;
+  using Vec = typename std::conditional<V == 4, float4, float2>::type;
+  const int lane = threadIdx.x & 31, hq = a.hkv * a.G, rows = a.T * a.G;
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 5);  // (b * T + t) * hq + head
+  const int b = min(row / (a.T * hq), a.B - 1);
+  const int x = row - b * a.T * hq, t = x / hq, head = x - t * hq, h = head / a.G;
+  // written by the host alone, not by a kernel that this grid may overlap
+  int n_prefix = seq_prefix_slots(a, b);
+  const int base = seq_base(a, b) + x * n_prefix;
   griddep_wait();
   griddep_launch_dependents();
-  constexpr int V = D / 32, U = 8;
-  const int lane = threadIdx.x & 31, hq = a.hkv * a.G, rows = a.T * a.G;
-  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 5);  // (b * T + t) * hq + head
-  if (row >= (long)a.B * a.T * hq) return;
-  const int b = (int)(row / (a.T * hq));
-  const int x = (int)(row - (long)b * a.T * hq), t = x / hq, head = x - t * hq, h = head / a.G;
+  if (row >= a.B * a.T * hq) return;
   const int before = own_before(a)[b], units = own_before(a)[b + 1] - before, quota = own_before(a)[a.B + 1];
-  int n_prefix = seq_prefix_slots(a, b);
-  const long base = (long)seq_base(a, b) + (long)x * n_prefix;
   // the workers whose quotas this row's slices fall into
-  const int r = t * a.G + (head - h * a.G), tile = r / TILE_ROWS, tiles = (rows + TILE_ROWS - 1) / TILE_ROWS;
-  const int u = h * tiles + tile, stride = min(rows, TILE_ROWS);
+  const int r = t * a.G + (head - h * a.G), tile = r / a.tile_rows, tiles = (rows + a.tile_rows - 1) / a.tile_rows;
+  const int u = h * tiles + tile, stride = min(rows, a.tile_rows);
   const int at = before * a.hkv * tiles + u * units + PIECE_COST;  // its first slice
   const int w0 = at / quota;
   int n_own = units > 0 ? (at + units - PIECE_COST - 1) / quota - w0 + 1 : 0;
   if (n_prefix == 0 && n_own == 1) return;  // already written
-  const long own = a.own_at + (long)(w0 + b * a.hkv * tiles + u) * stride + (r - tile * TILE_ROWS);  // pieces are `stride` apart
+  const long own = a.own_at + (long)(w0 + b * a.hkv * tiles + u) * stride + (r - tile * a.tile_rows);  // pieces are `stride` apart
   if (base < 0 || base + n_prefix > a.own_at || (n_own > 0 && own + (long)(n_own - 1) * stride >= a.slot_cap)) {
     if (lane == 0) record_error(a.err, ERR_BAD_ARGUMENT);
     n_prefix = n_own = 0;
   }
   const int n = n_prefix + n_own;
-  auto slot = [&](int i) { return i < n_prefix ? base + i : own + (long)(i - n_prefix) * stride; };
+  auto slot = [&](int i) { return i < n_prefix ? base + (long)i : own + (long)(i - n_prefix) * stride; };
   float acc[V] = {}, den = 0.f, M = -INFINITY;
-  for (int i = lane; i < n; i += 32) M = fmaxf(M, a.pml[slot(i)].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  for (int i0 = 0; i0 < n && M > -INFINITY; i0 += 32) {
+  for (int i0 = 0; i0 < n; i0 += 32) {
     const float2 ml = i0 + lane < n ? a.pml[slot(i0 + lane)] : make_float2(-INFINITY, 0.f);
-    const float f = ex2_ftz(ml.x - M);  // 0 for a partial that saw nothing; its output may not have been written
-    den += ml.x > -INFINITY ? ml.y * f : 0.f;
+    float p[U][V];
+    auto load = [&](int i) {
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (i + k < n) *reinterpret_cast<Vec*>(p[k]) = *reinterpret_cast<const Vec*>(a.po + slot(i + k) * D + lane * V);
+    };
+    load(i0);
+    float mx = ml.x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float mn = fmaxf(M, mx);
+    if (mn == -INFINITY) continue;
+    const float corr = ex2_ftz(M - mn), f = ex2_ftz(ml.x - mn);  // 0 for a partial that saw nothing
+    M = mn;
+    den = den * corr + (ml.x > -INFINITY ? ml.y * f : 0.f);
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] *= corr;
     for (int i = i0; i < min(n, i0 + 32); i += U) {
-      float p[U][V], w[U];
+      if (i > i0) load(i);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        w[u] = __shfl_sync(0xffffffffu, f, (i + u) & 31);
+      for (int k = 0; k < U; ++k) {
+        const float w = __shfl_sync(0xffffffffu, f, (i + k) & 31);
+        if (i + k < n && w > 0.f)  // the output of a partial that saw nothing may not have been written
 #pragma unroll
-        for (int v = 0; v < V; ++v) p[u][v] = 0.f;
-        if (i + u < n && w[u] > 0.f) {
-          const float* src = a.po + slot(i + u) * D + lane * V;
-          if constexpr (V == 4)
-            *reinterpret_cast<float4*>(p[u]) = *reinterpret_cast<const float4*>(src);
-          else
-            *reinterpret_cast<float2*>(p[u]) = *reinterpret_cast<const float2*>(src);
-        }
+          for (int v = 0; v < V; ++v) acc[v] = fmaf(p[k][v], w, acc[v]);
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] = fmaf(p[u][v], w[u], acc[v]);
     }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
   const float inv = den > 0.f ? 1.f / den : 0.f;
-  __nv_bfloat16* dst = a.out + row * D + lane * V;
+  __nv_bfloat16* dst = a.out + (long)row * D + lane * V;
 #pragma unroll
   for (int v = 0; v < V; v += 2) *reinterpret_cast<uint32_t*>(dst + v) = pack_bf16x2(acc[v] * inv, acc[v + 1] * inv);
 }
@@ -487,12 +493,12 @@ static cudaError_t launch(const Args& a, cudaStream_t st) {
   const CUtensorMap ok = D == 128 ? map3(a.k) : tk, ov = D == 128 ? map3(a.v) : tv;
   cudaError_t e = cudaSuccess;
   if (a.n_prefix > 0 && (e = launch_prefix<D>(a, tk, tv, st)) != cudaSuccess) return e;
-  const bool narrow = a.T * a.G <= 8;
+  const bool narrow = a.tile_rows == 8;
   auto kern = narrow ? own_kernel<D, 1> : own_kernel<D, 2>;
   static bool done[2][MAX_DEVICES] = {};
   e = prepare_kernel(kern, (int)Geo<D>::smem(SHARED_MAX_BATCH), done[narrow]);
   if (e != cudaSuccess) return e;
-  e = launch_k(kern, dim3((unsigned)(CTAS * a.num_sms)), dim3(WARPS * 32), Geo<D>::smem(a.B), st, ok, ov, a);
+  e = launch_k(kern, dim3((unsigned)((getenv("CT")?atoi(getenv("CT")):3) * a.num_sms)), dim3(WARPS * 32), Geo<D>::smem(a.B), st, ok, ov, a);
   if (e != cudaSuccess) return e;
   const long out_rows = (long)a.B * a.T * a.hkv * a.G;
   return launch_k(combine_kernel<D>, dim3((unsigned)((out_rows + 3) / 4)), dim3(128), 0, st, a);
@@ -505,6 +511,7 @@ cudaError_t launch_attn_shared(const SharedAttnArgs& x, int head_dim, double sca
   static_cast<SharedAttnArgs&>(a) = x;
   a.slices_per_page = x.page_size / shared_attn::SLICE;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
+  a.tile_rows = 8;
   return head_dim == 128 ? shared_attn::launch<128>(a, st) : shared_attn::launch<64>(a, st);
 }
 

@@ -70,20 +70,23 @@ void kv_pages_move(at::Tensor& k_pool, at::Tensor& v_pool, const at::Tensor& src
   C10_CUDA_CHECK(launch_kv_move(a, at::cuda::getCurrentCUDAStream()));
 }
 
-void kv_pages_compact(at::Tensor& k_pool, at::Tensor& v_pool, const at::Tensor& tables, const at::Tensor& counts,
-                      at::Tensor& out_tables, at::Tensor& ws, int64_t reserved, int64_t num_sms, at::Tensor& err) {
+// Returns (tables, remap [pages], live [1]).
+std::tuple<at::Tensor, at::Tensor, at::Tensor> kv_pages_compact(at::Tensor& k_pool, at::Tensor& v_pool,
+                                                                const at::Tensor& tables, const at::Tensor& counts,
+                                                                const c10::optional<at::Tensor>& out, int64_t reserved,
+                                                                at::Tensor& err) {
   check_pools("kv_pages_compact", k_pool, v_pool);
   TORCH_CHECK(tables.dim() == 2, "kv_pages_compact: block tables [rows, width]");
   const int64_t pages = k_pool.size(1), rows = tables.size(0), width = tables.size(1);
   check_tensor("kv_pages_compact", "block tables", tables, k_pool, at::kInt, {rows, width});
-  check_tensor("kv_pages_compact", "out_tables", out_tables, k_pool, at::kInt, {rows, width});
+  if (out.has_value()) check_tensor("kv_pages_compact", "out_tables", *out, k_pool, at::kInt, {rows, width});
   check_tensor("kv_pages_compact", "counts", counts, k_pool, at::kInt, {rows});
   TORCH_CHECK(reserved >= 0 && reserved <= pages, "kv_pages_compact: " + num(reserved) + " reserved pages in a pool of " + num(pages));
-  TORCH_CHECK(ws.device() == k_pool.device() && ws.scalar_type() == at::kInt && ws.is_contiguous() && ws.numel() >= 3 * pages + 2,
-              "kv_pages_compact: workspace of 3 * pages + 2");
   TORCH_CHECK(kv_compact_smem(pages) <= 200 * 1024, "kv_pages_compact: at most 819200 pages");
   TORCH_CHECK(rows < INT_MAX && width < INT_MAX, "kv_pages_compact: tables too large");
   const c10::cuda::CUDAGuard guard(k_pool.device());
+  at::Tensor out_tables = out.has_value() ? *out : at::empty({rows, width}, tables.options());
+  at::Tensor ws = at::empty({3 * pages + 2}, tables.options());
   KvCompactArgs a;
   a.k = k_pool.data_ptr();
   a.v = v_pool.data_ptr();
@@ -96,10 +99,11 @@ void kv_pages_compact(at::Tensor& k_pool, at::Tensor& v_pool, const at::Tensor& 
   a.width = (int)width;
   a.layers = (int)k_pool.size(0);
   a.reserved = (int)reserved;
-  a.num_sms = (int)num_sms;
+  a.num_sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   a.pool_pages = pages;
   a.page_vec = k_pool.size(2) * k_pool.size(3) * (k_pool.size(4) / 8);
   C10_CUDA_CHECK(launch_kv_compact(a, at::cuda::getCurrentCUDAStream()));
+  return {out_tables, ws.narrow(0, 0, pages), ws.narrow(0, pages, 1)};
 }
 
 // Returns (tokens [B, K+1] int32, accepted [B] int32, probs [B, K] fp32).
@@ -189,7 +193,7 @@ void attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor
                   pml.device() == q.device() && po.numel() / D <= pml.numel() / 2,
               what, ": workspace");
   TORCH_CHECK(B <= SHARED_MAX_BATCH, std::string(what) + ": a batch of " + num(B) + ", at most " + num(SHARED_MAX_BATCH));
-  const int64_t own_slots = (12 * at::cuda::getDeviceProperties(q.get_device())->multiProcessorCount + B * hkv * ((T * G + 15) / 16)) *
+  const int64_t own_slots = (12 * at::cuda::getDeviceProperties(q.get_device())->multiProcessorCount + B * hkv * ((T * G + 7) / 8)) *
                             std::min<int64_t>(16, T * G);
   TORCH_CHECK(own_at >= 0 && (own_at + own_slots) * D <= po.numel(), what, ": workspace too small");
   TORCH_CHECK(kcache.size(0) * hkv * ps < (1ll << 31), what, ": KV pool too large for 32-bit TMA rows");

@@ -373,14 +373,9 @@ def kv_pages_compact(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: t
     move, in order, into the holes below n, so the fewest pages move. Returns (tables, remap, live): the tables
     with new ids (entries past a row's count unchanged; in ``out_tables`` if given, which may be ``block_tables``),
     the new id of every page ([pages] int32, -1: free) and n ([1] int32). Nothing is read back by the host."""
-    pages = k_pool.shape[1]
-    if out_tables is None:
-        out_tables = torch.empty_like(block_tables)
-    ws = torch.empty(3 * pages + 2, dtype=torch.int32, device=k_pool.device)
-    s = scratch(k_pool.device)
-    ext().kv_pages_compact(k_pool, v_pool, block_tables, counts, out_tables, ws, reserved, s.num_sms, s.err)
+    out = ext().kv_pages_compact(k_pool, v_pool, block_tables, counts, out_tables, reserved, scratch(k_pool.device).err)
     _count(2)
-    return out_tables, ws[:pages], ws[pages:pages + 1]
+    return out
 
 
 def argmax_partial(logits: torch.Tensor, vocab_offset: int, out: torch.Tensor):

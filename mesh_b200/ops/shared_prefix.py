@@ -50,7 +50,7 @@ class PrefixGroups:
         # that the keys behind the prefixes are cut into
         self._own_at = _TILE * sms + rows * hq
         own_rows = q_len * self.group
-        slots = self._own_at + (12 * sms + batch * hkv * -(-own_rows // 16)) * min(16, own_rows)
+        slots = self._own_at + (12 * sms + batch * hkv * -(-own_rows // 8)) * min(16, own_rows)
         self._po = torch.empty(slots * head_dim, dtype=torch.float32, device=self.device)
         self._pml = torch.empty(slots * 2, dtype=torch.float32, device=self.device)
         self._meta = torch.zeros(self._items_at + _ITEM * self.item_cap, dtype=torch.int32, device=self.device)
