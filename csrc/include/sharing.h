@@ -53,6 +53,8 @@ int64_t verify_parts_bytes(int64_t B, int64_t K, int64_t V);
 cudaError_t launch_verify(const VerifyArgs& a, cudaStream_t st);
 
 // Attention over shared prefixes.
+constexpr int SHARED_OWN_ROWS = 8;   // query rows of one worker on a sequence's own keys
+constexpr int SHARED_OWN_WORKERS = 12;  // such workers per SM at most
 constexpr int SHARED_MAX_ROWS = 64;  // query rows (new tokens x heads of a KV group) of one sequence
 constexpr int SHARED_HDR = 8;        // header ints of meta, [0] = number of prefix items
 constexpr int SHARED_ITEM = 8;       // ints per prefix item

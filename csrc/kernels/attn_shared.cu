@@ -13,7 +13,6 @@
 //
 // The item list is made on the host when the groups change (PrefixGroups) and lives in device memory, so a
 // captured step follows later changes of groups, lengths and tables.
-#include <cstdlib>
 #include <type_traits>
 
 #include "attn_shared.cuh"
@@ -23,7 +22,17 @@ namespace shared_attn {
 namespace {
 
 constexpr int WARPS = 4;         // workers of a CTA
-constexpr int CTAS = 3;          // per SM; one beside a CTA of the prefix kernel
+// CTAs per SM. Nothing shared: two (64 KB of rings in flight each; 64 sessions of up to 512 keys 19.9 us, one 26.9,
+// three 23.3; 128 of up to 2048 keys 99.3, 141, 100).
+// Beside the prefix kernel one CTA finds room at a time. Up to LIGHT units an SM one is also the faster: more cut the
+// keys into more partials (16 sessions of up to 512 own keys behind 2048 16.1 us, three 20.9; 64 behind 8192, 69 units,
+// 36.4 and 36.9). With more to do, those that start when the prefix kernel's leave read the rest faster (96 behind 8192,
+// 98 units, 46.9 with one and 45.2 with three; 64 of up to 2048 behind 2048 67.4 and 59.4; 256 of them 274 and 204).
+// The lengths are known here, not on the host: three are launched, and two leave at once where one is to do it all,
+// which costs less than the timing shows.
+constexpr int CTAS_ALONE = 2, CTAS_SHARED = 3, LIGHT = 80;
+static_assert(CTAS_SHARED * WARPS <= SHARED_OWN_WORKERS, "partials are reserved for fewer workers");
+constexpr int TILE_ROWS = SHARED_OWN_ROWS;
 constexpr int PIECE_COST = 2;    // what a piece costs besides its slices, in slices
 constexpr int MIN_QUOTA = 4;     // units (slices and piece costs) a worker takes at least
 
@@ -108,7 +117,7 @@ __device__ __forceinline__ void own_sequences(const Args& a, Seq* seqs, int tid,
   sync();
 }
 
-// The keys behind the shared prefixes: 16 rows (new tokens x heads of a KV group) of one sequence against that sequence's
+// The keys behind the shared prefixes: 8 rows (new tokens x heads of a KV group) of one sequence against that sequence's
 // own slices of 16 keys. All of them, in the order (sequence, KV head, tile of rows, slice), are cut into equal quotas,
 // one per warp: lengths from one token to long ones then keep every SM as busy. A quota is a run of
 // pieces, one for each (sequence, head, tile) it touches; a piece counts as PIECE_COST slices besides its own, about
@@ -117,14 +126,15 @@ __device__ __forceinline__ void own_sequences(const Args& a, Seq* seqs, int tid,
 // warps; four warps that split each piece and merged it took twice as long (64 sessions of up to 512 keys). Bound by
 // reading K and V.
 // The products run transposed, S^T = K Q^T and O^T = V^T P^T on m16n8k16 fragments, so that the few query rows are the
-// narrow side: NT tiles of 8 rows. With the rows on the 16-wide side half of every product and of the accumulators
-// would be padding (168 registers, so no CTA fitted beside the prefix kernel's).
-template <int D, int NT>
+// narrow side. With the rows on the 16-wide side half of every product and of the accumulators would be padding (168
+// registers, so no CTA fitted beside the prefix kernel's). More than 8 rows are cut into tiles, each reading the keys
+// again, mostly from L2: one worker for two tiles needs those registers too and was slower at every size (20 rows, 16
+// sessions, 8192 shared keys: 46.9 us, tiles 41.9; 16 rows, 64 sessions of 512 keys 36.3 and 31.1).
+template <int D>
 __device__ __forceinline__ void own_worker(const CUtensorMap& tmK, const CUtensorMap& tmV, const Args& a, const Seq* seqs,
                                            uint8_t* ring, uint64_t* full, int lane, int worker, int workers) {
   using g = Geo<D>;
   constexpr int SLOTS = g::SLOTS;
-  constexpr int TILE_ROWS = 8 * NT;
   const int rows = a.T * a.G, hq = a.hkv * a.G, tiles = (rows + TILE_ROWS - 1) / TILE_ROWS;
   const int per_seq = a.hkv * tiles;
   const int total = seqs[a.B].before * per_seq;
@@ -235,36 +245,28 @@ __device__ __forceinline__ void own_worker(const CUtensorMap& tmK, const CUtenso
       const int h = p.u / tiles, row0 = (p.u - h * tiles) * TILE_ROWS, n_rows = min(TILE_ROWS, rows - row0);
       const int s0 = q.first / SLICE + p.sl;
       const int k0 = max(q.first, s0 * SLICE), k1 = min(q.L, (s0 + p.n) * SLICE);
-      // query fragments straight from memory: row lane / 4 of each tile, columns (lane % 4) * 2 and 8 to the right
-      uint32_t qf[NT][D / 16][2];
+      // query fragments straight from memory: row lane / 4, columns (lane % 4) * 2 and 8 to the right
+      uint32_t qf[D / 16][2];
+      const int r = lane >> 2, x = row0 + min(r, n_rows - 1), t = x / a.G;
+      const __nv_bfloat16* src = a.q + ((long)(p.b * a.T + t) * hq + h * a.G + x - t * a.G) * D + (lane & 3) * 2;
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int r = (lane >> 2) + 8 * j, x = row0 + min(r, n_rows - 1), t = x / a.G;
-        const __nv_bfloat16* src = a.q + ((long)(p.b * a.T + t) * hq + h * a.G + x - t * a.G) * D + (lane & 3) * 2;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          qf[j][kk][0] = r < n_rows ? *reinterpret_cast<const uint32_t*>(src + kk * 16) : 0u;
-          qf[j][kk][1] = r < n_rows ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8) : 0u;
-        }
+      for (int kk = 0; kk < D / 16; ++kk) {
+        qf[kk][0] = r < n_rows ? *reinterpret_cast<const uint32_t*>(src + kk * 16) : 0u;
+        qf[kk][1] = r < n_rows ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8) : 0u;
       }
-      int hi_k[NT][2], lo_k[NT][2];  // keys that this lane's rows (lane % 4) * 2 + i of each tile may attend: [lo_k, hi_k)
+      int hi_k[2], lo_k[2];  // keys that this lane's rows (lane % 4) * 2 + i may attend: [lo_k, hi_k)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = (lane & 3) * 2 + i + 8 * j, pos = q.L - a.T + (row0 + r) / a.G;
-          hi_k[j][i] = r < n_rows ? min(k1, pos + 1) : 0;
-          lo_k[j][i] = a.window > 0 ? max(k0, pos + 1 - a.window) : k0;
-        }
-      float o[NT][D / 16][4];  // [tile][16 columns of the head]: columns lane / 4 and 8 below, rows (lane % 4) * 2 + {0, 1}
-      float m[NT][2], l[NT][2];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-#pragma unroll
-        for (int x = 0; x < D / 16; ++x) o[j][x][0] = o[j][x][1] = o[j][x][2] = o[j][x][3] = 0.f;
-        m[j][0] = m[j][1] = -INFINITY;
-        l[j][0] = l[j][1] = 0.f;
+      for (int i = 0; i < 2; ++i) {
+        const int r = (lane & 3) * 2 + i, pos = q.L - a.T + (row0 + r) / a.G;
+        hi_k[i] = r < n_rows ? min(k1, pos + 1) : 0;
+        lo_k[i] = a.window > 0 ? max(k0, pos + 1 - a.window) : k0;
       }
+      float o[D / 16][4];  // [16 columns of the head]: columns lane / 4 and 8 below, rows (lane % 4) * 2 + {0, 1}
+      float m[2], l[2];
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) o[x][0] = o[x][1] = o[x][2] = o[x][3] = 0.f;
+      m[0] = m[1] = -INFINITY;
+      l[0] = l[1] = 0.f;
 #pragma unroll 1
       for (int i = 0; i < p.n; ++i) {
         ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(&full[s], ph, a.err, ERR_MBAR_TIMEOUT_MMA, nullptr, WAIT_NS));
@@ -280,46 +282,40 @@ __device__ __forceinline__ void own_worker(const CUtensorMap& tmK, const CUtenso
           const int left = k1 - (key0 + x * 8 + (lane & 3) * 2);  // of this lane's two keys
           keep[x] = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
         }
-        float sc[NT][4], sd[NT][4];  // keys lane / 4 and 8 below; two chains of products each
+        float sc[4], sd[4];  // keys lane / 4 and 8 below; two chains of products each
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[j][e] = sd[j][e] = 0.f;
+        for (int e = 0; e < 4; ++e) sc[e] = sd[e] = 0.f;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           uint32_t kf[4];
           ldsm_x4(kb + (kk >> 2) * g::BOX + swz((lane & 7) + ((lane >> 3) & 1) * 8, (kk & 3) * 2 + (lane >> 4)), kf);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) mma((kk & 1) ? sd[j] : sc[j], kf, qf[j][kk][0], qf[j][kk][1]);
+          mma((kk & 1) ? sd : sc, kf, qf[kk][0], qf[kk][1]);
         }
-        uint32_t pf[NT][2];
+        uint32_t pf[2];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
+        for (int i = 0; i < 2; ++i) {
+          const int key = key0 + (lane >> 2);
+          const bool in0 = key < hi_k[i] && key >= lo_k[i], in1 = key + 8 < hi_k[i] && key + 8 >= lo_k[i];
+          const float s0v = in0 ? (sc[i] + sd[i]) * a.scale_log2 : -INFINITY;
+          const float s1v = in1 ? (sc[2 + i] + sd[2 + i]) * a.scale_log2 : -INFINITY;
+          float mx = fmaxf(s0v, s1v);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int key = key0 + (lane >> 2);
-            const bool in0 = key < hi_k[j][i] && key >= lo_k[j][i], in1 = key + 8 < hi_k[j][i] && key + 8 >= lo_k[j][i];
-            const float s0v = in0 ? (sc[j][i] + sd[j][i]) * a.scale_log2 : -INFINITY;
-            const float s1v = in1 ? (sc[j][2 + i] + sd[j][2 + i]) * a.scale_log2 : -INFINITY;
-            float mx = fmaxf(s0v, s1v);
+          for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+          const float mn = fmaxf(m[i], mx), mb = mn == -INFINITY ? 0.f : mn;
+          const float corr = ex2_ftz(m[i] - mb);
+          sc[i] = ex2_ftz(s0v - mb);
+          sc[2 + i] = ex2_ftz(s1v - mb);
+          l[i] = l[i] * corr + (sc[i] + sc[2 + i]);
+          m[i] = mn;
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-            const float mn = fmaxf(m[j][i], mx), mb = mn == -INFINITY ? 0.f : mn;
-            const float corr = ex2_ftz(m[j][i] - mb);
-            sc[j][i] = ex2_ftz(s0v - mb);
-            sc[j][2 + i] = ex2_ftz(s1v - mb);
-            l[j][i] = l[j][i] * corr + (sc[j][i] + sc[j][2 + i]);
-            m[j][i] = mn;
-#pragma unroll
-            for (int x = 0; x < D / 16; ++x) {
-              o[j][x][i] *= corr;
-              o[j][x][2 + i] *= corr;
-            }
+          for (int x = 0; x < D / 16; ++x) {
+            o[x][i] *= corr;
+            o[x][2 + i] *= corr;
           }
-          // the weights are rounded to bf16 for the product (half a step of 2^-8 each); their sum keeps fp32
-          pf[j][0] = transposed(pack_bf16x2(sc[j][0], sc[j][1]));
-          pf[j][1] = transposed(pack_bf16x2(sc[j][2], sc[j][3]));
         }
+        // the weights are rounded to bf16 for the product (half a step of 2^-8 each); their sum keeps fp32
+        pf[0] = transposed(pack_bf16x2(sc[0], sc[1]));
+        pf[1] = transposed(pack_bf16x2(sc[2], sc[3]));
 #pragma unroll
         for (int x = 0; x < D / 16; ++x) {
           uint32_t vf[4];
@@ -328,8 +324,7 @@ __device__ __forceinline__ void own_worker(const CUtensorMap& tmK, const CUtenso
           vf[1] &= keep[0];
           vf[2] &= keep[1];
           vf[3] &= keep[1];
-#pragma unroll
-          for (int j = 0; j < NT; ++j) mma(o[j][x], vf, pf[j][0], pf[j][1]);
+          mma(o[x], vf, pf[0], pf[1]);
         }
         // the products above have taken every fragment of this slot, so it may be filled again
         __syncwarp();
@@ -340,11 +335,9 @@ __device__ __forceinline__ void own_worker(const CUtensorMap& tmK, const CUtenso
         }
       }
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) l[j][i] += __shfl_xor_sync(0xffffffffu, l[j][i], x);
+        for (int x = 4; x < 32; x <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
       // a sequence without a prefix whose keys are all in this piece is done: its rows go out; else a partial
       const bool whole = p.n == q.slices() && q.slots == 0;
       const int stride = min(rows, TILE_ROWS);
@@ -354,26 +347,24 @@ __device__ __forceinline__ void own_worker(const CUtensorMap& tmK, const CUtenso
         continue;
       }
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+      for (int i = 0; i < 2; ++i) {
+        const int r = (lane & 3) * 2 + i;
+        if (r >= n_rows) continue;
+        const int x0 = row0 + r, t = x0 / a.G;
+        __nv_bfloat16* out = a.out + ((long)(p.b * a.T + t) * hq + h * a.G + x0 - t * a.G) * D + (lane >> 2);
+        float* po = a.po + (part + r) * D + (lane >> 2);
+        const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = (lane & 3) * 2 + i + 8 * j;
-          if (r >= n_rows) continue;
-          const int x0 = row0 + r, t = x0 / a.G;
-          __nv_bfloat16* out = a.out + ((long)(p.b * a.T + t) * hq + h * a.G + x0 - t * a.G) * D + (lane >> 2);
-          float* po = a.po + (part + r) * D + (lane >> 2);
-          const float inv = l[j][i] > 0.f ? 1.f / l[j][i] : 0.f;
+        for (int x = 0; x < D / 16; ++x)
 #pragma unroll
-          for (int x = 0; x < D / 16; ++x)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              if (whole)
-                out[x * 16 + e * 8] = f2bf(o[j][x][2 * e + i] * inv);
-              else
-                po[x * 16 + e * 8] = o[j][x][2 * e + i];
-            }
-          if (!whole && lane < 4) a.pml[part + r] = make_float2(m[j][i], l[j][i]);
-        }
+          for (int e = 0; e < 2; ++e) {
+            if (whole)
+              out[x * 16 + e * 8] = f2bf(o[x][2 * e + i] * inv);
+            else
+              po[x * 16 + e * 8] = o[x][2 * e + i];
+          }
+        if (!whole && lane < 4) a.pml[part + r] = make_float2(m[i], l[i]);
+      }
     }
     if (!ok) {
       // the copies still in flight land before the warp goes (bounded)
@@ -384,9 +375,9 @@ __device__ __forceinline__ void own_worker(const CUtensorMap& tmK, const CUtenso
   }
 }
 
-// Three CTAs an SM; for up to 8 rows, whose registers (128) allow it, also one beside a CTA of the prefix kernel.
-template <int D, int NT>
-__global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : CTAS) own_kernel(const __grid_constant__ CUtensorMap tmK,
+// 128 registers a thread, so that a CTA fits beside one of the prefix kernel.
+template <int D>
+__global__ void __launch_bounds__(WARPS * 32, 4) own_kernel(const __grid_constant__ CUtensorMap tmK,
                                                             const __grid_constant__ CUtensorMap tmV, const Args a) {
   using g = Geo<D>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -404,9 +395,13 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : CTAS) own_kernel(con
   // behind a prefix kernel, whose own inputs are complete when it lets this one start, only the end has to wait
   if (a.n_prefix == 0) griddep_wait();
   own_sequences(a, seqs, threadIdx.x, [] { __syncthreads(); });
+  const int tiles = (a.T * a.G + TILE_ROWS - 1) / TILE_ROWS;
+  const bool light = a.n_prefix != 0 && (long)seqs[a.B].before * a.hkv * tiles < (long)a.num_sms * LIGHT;
+  const int ctas = light ? a.num_sms : (int)gridDim.x;
   // few workers spread over the SMs
-  own_worker<D, NT>(tmK, tmV, a, seqs, base + warp * g::SLOTS * g::SLICE_BYTES, bars[warp], lane,
-                      warp * (int)gridDim.x + (int)blockIdx.x, WARPS * (int)gridDim.x);
+  if ((int)blockIdx.x < ctas)
+    own_worker<D>(tmK, tmV, a, seqs, base + warp * g::SLOTS * g::SLICE_BYTES, bars[warp], lane,
+                  warp * ctas + (int)blockIdx.x, WARPS * ctas);
   // this grid is complete only when the prefix grid is; one CTA sees to that, the others make room for the next
   if (a.n_prefix != 0 && blockIdx.x == gridDim.x - 1) griddep_wait();
 }
@@ -429,13 +424,13 @@ __global__ void __launch_bounds__(128) combine_kernel(const Args a) {
   if (row >= a.B * a.T * hq) return;
   const int before = own_before(a)[b], units = own_before(a)[b + 1] - before, quota = own_before(a)[a.B + 1];
   // the workers whose quotas this row's slices fall into
-  const int r = t * a.G + (head - h * a.G), tile = r / a.tile_rows, tiles = (rows + a.tile_rows - 1) / a.tile_rows;
-  const int u = h * tiles + tile, stride = min(rows, a.tile_rows);
+  const int r = t * a.G + (head - h * a.G), tile = r / TILE_ROWS, tiles = (rows + TILE_ROWS - 1) / TILE_ROWS;
+  const int u = h * tiles + tile, stride = min(rows, TILE_ROWS);
   const int at = before * a.hkv * tiles + u * units + PIECE_COST;  // its first slice
   const int w0 = at / quota;
   int n_own = units > 0 ? (at + units - PIECE_COST - 1) / quota - w0 + 1 : 0;
   if (n_prefix == 0 && n_own == 1) return;  // already written
-  const long own = a.own_at + (long)(w0 + b * a.hkv * tiles + u) * stride + (r - tile * a.tile_rows);  // pieces are `stride` apart
+  const long own = a.own_at + (long)(w0 + b * a.hkv * tiles + u) * stride + (r - tile * TILE_ROWS);  // pieces are `stride` apart
   if (base < 0 || base + n_prefix > a.own_at || (n_own > 0 && own + (long)(n_own - 1) * stride >= a.slot_cap)) {
     if (lane == 0) record_error(a.err, ERR_BAD_ARGUMENT);
     n_prefix = n_own = 0;
@@ -493,12 +488,10 @@ static cudaError_t launch(const Args& a, cudaStream_t st) {
   const CUtensorMap ok = D == 128 ? map3(a.k) : tk, ov = D == 128 ? map3(a.v) : tv;
   cudaError_t e = cudaSuccess;
   if (a.n_prefix > 0 && (e = launch_prefix<D>(a, tk, tv, st)) != cudaSuccess) return e;
-  const bool narrow = a.tile_rows == 8;
-  auto kern = narrow ? own_kernel<D, 1> : own_kernel<D, 2>;
-  static bool done[2][MAX_DEVICES] = {};
-  e = prepare_kernel(kern, (int)Geo<D>::smem(SHARED_MAX_BATCH), done[narrow]);
+  static bool done[MAX_DEVICES] = {};
+  e = prepare_kernel(own_kernel<D>, (int)Geo<D>::smem(SHARED_MAX_BATCH), done);
   if (e != cudaSuccess) return e;
-  e = launch_k(kern, dim3((unsigned)((getenv("CT")?atoi(getenv("CT")):3) * a.num_sms)), dim3(WARPS * 32), Geo<D>::smem(a.B), st, ok, ov, a);
+  e = launch_k(own_kernel<D>, dim3((unsigned)((a.n_prefix > 0 ? CTAS_SHARED : CTAS_ALONE) * a.num_sms)), dim3(WARPS * 32), Geo<D>::smem(a.B), st, ok, ov, a);
   if (e != cudaSuccess) return e;
   const long out_rows = (long)a.B * a.T * a.hkv * a.G;
   return launch_k(combine_kernel<D>, dim3((unsigned)((out_rows + 3) / 4)), dim3(128), 0, st, a);
@@ -511,7 +504,6 @@ cudaError_t launch_attn_shared(const SharedAttnArgs& x, int head_dim, double sca
   static_cast<SharedAttnArgs&>(a) = x;
   a.slices_per_page = x.page_size / shared_attn::SLICE;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
-  a.tile_rows = 8;
   return head_dim == 128 ? shared_attn::launch<128>(a, st) : shared_attn::launch<64>(a, st);
 }
 

@@ -14,7 +14,7 @@ constexpr int HDR = SHARED_HDR, ITEM = SHARED_ITEM;
 constexpr uint64_t WAIT_NS = 2000000000ull;
 
 struct Args : SharedAttnArgs {
-  int slices_per_page, tile_rows;  // tile_rows: query rows of a worker of the sequences' own keys
+  int slices_per_page;
   float scale_log2;
 };
 

@@ -193,11 +193,16 @@ void attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor
                   pml.device() == q.device() && po.numel() / D <= pml.numel() / 2,
               what, ": workspace");
   TORCH_CHECK(B <= SHARED_MAX_BATCH, std::string(what) + ": a batch of " + num(B) + ", at most " + num(SHARED_MAX_BATCH));
-  const int64_t own_slots = (12 * at::cuda::getDeviceProperties(q.get_device())->multiProcessorCount + B * hkv * ((T * G + 7) / 8)) *
-                            std::min<int64_t>(16, T * G);
+  const int64_t own_slots = (SHARED_OWN_WORKERS * at::cuda::getDeviceProperties(q.get_device())->multiProcessorCount +
+                             B * hkv * ((T * G + SHARED_OWN_ROWS - 1) / SHARED_OWN_ROWS)) *
+                            std::min<int64_t>(SHARED_OWN_ROWS, T * G);
   TORCH_CHECK(own_at >= 0 && (own_at + own_slots) * D <= po.numel(), what, ": workspace too small");
   TORCH_CHECK(kcache.size(0) * hkv * ps < (1ll << 31), what, ": KV pool too large for 32-bit TMA rows");
   TORCH_CHECK(block_tables.size(1) * ps < (1ll << 31), what, ": block tables too wide");
+  // the own keys of a call are counted in slices of 16, for every (sequence, KV head, tile of rows), in 32 bits
+  const int64_t tiles = (T * G + SHARED_OWN_ROWS - 1) / SHARED_OWN_ROWS;
+  TORCH_CHECK(B * hkv * tiles * (block_tables.size(1) * ps / 16 + 4) < (1ll << 30), what,
+              ": the block tables hold more keys than one call can attend");
   const c10::cuda::CUDAGuard guard(q.device());
   SharedAttnArgs a;
   a.q = static_cast<const __nv_bfloat16*>(q.data_ptr());

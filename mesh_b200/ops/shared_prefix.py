@@ -15,6 +15,8 @@ _HDR = 8      # header ints of the device table, [0] = number of prefix items
 _ITEM = 8     # ints per prefix item
 _ROWS = 64    # query rows of a sequence: new tokens x heads of a KV group
 _TILE = 256   # query rows per prefix item
+_OWN = 8      # query rows per worker on a sequence's own keys
+_WORKERS = 12  # such workers per SM
 _MAX_BATCH = 1024
 _KEYS = 64    # key ranges of prefix items are multiples of this
 
@@ -50,7 +52,7 @@ class PrefixGroups:
         # that the keys behind the prefixes are cut into
         self._own_at = _TILE * sms + rows * hq
         own_rows = q_len * self.group
-        slots = self._own_at + (12 * sms + batch * hkv * -(-own_rows // 8)) * min(16, own_rows)
+        slots = self._own_at + (_WORKERS * sms + batch * hkv * -(-own_rows // _OWN)) * min(_OWN, own_rows)
         self._po = torch.empty(slots * head_dim, dtype=torch.float32, device=self.device)
         self._pml = torch.empty(slots * 2, dtype=torch.float32, device=self.device)
         self._meta = torch.zeros(self._items_at + _ITEM * self.item_cap, dtype=torch.int32, device=self.device)

@@ -622,3 +622,27 @@ def test_verify_drafts_refusals():
     big = torch.zeros(1, 33, 4, device=DEV)
     with pytest.raises(RuntimeError):
         ops.verify_drafts(big, torch.zeros(1, 32, dtype=torch.int32, device=DEV), torch.zeros(1, 33, device=DEV))
+
+
+def test_attn_shared_prefix_counts_its_keys_in_32_bits():
+    """1024 sequences x 8 KV heads x 8 tiles of rows x 16384 slices of 16 keys: 2^30 pieces of work."""
+    plan = ops.PrefixGroups(1024, 64, 8, 64, q_len=8)
+    q = torch.zeros(8192, 4096, dtype=torch.bfloat16, device="cuda")
+    pool = torch.zeros(2, 8, 256, 64, dtype=torch.bfloat16, device="cuda")
+    lens = torch.full((1024,), 8, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="more keys than one call"):
+        ops.attn_shared_prefix(q, pool, pool, torch.zeros(1024, 1024, dtype=torch.int32, device="cuda"), lens, plan,
+                               torch.empty_like(q), 1.0)
+    out = torch.full_like(q, 7)
+    ops.attn_shared_prefix(q, pool, pool, torch.ones(1024, 1020, dtype=torch.int32, device="cuda"), lens, plan, out, 1.0)
+    assert bool((out == 0).all())  # every value is zero
+
+
+@pytest.mark.parametrize("own", [700, 40, 3])
+def test_attn_shared_prefix_own_keys_of_either_amount(own):
+    """Much to read behind the prefix (all workers take part) and little (those of one CTA per SM)."""
+    B, hq, hkv, D = 96, 32, 8, 128
+    groups = [(list(range(B)), 256)]
+    case = _shared_case(B, 1, hq, hkv, D, 16, groups, [own] * B, seed=31)
+    out, _ = _run_shared(case, 1, hq, hkv, D, groups)
+    _check_attn(out, *_attn_64(*case, 1, 1 / math.sqrt(D)))
