@@ -597,7 +597,7 @@ class Engine:
             if s.forked and s.pages:
                 first.setdefault(s.pages[0], []).append(s)
         r = self.runner
-        if not first or self.page_size % 16 or r.D not in (64, 128) or r.hq // r.hkv > 64:
+        if not first or self.page_size % 16 or r.D not in (64, 128) or r.hq // r.hkv > 64 or self.max_batch > 1024:
             return []
         out, saved = [], 0
         for group in first.values():

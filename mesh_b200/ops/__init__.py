@@ -357,6 +357,8 @@ def kv_pages_copy(k_pool: torch.Tensor, v_pool: torch.Tensor, src, dst, tokens=N
             raise ValueError(f"token counts outside a page of {k_pool.shape[3]}")
         if not src:
             return
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("lists of pages come from host memory: give device tensors inside a capture")
         n = len(src)
         idx = torch.tensor(src + dst + [int(t) for t in tokens or ()], dtype=torch.int32)
         idx = idx.pin_memory().to(k_pool.device, non_blocking=True)

@@ -64,7 +64,10 @@ class PrefixGroups:
     def set(self, groups: Sequence[Tuple[Sequence[int], int]]) -> "PrefixGroups":
         """``groups``: (sequences, shared keys) pairs. The first ``shared`` keys of every sequence of a group
         must be the same tokens; they are read through the block table of the group's first sequence. A
-        sequence may be in one group at most; one in none attends its own pages alone."""
+        sequence may be in one group at most; one in none attends its own pages alone. Not inside a capture: the
+        list comes from the host."""
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("PrefixGroups.set copies from host memory: call it before the capture, or between replays")
         B, T, G = self.batch, self.q_len, self.group
         seen = set()
         for seqs, shared in groups:
@@ -138,7 +141,8 @@ def attn_shared_prefix(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tens
         raise ValueError(f"cache {tuple(kcache.shape)} does not fit groups of {groups.hkv} KV heads of {groups.head_dim}")
     if groups.device != q.device:
         raise ValueError(f"groups on {groups.device}, q on {q.device}")
-    capturing = torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(q.device):
+        capturing = torch.cuda.is_current_stream_capturing()
     ext().attn_shared(q, kcache, vcache, block_tables, seq_lens, groups._meta, groups._po, groups._pml, out,
                       groups._err, groups.item_cap if capturing else groups.n_items, groups._own_at, scale, window)
     _count(2 + (capturing or groups.n_items > 0))

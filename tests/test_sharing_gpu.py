@@ -646,3 +646,53 @@ def test_attn_shared_prefix_own_keys_of_either_amount(own):
     case = _shared_case(B, 1, hq, hkv, D, 16, groups, [own] * B, seed=31)
     out, _ = _run_shared(case, 1, hq, hkv, D, groups)
     _check_attn(out, *_attn_64(*case, 1, 1 / math.sqrt(D)))
+
+
+def test_host_lists_are_refused_inside_a_capture():
+    """Their copy would read the same, by then reused, host memory at every replay."""
+    plan = ops.PrefixGroups(2, 8, 2, 64)
+    pool = torch.zeros(1, 4, 2, 16, 64, dtype=torch.bfloat16, device=DEV)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="host"):
+            plan.set([([0, 1], 16)])
+        with pytest.raises(RuntimeError, match="host"):
+            ops.kv_pages_copy(pool, pool.clone(), [1], [2])
+        pool.add_(1)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert bool((pool == 1).all()) and plan.n_items == 0
+
+
+def test_attention_and_verification_on_two_streams_at_once():
+    """Calls with groups of their own on two streams give what they give alone."""
+    hq, hkv, D = 32, 8, 128
+    groups = [(list(range(24)), 700)]
+    cases = [_shared_case(24, 1, hq, hkv, D, 16, groups, [30 + 9 * i for i in range(24)], seed=s) for s in (41, 42)]
+    plans = [ops.PrefixGroups(24, hq, hkv, D).set(groups) for _ in cases]
+    logits = [torch.randn(3, 5, 32000, device=DEV, generator=_gen(s)) for s in (43, 44)]
+    ids = torch.randint(0, 32000, (3, 4), dtype=torch.int32, device=DEV, generator=_gen(45))
+    u = torch.rand(3, 5, device=DEV, generator=_gen(46))
+
+    def run(i, out):
+        q, kc, vc, table, lens = cases[i]
+        ops.attn_shared_prefix(q, kc, vc, table, lens, plans[i], out, 1 / math.sqrt(D))
+        return ops.verify_drafts(logits[i], ids, u)
+
+    alone = []
+    for i in range(2):
+        out = torch.empty_like(cases[i][0])
+        alone.append((out, *run(i, out)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = [[torch.empty_like(cases[i][0]) for _ in range(8)] for i in range(2)]
+    got = [[], []]
+    for k in range(8):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append((outs[i][k], *run(i, outs[i][k])))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for one in got[i]:
+            assert all(torch.equal(x, y) for x, y in zip(one, alone[i]))
