@@ -18,7 +18,9 @@
 // Two launches:
 //   stats    grid (chunk, row): one CTA reads one chunk of a row once, keeps it in registers, and writes its
 //            maximum (first index) and its mass relative to that maximum. Rows past a session's drafts are
-//            not read. Bound by reading the logits and, as closely, by the 64-bit exponentials.
+//            not read. Bound by the 64-bit exponentials: 64 sessions of 5 rows over 128256 tokens (164 MB of fp32) take
+//            56 us; with greedy sessions, which need none, the whole call takes 28, 5.9 TB/s. More or fewer warps on an
+//            SM, and warps that load ahead of their exponentials, cost more.
 //   resolve  one cluster of 8 CTAs per session: joins the chunks of the session's rows and decides. Drawing from p (or
 //            p without one token) the chunks' masses are known and one CTA goes on: it picks the chunk, the
 //            256-token unit in it, and the token. For max(p - q, 0) every CTA first sums the units of its eighth of the
@@ -37,13 +39,14 @@ constexpr int SNT = 256;                // threads of a stats CTA
 constexpr int RNT = 256;                // threads of a resolve CTA
 constexpr int CLUSTER = 8;
 constexpr int MAX_DRAFTS = VERIFY_MAX_DRAFTS;
+constexpr int STEP = 4;                 // exponentials of a thread side by side (64 registers keep four CTAs on an SM)
 constexpr int PER_LANE = 8;            // tokens of a unit per lane
 constexpr int UNIT = 32 * PER_LANE;     // tokens whose sum one warp of the resolve kernel makes
 constexpr int MAX_SUMS = 4096;          // chunks of a row, units of a CTA's share
 // Logits per stats thread, by the CTAs that 32 each would make: 8 below two per SM (one session of 5 rows over 128256
 // tokens then makes 315 CTAs instead of 80), 16 below sixteen per SM (33 sessions of 1-8 rows over 32000 tokens: 19.8 us,
 // with 32 each 25.9), else 32, which spreads a CTA's fixed work over more logits (64 sessions of 5 rows over 128256:
-// 77 us, with 16 each 86).
+// 77 us, with 16 each 86; both pairs before the exponentials ran side by side).
 constexpr int EPT_MANY = 32, EPT_SOME = 16, EPT_FEW = 8;
 inline int logits_per_thread(int64_t rows, int64_t V) {
   const int64_t ctas = rows * ((V + SNT * EPT_MANY - 1) / (SNT * EPT_MANY));
@@ -65,18 +68,31 @@ __device__ __forceinline__ int drafts_of(const Args& a, int b) {
   return a.lens ? max(0, min(a.lens[b], a.K)) : a.K;
 }
 
+// 2^(j / 32)
+__device__ const double POW2[32] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.6457554781539649,
+    1.681792830507429, 1.7186192981224779, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
+};
+
 // e^((x - m) / T) in 64 bits for one row with a finite maximum m. Reduction by a table (Tang, 1989): with
 // z = (x - m) 32 / (T ln 2) = n + f, |f| <= 1/2, it is 2^(n / 32) e^(f ln2 / 32): lane j of the warp holds 2^(j / 32),
 // fetched by shuffle, and a polynomial of degree 4 does the rest (its next term, (ln2 / 64)^5 / 120 = 1.2e-12, bounds
-// the relative error). Ten 64-bit operations and about as many others; the loops below are bound by their issue,
+// the relative error). Eight 64-bit operations and half as many others; the loops below are bound by their issue,
 // and CUDA's exp() made them four times slower. All 32 lanes of a warp must call it together.
 // The exponential has to stay a normal number, so tokens below `low` = m - 700 T (masked ones, NaN) are taken
-// there, and what is not well above their mass, `none`, has none. T is taken as at most 1e30 and at least 1e-30.
+// there, and what is not well above their mass, `least()`, has none. T is taken as at most 1e30 and at least 1e-30.
 struct Exp {
-  double scale, top, table, none;
+  double scale, top;
   float low, m;
-  bool only;  // no logit other than m itself is within 700 T (m is infinite, or its neighbours are further): equal shares
-  __device__ __forceinline__ Exp(float m_, float inv_t) : m(m_) {
+  int hi, lo;  // of 2^(j / 32), less j in the exponent's place, so that n adds the whole exponent
+  bool only;   // no logit other than m itself is within 700 T (m is infinite, or its neighbours are further): equal shares
+  __device__ __forceinline__ Exp(float m_, float inv_t, double pow2) : m(m_) {
     constexpr double PER = 46.166241308446828384;  // 32 / ln 2
     inv_t = fmaxf(fminf(inv_t, 1e30f), 1e-30f);
     low = __fsub_ru(m_, 700.f / inv_t);
@@ -87,29 +103,55 @@ struct Exp {
     }
     scale = (double)inv_t * PER;
     top = only ? 0.0 : (double)m_;
-    table = exp2((double)(threadIdx.x & 31) * 0.03125);
-    double w, p;
-    split(low, w, p);
-    none = w * p * 1e12;  // above the sum of any chunk of masked tokens
+    hi = __double2hiint(pow2) - (int)(threadIdx.x & 31) * 32768;
+    lo = __double2loint(pow2);
   }
+  // this lane's entry of the table, to be asked for early
+  static __device__ __forceinline__ double entry() { return POW2[threadIdx.x & 31]; }
   // what split takes for logit x
   __device__ __forceinline__ float arg(float x) const { return only ? (x == m ? 0.f : -INFINITY) : x; }
-  __device__ __forceinline__ void split(float x, double& w, double& poly) const {  // the mass is w * poly
+  // N logits in step, so that their chains of dependent operations overlap; the masses are w[i] * poly[i]
+  template <int N>
+  __device__ __forceinline__ void split(const float (&x)[N], double (&w)[N], double (&poly)[N]) const {
     constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the nearest integer
     constexpr double L = 0.021660849392498290;     // ln 2 / 32
-    constexpr double C2 = L * L / 2, C3 = C2 * L / 3, C4 = C3 * L / 4;
-    const double z = ((double)fmaxf(x, low) - top) * scale;
-    const double k = z + MAGIC;
-    const int n = __double2loint(k);
-    const double f = z - (k - MAGIC);
-    const double t = __shfl_sync(0xffffffffu, table, n);  // the low five bits choose the lane
-    w = __hiloint2double(__double2hiint(t) + (n & ~31) * 32768, __double2loint(t));
-    poly = fma(fma(fma(fma(C4, f, C3), f, C2), f, L), f, 1.0);
+    constexpr double C2 = L * L / 2, C3 = 0x1.c6b09p-20, C4 = 0x1.3b2abp-27;  // L^3 / 6 and L^4 / 24 to 20 bits, which
+    double f[N];                                   // an instruction holds itself: within 2e-14 and 2e-16 of the result
+    int n[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = (double)fmaxf(x[i], low) - top;
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = fma(f[i], scale, MAGIC);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      n[i] = __double2loint(w[i]);
+      w[i] = MAGIC - w[i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = fma(f[i], scale, w[i]);
+#pragma unroll
+    for (int i = 0; i < N; ++i)  // the low five bits of n choose the lane
+      w[i] = __hiloint2double(__shfl_sync(0xffffffffu, hi, n[i]) + n[i] * 32768, __shfl_sync(0xffffffffu, lo, n[i]));
+#pragma unroll
+    for (int i = 0; i < N; ++i) poly[i] = fma(C4, f[i], C3);
+#pragma unroll
+    for (int i = 0; i < N; ++i) poly[i] = fma(poly[i], f[i], C2);
+#pragma unroll
+    for (int i = 0; i < N; ++i) poly[i] = fma(poly[i], f[i], L);
+#pragma unroll
+    for (int i = 0; i < N; ++i) poly[i] = fma(poly[i], f[i], 1.0);
   }
   __device__ __forceinline__ double operator()(float x) const {
-    double w, p;
-    split(arg(x), w, p);
-    return w * p;
+    const float v[1] = {arg(x)};
+    double w[1], p[1];
+    split(v, w, p);
+    return w[0] * p[0];
+  }
+  __device__ __forceinline__ double least() const {
+    const float v[1] = {low};
+    double w[1], p[1];
+    split(v, w, p);
+    return w[0] * p[0] * 1e12;  // above the sum of any chunk of masked tokens
   }
 };
 
@@ -162,14 +204,16 @@ __device__ __forceinline__ void load_run(const T* x, int i, int V, float fill, f
   }
 }
 
-// Logits of a chunk in a stats thread: runs of RUN elements, SNT * RUN apart.
+// Logits of a chunk in a stats thread: runs of RUN elements, SNT * RUN apart. A warp takes its mass relative to its own
+// maximum, so that the warps of an SM run apart, some loading while others compute; the chunk's is joined from theirs.
 template <typename T, int EPT, bool VEC>
-__global__ void __launch_bounds__(SNT) stats_kernel(const Args a) {
+__global__ void __launch_bounds__(SNT, 4) stats_kernel(const Args a) {
   constexpr int RUN = VEC ? 16 / (int)sizeof(T) : 1;
-  constexpr int CHUNK = SNT * EPT;
-  __shared__ float red_m[SNT / 32];
+  constexpr int CHUNK = SNT * EPT, WARPS = SNT / 32;
+  __shared__ float red_m[WARPS];
   __shared__ int first;
-  __shared__ double red_s[SNT / 32];
+  __shared__ double red_s[WARPS];
+  const double pow2 = Exp::entry();
   griddep_wait();
   griddep_launch_dependents();
   const int row = blockIdx.y, b = row / (a.K + 1), k = row - b * (a.K + 1);
@@ -181,19 +225,48 @@ __global__ void __launch_bounds__(SNT) stats_kernel(const Args a) {
   float v[EPT / RUN][RUN];
 #pragma unroll
   for (int e = 0; e < EPT / RUN; ++e) load_run<T, RUN, VEC>(x, i0 + e * SNT * RUN, a.V, -INFINITY, v[e]);
-  float m = -INFINITY;
+  float own = -INFINITY;
 #pragma unroll
   for (int e = 0; e < EPT / RUN; ++e)
 #pragma unroll
-    for (int j = 0; j < RUN; ++j) m = fmaxf(m, v[e][j]);
+    for (int j = 0; j < RUN; ++j) own = fmaxf(own, v[e][j]);
+  float wm = own;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int o = 16; o > 0; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
+  double s = 0.0, s1 = 0.0;
+  if (t > 0.f && wm > -INFINITY) {
+    const Exp mass(wm, t, pow2);
+    if (mass.only) {
+#pragma unroll
+      for (int e = 0; e < EPT / RUN; ++e)
+#pragma unroll
+        for (int j = 0; j < RUN; ++j) s += v[e][j] == wm ? 1.0 : 0.0;
+    } else {
+#pragma unroll
+      for (int k = 0; k < EPT; k += STEP) {
+        float x[STEP];
+        double w[STEP], p[STEP];
+#pragma unroll
+        for (int i = 0; i < STEP; ++i) x[i] = v[(k + i) / RUN][(k + i) % RUN];
+        mass.split(x, w, p);
+#pragma unroll
+        for (int i = 0; i < STEP; i += 2) {
+          s = fma(w[i], p[i], s);
+          s1 = fma(w[i + 1], p[i + 1], s1);
+        }
+      }
+    }
+    s = warp_sum(s + s1);
+  }
   if (tid == 0) first = INT_MAX;
-  if (lane == 0) red_m[warp] = m;
+  if (lane == 0) {
+    red_m[warp] = wm;
+    red_s[warp] = s;
+  }
   __syncthreads();
-  const float own = m;
+  float m = red_m[0];
 #pragma unroll
-  for (int w = 0; w < SNT / 32; ++w) m = fmaxf(m, red_m[w]);
+  for (int w = 1; w < WARPS; ++w) m = fmaxf(m, red_m[w]);
   if (own == m && m > -INFINITY) {  // few warps hold the maximum: only they look for its index
     int at = INT_MAX;
 #pragma unroll
@@ -203,31 +276,13 @@ __global__ void __launch_bounds__(SNT) stats_kernel(const Args a) {
         if (v[e][j] == m) at = i0 + e * SNT * RUN + j;
     if (at != INT_MAX) atomicMin(&first, at);
   }
-  double s = 0.0;
-  if (t > 0.f && m > -INFINITY) {
-    const Exp mass(m, t);
-    if (mass.only)
-#pragma unroll
-      for (int e = 0; e < EPT / RUN; ++e)
-#pragma unroll
-        for (int j = 0; j < RUN; ++j) v[e][j] = mass.arg(v[e][j]);
-#pragma unroll
-    for (int e = 0; e < EPT / RUN; ++e)
-#pragma unroll
-      for (int j = 0; j < RUN; ++j) {
-        double w, p;
-        mass.split(v[e][j], w, p);
-        s = fma(w, p, s);
-      }
-    s = warp_sum(s);
-    if (lane == 0) red_s[warp] = s;
+  s = 0.0;
+  if (warp == 0 && t > 0.f && m > -INFINITY) {
+    const Exp mass(m, t, pow2);
+    const double f = mass(lane < WARPS ? red_m[lane] : -INFINITY);
+    s = warp_sum(lane < WARPS ? red_s[lane] * f : 0.0);
   }
   __syncthreads();
-  if (t > 0.f && m > -INFINITY) {
-    s = 0.0;
-#pragma unroll
-    for (int w = 0; w < SNT / 32; ++w) s += red_s[w];
-  }
   if (tid == 0) {
     Part p;
     p.m = m;
@@ -255,6 +310,7 @@ __global__ void __launch_bounds__(RNT, 4) resolve_kernel(const Args a, int chunk
   const int b = blockIdx.x / CLUSTER, rank = blockIdx.x % CLUSTER;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int K = a.K, V = a.V;
+  const double pow2 = Exp::entry();
   const T* xs = static_cast<const T*>(a.logits) + (long)b * a.ld_seq;
   const Q* qs = static_cast<const Q*>(a.probs) + (a.probs ? (long)b * a.lq_seq : 0);
   // The stats kernel lets this one start once everything before it is complete, so all inputs but its
@@ -295,7 +351,7 @@ __global__ void __launch_bounds__(RNT, 4) resolve_kernel(const Args a, int chunk
       take(m, idx, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, idx, o));
     double z = 0.0, px = 0.0;
     if (!greedy && m > -INFINITY) {
-      const Exp mass(m, t);
+      const Exp mass(m, t, pow2);
 #pragma unroll 1
       for (int c = lane; c - lane < a.chunks; c += 32) {
         const double f = mass(c < a.chunks ? p[c].m : -INFINITY);
@@ -303,7 +359,7 @@ __global__ void __launch_bounds__(RNT, 4) resolve_kernel(const Args a, int chunk
       }
       z = warp_sum(z);
       const double w = mass(at_x);
-      px = w > mass.none ? w / z : 0.0;
+      px = w > mass.least() ? w / z : 0.0;
     } else if (greedy) {
       px = m > -INFINITY && k < n && idx == id ? 1.0 : 0.0;
     }
@@ -335,7 +391,8 @@ __global__ void __launch_bounds__(RNT, 4) resolve_kernel(const Args a, int chunk
   const T* x = xs + (long)acc * a.ld_row;
   const Q* q = qs + (a.probs && acc < n ? (long)acc * a.lq_row : 0);
   const Part* parts = static_cast<const Part*>(a.parts) + ((long)b * (K + 1) + acc) * a.chunks;
-  const Exp mass(m, t);
+  const Exp mass(m, t, pow2);
+  const double none = mass.least();
   const double inv_z = 1.0 / row_z[acc];
   // what is drawn from: 0 p, 1 max(p - q, 0), 2 p without the token `skip`
   const int skip = acc < n ? row_x[acc] : -1;
@@ -354,15 +411,25 @@ __global__ void __launch_bounds__(RNT, 4) resolve_kernel(const Args a, int chunk
       if (mode == 1) load_run<Q, RUN, VEC>(q, i, end, 0.f, r.f[e]);
     }
   };
-  auto weight = [&](const Raw& r, int i0, int e, int j) -> double {
-    double p = mass(r.v[e][j]);
-    if (mode == 1) {
-      p = fma(p, inv_z, -(double)fmaxf(r.f[e][j], 0.f));  // a NaN or negative q counts as none
-    } else {
-      p *= inv_z;
-      if (mode == 2 && i0 + (e * 32 + lane) * RUN + j == skip) p = 0.0;
+  // the shares of STEP tokens of a lane, from its k-th of the unit on
+  auto weights = [&](const Raw& r, int i0, int k, double (&p)[STEP]) {
+    float x[STEP];
+    double w[STEP];
+#pragma unroll
+    for (int i = 0; i < STEP; ++i) x[i] = mass.arg(r.v[(k + i) / RUN][(k + i) % RUN]);
+    mass.split(x, w, p);
+#pragma unroll
+    for (int i = 0; i < STEP; ++i) {
+      const int e = (k + i) / RUN, j = (k + i) % RUN;
+      p[i] *= w[i];
+      if (mode == 1) {
+        p[i] = fma(p[i], inv_z, -(double)fmaxf(r.f[e][j], 0.f));  // a NaN or negative q counts as none
+      } else {
+        p[i] *= inv_z;
+        if (mode == 2 && i0 + (e * 32 + lane) * RUN + j == skip) p[i] = 0.0;
+      }
+      p[i] = p[i] > none ? p[i] : 0.0;
     }
-    return p > mass.none ? p : 0.0;
   };
   // sums[] of the units of [i0, end): a warp each, the next unit's loads in flight under this one's exponentials
   auto unit_sums = [&](int i0, int end) {
@@ -374,9 +441,12 @@ __global__ void __launch_bounds__(RNT, 4) resolve_kernel(const Args a, int chunk
       if (i + WARPS * UNIT < end) fetch_unit(i + WARPS * UNIT, end, next);
       double s = 0.0;
 #pragma unroll
-      for (int e = 0; e < PER_LANE / RUN; ++e)
+      for (int k = 0; k < PER_LANE; k += STEP) {
+        double p[STEP];
+        weights(r, i, k, p);
 #pragma unroll
-        for (int j = 0; j < RUN; ++j) s += weight(r, i, e, j);
+        for (int i = 0; i < STEP; ++i) s += p[i];
+      }
       s = warp_sum(s);
       if (lane == 0) sums[(i - i0) / UNIT] = s;
       r = next;
@@ -451,7 +521,7 @@ __global__ void __launch_bounds__(RNT, 4) resolve_kernel(const Args a, int chunk
       const double f = mass(e < a.chunks ? parts[e].m : -INFINITY);
       if (e < a.chunks) {
         const double s = mode == 2 && e == skip / chunk ? without : parts[e].s * f * inv_z;
-        sums[e] = s > mass.none ? s : 0.0;
+        sums[e] = s > none ? s : 0.0;
       }
     }
     __syncthreads();
@@ -475,12 +545,20 @@ __global__ void __launch_bounds__(RNT, 4) resolve_kernel(const Args a, int chunk
   Raw r;
   fetch_unit(i0, end, r);
   int last = -1;
+  double all[PER_LANE];
+#pragma unroll
+  for (int k = 0; k < PER_LANE; k += STEP) {
+    double p[STEP];
+    weights(r, i0, k, p);
+#pragma unroll
+    for (int i = 0; i < STEP; ++i) all[k + i] = p[i];
+  }
 #pragma unroll
   for (int e = 0; e < PER_LANE / RUN; ++e) {  // the runs of step e lie before those of step e + 1
     double w[RUN], mine = 0.0;
 #pragma unroll
     for (int j = 0; j < RUN; ++j) {
-      w[j] = weight(r, i0, e, j);
+      w[j] = all[e * RUN + j];
       mine += w[j];
     }
     const double incl = warp_scan(mine, lane);
