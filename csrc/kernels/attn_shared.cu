@@ -11,6 +11,11 @@
 // combine kernel merges a row's partials: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i. All partials of a row
 // are summed in a fixed order, so results do not depend on the schedule.
 //
+// Measured (32 query and 8 KV heads of 128): 64 sessions with up to 512 keys of their own behind 8192 shared ones 35.8 us, of
+// which reading every key once takes 15.8 at the copy rate; 128 with up to 1024 behind 16384 92 us (52.5); 4 forks of 512
+// keys 10.5 us. About 19 us of the large calls go by before and after the keys: first queries and pages (5), partials
+// written (3: 256 rows x 128 fp32 from every SM) and merged (6), and three kernels following one another.
+//
 // The item list is made on the host when the groups change (PrefixGroups) and lives in device memory, so a
 // captured step follows later changes of groups, lengths and tables.
 #include <type_traits>
@@ -124,7 +129,8 @@ __device__ __forceinline__ void own_sequences(const Args& a, Seq* seqs, int tid,
 // what loading its queries and writing its result take. Piece number = worker + (sequence, head, tile), which no other
 // piece has. A warp works by itself: it requests slices SLOTS ahead (TMA, 128-byte swizzle), without a barrier between
 // warps; four warps that split each piece and merged it took twice as long (64 sessions of up to 512 keys). Bound by
-// reading K and V.
+// reading K and V: 128 sessions of up to 1024 keys, 269 MB, take 51.7 us (5.2 TB/s, 0.81 of a copy). Leaving out the rescale and
+// the masks where a slice needs neither changed nothing.
 // The products run transposed, S^T = K Q^T and O^T = V^T P^T on m16n8k16 fragments, so that the few query rows are the
 // narrow side. With the rows on the 16-wide side half of every product and of the accumulators would be padding (168
 // registers, so no CTA fitted beside the prefix kernel's). More than 8 rows are cut into tiles, each reading the keys
@@ -407,7 +413,7 @@ __global__ void __launch_bounds__(WARPS * 32, 4) own_kernel(const __grid_constan
 }
 
 // One warp per row (sequence, token, head): merge its partials, the prefix's first, in order. Bound by latency, not by the
-// bytes: lane i asks for the (m, l) of partial i and the warp for all of its first 16 outputs at once, weights follow.
+// bytes (5 to 6 us for 16.8 MB of partials, all in L2): lane i asks for the (m, l) of partial i and the warp for all of its first 16 outputs at once, weights follow.
 template <int D>
 __global__ void __launch_bounds__(128) combine_kernel(const Args a) {
   constexpr int V = D / 32, U = 16;
