@@ -14,6 +14,8 @@
 namespace mesh {
 namespace {
 
+std::string num(int64_t n) { return std::to_string(n); }
+
 void check_pools(const char* what, const at::Tensor& k_pool, const at::Tensor& v_pool) {
   TORCH_CHECK(k_pool.is_cuda() && v_pool.device() == k_pool.device() && k_pool.dim() == 5 &&
                   k_pool.sizes() == v_pool.sizes() && k_pool.is_contiguous() && v_pool.is_contiguous(),
@@ -26,7 +28,6 @@ void check_pools(const char* what, const at::Tensor& k_pool, const at::Tensor& v
   TORCH_CHECK(k_pool.size(0) < 65536 && k_pool.size(1) < INT_MAX, what, ": too many layers or pages");
 }
 
-std::string num(int64_t n) { return std::to_string(n); }
 std::string dims(at::IntArrayRef shape) {
   std::string s = "[";
   for (size_t i = 0; i < shape.size(); ++i) s += (i ? ", " : "") + num(shape[i]);
@@ -169,6 +170,7 @@ void attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor
   TORCH_CHECK(q.is_cuda() && q.scalar_type() == at::kBFloat16 && q.is_contiguous() && q.dim() == 2, what,
               ": q contiguous bf16 [B * T, hq * D] on a GPU");
   check_tensor(what, "out", out, q, at::kBFloat16, q.sizes());
+  TORCH_CHECK((uintptr_t)q.data_ptr() % 16 == 0 && (uintptr_t)out.data_ptr() % 16 == 0, what, ": q and out must be 16-byte aligned");
   TORCH_CHECK(kcache.dim() == 4, what, ": cache [pages, hkv, page, D]");
   check_tensor(what, "kcache", kcache, q, at::kBFloat16, kcache.sizes());
   check_tensor(what, "vcache", vcache, q, at::kBFloat16, kcache.sizes());

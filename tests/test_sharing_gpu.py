@@ -696,3 +696,21 @@ def test_attention_and_verification_on_two_streams_at_once():
     for i in range(2):
         for one in got[i]:
             assert all(torch.equal(x, y) for x, y in zip(one, alone[i]))
+
+
+def test_unaligned_views_and_empty_pools_are_refused():
+    """The kernels read 16 bytes at a time."""
+    q, kc, vc, table, lens = _shared_case(2, 1, 8, 2, 64, 16, [], [5, 6], seed=51)
+    plan = ops.PrefixGroups(2, 8, 2, 64)
+    off = torch.zeros(q.numel() + 1, dtype=torch.bfloat16, device=DEV)[1:].view_as(q)
+    with pytest.raises(RuntimeError, match="aligned"):
+        ops.attn_shared_prefix(off, kc, vc, table, lens, plan, torch.empty_like(q), 1.0)
+    with pytest.raises(RuntimeError, match="aligned"):
+        ops.attn_shared_prefix(q, kc, vc, table, lens, plan, off, 1.0)
+    off_kv = torch.zeros(kc.numel() + 1, dtype=torch.bfloat16, device=DEV)[1:].view_as(kc)
+    with pytest.raises(RuntimeError, match="aligned"):
+        ops.attn_shared_prefix(q, off_kv, vc, table, lens, plan, torch.empty_like(q), 1.0)
+    none = torch.zeros(0, 4, 2, 16, 64, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(RuntimeError, match="empty pools"):
+        ops.kv_pages_copy(none, none.clone(), [1], [2])
+    torch.cuda.synchronize()
