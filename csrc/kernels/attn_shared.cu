@@ -11,10 +11,10 @@
 // combine kernel merges a row's partials: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i. All partials of a row
 // are summed in a fixed order, so results do not depend on the schedule.
 //
-// Measured (32 query and 8 KV heads of 128): 64 sessions with up to 512 keys of their own behind 8192 shared ones 35.8 us, of
+// Measured (32 query and 8 KV heads of 128): 64 sessions with up to 512 keys of their own behind 8192 shared ones 36.9 us, of
 // which reading every key once takes 15.8 at the copy rate; 128 with up to 1024 behind 16384 92 us (52.5); 4 forks of 512
 // keys 10.5 us. About 19 us of the large calls go by before and after the keys: first queries and pages (5), partials
-// written (3: 256 rows x 128 fp32 from every SM) and merged (6), and three kernels following one another.
+// written (3: 256 rows x 128 fp32 from every SM) and merged (5), and three kernels following one another.
 //
 // The item list is made on the host when the groups change (PrefixGroups) and lives in device memory, so a
 // captured step follows later changes of groups, lengths and tables.
@@ -413,10 +413,12 @@ __global__ void __launch_bounds__(WARPS * 32, 4) own_kernel(const __grid_constan
 }
 
 // One warp per row (sequence, token, head): merge its partials, the prefix's first, in order. Bound by latency, not by the
-// bytes (5 to 6 us for 16.8 MB of partials, all in L2): lane i asks for the (m, l) of partial i and the warp for all of its first 16 outputs at once, weights follow.
+// bytes (5 us for 16.8 MB of partials, all in L2): lane i asks for the (m, l) of partial i and the warp for its first eight
+// outputs at once, those of the prefix before it is known which workers had the rest; weights follow. With sixteen at once
+// (128 registers instead of 80, fewer warps on an SM) up to 64 sessions gain 0.4 us and 256 lose 2.5.
 template <int D>
 __global__ void __launch_bounds__(128) combine_kernel(const Args a) {
-  constexpr int V = D / 32, U = 16;
+  constexpr int V = D / 32, U = 8, U_OWN = 2;
   using Vec = typename std::conditional<V == 4, float4, float2>::type;
   const int lane = threadIdx.x & 31, hq = a.hkv * a.G, rows = a.T * a.G;
   const int row = blockIdx.x * 4 + (threadIdx.x >> 5);  // (b * T + t) * hq + head
@@ -425,54 +427,73 @@ __global__ void __launch_bounds__(128) combine_kernel(const Args a) {
   // written by the host alone, not by a kernel that this grid may overlap
   int n_prefix = seq_prefix_slots(a, b);
   const int base = seq_base(a, b) + x * n_prefix;
+  const bool bad = base < 0 || base + n_prefix > a.own_at;
+  if (bad) n_prefix = 0;
   griddep_wait();
   griddep_launch_dependents();
   if (row >= a.B * a.T * hq) return;
-  const int before = own_before(a)[b], units = own_before(a)[b + 1] - before, quota = own_before(a)[a.B + 1];
+  const int before = own_before(a)[b], after = own_before(a)[b + 1], quota = own_before(a)[a.B + 1];
+  float acc[V] = {}, den = 0.f, M = -INFINITY;
+  auto stats = [&](long first, long step, int n, int i) {
+    return i + lane < n ? a.pml[first + (i + lane) * step] : make_float2(-INFINITY, 0.f);
+  };
+  auto load = [&](long first, long step, int n, int i, auto& p) {
+#pragma unroll
+    for (int k = 0; k < (int)(sizeof(p) / sizeof(p[0])); ++k)
+      if (i + k < n) *reinterpret_cast<Vec*>(p[k]) = *reinterpret_cast<const Vec*>(a.po + (first + (i + k) * step) * D + lane * V);
+  };
+  // n partials, `step` apart; ml and p: the first of them, already on their way
+  auto merge = [&](long first, long step, int n, float2 ml, auto& p) {
+    constexpr int N = (int)(sizeof(p) / sizeof(p[0]));
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      if (i0 > 0) ml = stats(first, step, n, i0);
+      float mx = ml.x;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float mn = fmaxf(M, mx);
+      if (mn == -INFINITY) continue;
+      const float corr = ex2_ftz(M - mn), f = ex2_ftz(ml.x - mn);  // 0 for a partial that saw nothing
+      M = mn;
+      den = den * corr + (ml.x > -INFINITY ? ml.y * f : 0.f);
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] *= corr;
+      for (int i = i0; i < min(n, i0 + 32); i += N) {
+        if (i > 0) load(first, step, n, i, p);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const float w = __shfl_sync(0xffffffffu, f, (i + k) & 31);
+          if (i + k < n && w > 0.f)  // the output of a partial that saw nothing may not have been written
+#pragma unroll
+            for (int v = 0; v < V; ++v) acc[v] = fmaf(p[k][v], w, acc[v]);
+        }
+      }
+    }
+  };
+  float p[U][V];
+  float2 ml = stats(base, 1, n_prefix, 0);
+  load(base, 1, n_prefix, 0, p);
   // the workers whose quotas this row's slices fall into
-  const int r = t * a.G + (head - h * a.G), tile = r / TILE_ROWS, tiles = (rows + TILE_ROWS - 1) / TILE_ROWS;
-  const int u = h * tiles + tile, stride = min(rows, TILE_ROWS);
+  const int units = after - before, r = t * a.G + (head - h * a.G);
+  const int tile = r / TILE_ROWS, tiles = (rows + TILE_ROWS - 1) / TILE_ROWS, u = h * tiles + tile, stride = min(rows, TILE_ROWS);
   const int at = before * a.hkv * tiles + u * units + PIECE_COST;  // its first slice
   const int w0 = at / quota;
   int n_own = units > 0 ? (at + units - PIECE_COST - 1) / quota - w0 + 1 : 0;
-  if (n_prefix == 0 && n_own == 1) return;  // already written
+  if (n_prefix == 0 && n_own == 1 && !bad) return;  // already written
   const long own = a.own_at + (long)(w0 + b * a.hkv * tiles + u) * stride + (r - tile * TILE_ROWS);  // pieces are `stride` apart
-  if (base < 0 || base + n_prefix > a.own_at || (n_own > 0 && own + (long)(n_own - 1) * stride >= a.slot_cap)) {
+  if (bad || (n_own > 0 && own + (long)(n_own - 1) * stride >= a.slot_cap)) {
     if (lane == 0) record_error(a.err, ERR_BAD_ARGUMENT);
-    n_prefix = n_own = 0;
+    n_own = 0;
   }
-  const int n = n_prefix + n_own;
-  auto slot = [&](int i) { return i < n_prefix ? base + (long)i : own + (long)(i - n_prefix) * stride; };
-  float acc[V] = {}, den = 0.f, M = -INFINITY;
-  for (int i0 = 0; i0 < n; i0 += 32) {
-    const float2 ml = i0 + lane < n ? a.pml[slot(i0 + lane)] : make_float2(-INFINITY, 0.f);
-    float p[U][V];
-    auto load = [&](int i) {
-#pragma unroll
-      for (int k = 0; k < U; ++k)
-        if (i + k < n) *reinterpret_cast<Vec*>(p[k]) = *reinterpret_cast<const Vec*>(a.po + slot(i + k) * D + lane * V);
-    };
-    load(i0);
-    float mx = ml.x;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const float mn = fmaxf(M, mx);
-    if (mn == -INFINITY) continue;
-    const float corr = ex2_ftz(M - mn), f = ex2_ftz(ml.x - mn);  // 0 for a partial that saw nothing
-    M = mn;
-    den = den * corr + (ml.x > -INFINITY ? ml.y * f : 0.f);
-#pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] *= corr;
-    for (int i = i0; i < min(n, i0 + 32); i += U) {
-      if (i > i0) load(i);
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const float w = __shfl_sync(0xffffffffu, f, (i + k) & 31);
-        if (i + k < n && w > 0.f)  // the output of a partial that saw nothing may not have been written
-#pragma unroll
-          for (int v = 0; v < V; ++v) acc[v] = fmaf(p[k][v], w, acc[v]);
-      }
-    }
+  if (n_prefix > 0) {
+    float p_own[U_OWN][V];
+    const float2 ml_own = stats(own, stride, n_own, 0);
+    load(own, stride, n_own, 0, p_own);
+    merge(base, 1, n_prefix, ml, p);
+    merge(own, stride, n_own, ml_own, p_own);
+  } else {
+    ml = stats(own, stride, n_own, 0);
+    load(own, stride, n_own, 0, p);
+    merge(own, stride, n_own, ml, p);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
