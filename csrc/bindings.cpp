@@ -65,9 +65,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> verify_drafts(const at::Tensor& l
                                                              const c10::optional<at::Tensor>& inv_t,
                                                              const c10::optional<at::Tensor>& probs,
                                                              const c10::optional<at::Tensor>& lens);
-void attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor& vcache, const at::Tensor& block_tables,
-                 const at::Tensor& seq_lens, at::Tensor& meta, at::Tensor& po, at::Tensor& pml, at::Tensor& out,
-                 at::Tensor& err, int64_t n_prefix, int64_t own_at, double scale, int64_t window);
+int64_t attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor& vcache, const at::Tensor& block_tables,
+                    const at::Tensor& seq_lens, at::Tensor& meta, at::Tensor& po, at::Tensor& pml, at::Tensor& out,
+                    at::Tensor& err, int64_t n_items, int64_t item_cap, int64_t own_at, double scale, int64_t window);
 void ar_fused_norm(const at::Tensor& bases, int64_t off_flags, int64_t off_p0, int64_t off_p1, int64_t off_resid,
                    int64_t off_normed, int64_t rank, int64_t world, int64_t T, int64_t H, int64_t parity,
                    const at::Tensor& gamma, double eps, at::Tensor& epoch, at::Tensor& err, int64_t nblocks,

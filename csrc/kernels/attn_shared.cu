@@ -13,7 +13,7 @@
 //
 // Measured (32 query and 8 KV heads of 128): 64 sessions with up to 512 keys of their own behind 8192 shared ones 36.9 us, of
 // which reading every key once takes 15.8 at the copy rate; 128 with up to 1024 behind 16384 92 us (52.5); 4 forks of 512
-// keys 10.5 us. About 19 us of the large calls go by before and after the keys: first queries and pages (5), partials
+// keys 10.7 us in a captured graph. About 19 us of the large calls go by before and after the keys: first queries and pages (5), partials
 // written (3: 256 rows x 128 fp32 from every SM) and merged (5), and three kernels following one another.
 //
 // The item list is made on the host when the groups change (PrefixGroups) and lives in device memory, so a
@@ -508,11 +508,18 @@ __global__ void __launch_bounds__(128) combine_kernel(const Args a) {
 template <int D>
 static cudaError_t launch(const Args& a, cudaStream_t st) {
   const uint64_t rows = (uint64_t)a.pool_pages * a.hkv * a.page_size;
-  const CUtensorMap tk = tma_map_2d_bf16(a.k, D, rows, D, 64, SLICE);
-  const CUtensorMap tv = tma_map_2d_bf16(a.v, D, rows, D, 64, SLICE);
-  // a slice of 128 columns in one box: two halves of 64 columns, 16 rows each
-  auto map3 = [&](const void* p) { return tma_map_3d_bf16(p, 64, rows, 2, D * 2, 128, 64, SLICE, 2); };
-  const CUtensorMap ok = D == 128 ? map3(a.k) : tk, ov = D == 128 ? map3(a.v) : tv;
+  CUtensorMap tk, tv, ok, ov;
+  if (a.n_prefix > 0 || D == 64) {
+    tk = tma_map_2d_bf16(a.k, D, rows, D, 64, SLICE);
+    tv = tma_map_2d_bf16(a.v, D, rows, D, 64, SLICE);
+  }
+  if (D == 128) {  // a slice of 128 columns in one box: two halves of 64 columns, 16 rows each
+    ok = tma_map_3d_bf16(a.k, 64, rows, 2, D * 2, 128, 64, SLICE, 2);
+    ov = tma_map_3d_bf16(a.v, 64, rows, 2, D * 2, 128, 64, SLICE, 2);
+  } else {
+    ok = tk;
+    ov = tv;
+  }
   cudaError_t e = cudaSuccess;
   if (a.n_prefix > 0 && (e = launch_prefix<D>(a, tk, tv, st)) != cudaSuccess) return e;
   static bool done[MAX_DEVICES] = {};

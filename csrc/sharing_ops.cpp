@@ -2,6 +2,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
@@ -163,9 +164,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> verify_drafts(const at::Tensor& l
   return {tokens, accepted, draft_p};
 }
 
-void attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor& vcache, const at::Tensor& block_tables,
-                 const at::Tensor& seq_lens, at::Tensor& meta, at::Tensor& po, at::Tensor& pml, at::Tensor& out,
-                 at::Tensor& err, int64_t n_prefix, int64_t own_at, double scale, int64_t window) {
+// n_items prefix items now; a captured call is launched for item_cap, the most there can be. Returns the kernels launched.
+int64_t attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor& vcache, const at::Tensor& block_tables,
+                    const at::Tensor& seq_lens, at::Tensor& meta, at::Tensor& po, at::Tensor& pml, at::Tensor& out,
+                    at::Tensor& err, int64_t n_items, int64_t item_cap, int64_t own_at, double scale, int64_t window) {
   const char* what = "attn_shared_prefix";
   TORCH_CHECK(q.is_cuda() && q.scalar_type() == at::kBFloat16 && q.is_contiguous() && q.dim() == 2, what,
               ": q contiguous bf16 [B * T, hq * D] on a GPU");
@@ -181,7 +183,7 @@ void attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor
   const int64_t B = seq_lens.size(0);
   check_tensor(what, "seq_lens", seq_lens, q, at::kInt, {B});
   check_tensor(what, "block_tables", block_tables, q, at::kInt, {B, block_tables.size(1)});
-  if (B == 0) return;
+  if (B == 0) return 0;
   TORCH_CHECK(q.size(0) % B == 0 && q.size(1) % D == 0, std::string(what) + ": q " + dims(q.sizes()) + " for " + num(B) + " sequences of head_dim " + num(D));
   const int64_t T = q.size(0) / B, hq = q.size(1) / D;
   TORCH_CHECK(hkv > 0 && hq % hkv == 0, std::string(what) + ": " + num(hq) + " query heads over " + num(hkv) + " KV heads");
@@ -189,7 +191,7 @@ void attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor
   TORCH_CHECK(T >= 1 && T * G <= SHARED_MAX_ROWS, std::string(what) + ": " + num(T) + " new tokens x " + num(G) +
               " heads of a KV group, at most " + num(SHARED_MAX_ROWS) + " rows");
   TORCH_CHECK(meta.device() == q.device() && meta.scalar_type() == at::kInt && meta.is_contiguous() &&
-                  meta.numel() >= shared_items_at((int)B) + SHARED_ITEM * n_prefix && (uintptr_t)meta.data_ptr() % 16 == 0,
+                  meta.numel() >= shared_items_at((int)B) + SHARED_ITEM * std::max(n_items, item_cap) && (uintptr_t)meta.data_ptr() % 16 == 0,
               what, ": groups of another batch");
   TORCH_CHECK(po.scalar_type() == at::kFloat && pml.scalar_type() == at::kFloat && po.device() == q.device() &&
                   pml.device() == q.device() && po.numel() / D <= pml.numel() / 2,
@@ -223,13 +225,14 @@ void attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Tensor
   a.hkv = (int)hkv;
   a.max_pages = (int)block_tables.size(1);
   a.page_size = (int)ps;
-  a.n_prefix = (int)n_prefix;
+  a.n_prefix = (int)(c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None ? n_items : item_cap);
   a.own_at = own_at;
   a.window = (int)window;
   a.slot_cap = po.numel() / D;
   a.num_sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   a.pool_pages = kcache.size(0);
   C10_CUDA_CHECK(launch_attn_shared(a, (int)D, scale, at::cuda::getCurrentCUDAStream()));
+  return a.n_prefix > 0 ? 3 : 2;
 }
 
 }  // namespace mesh

@@ -141,9 +141,6 @@ def attn_shared_prefix(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tens
         raise ValueError(f"cache {tuple(kcache.shape)} does not fit groups of {groups.hkv} KV heads of {groups.head_dim}")
     if groups.device != q.device:
         raise ValueError(f"groups on {groups.device}, q on {q.device}")
-    with torch.cuda.device(q.device):
-        capturing = torch.cuda.is_current_stream_capturing()
-    ext().attn_shared(q, kcache, vcache, block_tables, seq_lens, groups._meta, groups._po, groups._pml, out,
-                      groups._err, groups.item_cap if capturing else groups.n_items, groups._own_at, scale, window)
-    _count(2 + (capturing or groups.n_items > 0))
+    _count(ext().attn_shared(q, kcache, vcache, block_tables, seq_lens, groups._meta, groups._po, groups._pml, out,
+                             groups._err, groups.n_items, groups.item_cap, groups._own_at, scale, window))
     return out
