@@ -206,8 +206,19 @@ class DecodeGraphs:
 # again. Measured with 8 KV heads: 2 sessions behind 4096 keys (17 MB) 13.8 us against 11.3, 4 behind 4096 (50 MB) 14.4 against
 # 15.9, 16 behind 4096 (252 MB) 18.5 against 66.2; 64 behind 256 (66 MB, mostly found in L2) 18.2 against 15.5.
 SHARED_PREFIX_MIN_BYTES = 64 << 20
-# keeps the thresholds that accept drafts apart from those that draw tokens at the same position
+# Rejection sampling needs its uniforms to be independent of the drafts, and a draft model served by an engine like this one
+# may have drawn them with the session's own seed: the thresholds that accept drafts, and the one that draws the token after
+# them, are apart from decode_step's and prefill's at every position, and from one another (they differ above any position).
 _ACCEPT_SEED = 0x5EED_D4AF7
+_DRAW_SEED = 0x3D7A_0000_5EED
+
+
+def _verify_thresholds(seed_base: int, kv_len: int, n: int) -> Tuple[List[float], float]:
+    """The uniforms with which ``verify_step`` accepts each of ``n`` drafts behind ``kv_len`` keys and draws the token after
+    the accepted ones. Without drafts the token is decode_step's, drawn with its threshold."""
+    from ..oracle.tensor_ops import deterministic_sample_threshold
+    accept = [deterministic_sample_threshold(seed_base ^ (kv_len + 1 + k) ^ _ACCEPT_SEED) for k in range(n)]
+    return accept, deterministic_sample_threshold(seed_base ^ (kv_len + 1) ^ (_DRAW_SEED if n else 0))
 
 
 class Engine:
@@ -682,10 +693,10 @@ class Engine:
         in one pass, keeps those that its own distribution allows and adds one of its own. ``drafts``: session id ->
         proposed next tokens (possibly none); ``probs``: session id -> [drafts, vocabulary] probabilities they were
         drawn from (sessions without: guesses). Greedy sessions then generate exactly what ``decode_step`` would, sampled
-        ones (temperature with top_p 1) what it would in distribution. Returns the new tokens per session, which
-        are appended to it."""
+        ones (temperature with top_p 1) what it would in distribution. Drafts may come from an engine whose sessions have the
+        same seeds and decode or prefill them; one that verifies drafts of its own needs other seeds. Returns the new tokens
+        per session, which are appended to it."""
         from .. import ops
-        from ..oracle.tensor_ops import deterministic_sample_threshold
         r, ps = self.runner, self.page_size
         if r.world > 1:
             raise ValueError("verify_step needs the whole vocabulary on one rank (TP 1)")
@@ -738,9 +749,7 @@ class Engine:
             draft_ids[i, :n] = d
             if s.temperature > 0.0 and s.top_p > 0.0:
                 inv_t[i] = 1.0 / s.temperature
-            # the token drawn at a position has the threshold decode_step would use there; accepting has one of its own
-            u[i, :n] = [deterministic_sample_threshold(s.seed_base ^ (s.kv_len + 1 + k) ^ _ACCEPT_SEED) for k in range(n)]
-            u[i, K] = deterministic_sample_threshold(s.seed_base ^ (s.kv_len + 1))
+            u[i, :n], u[i, K] = _verify_thresholds(s.seed_base, s.kv_len, n)
         dev = self.device
         up = lambda a: torch.from_numpy(a).pin_memory().to(dev, non_blocking=True)
         index = {s.sid: i for i, s in enumerate(act)}

@@ -1,0 +1,83 @@
+"""Sessions that share pages and verify drafts, at their edges: drafts that another engine drew with the same seeds."""
+import pytest
+import torch
+
+from mesh_b200 import ops
+from mesh_b200.engine.serving import _verify_thresholds
+from test_fork_verify_gpu import _engine, _prompt
+from test_sharing_gpu import _i32, _verify_plain
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.fixture(autouse=True)
+def _check_err():
+    yield
+    ops.scratch(torch.device("cuda", torch.cuda.current_device())).check("kernel")
+
+
+def _draft(eng, prompts, counts, temps, seeds):
+    """Tokens that a draft model's engine gives behind each prompt, and the probabilities they were drawn from."""
+    eng.runner.keep_logits = True
+    sids = [eng.submit(p, c, temperature=t, seed_base=z) for p, c, t, z in zip(prompts, counts, temps, seeds)]
+    eng.prefill_step(token_budget=1 << 20)
+    assert not eng.waiting
+    rows = {i: [eng.runner.last_logits[i].clone()] for i in range(len(sids))}
+    for k in range(1, max(counts)):
+        at = {i: eng.sessions[sid].slot for i, sid in enumerate(sids) if counts[i] > k}
+        eng.decode_step()
+        for i, slot in at.items():
+            rows[i].append(eng.runner.last_logits[slot].clone())
+    eng.flush_history()
+    return [eng.sessions[sid].generated for sid in sids], [torch.softmax(torch.stack(rows[i]) / t, -1) for i, t in enumerate(temps)]
+
+
+def test_sampled_verification_is_the_rule_on_the_targets_logits():
+    """Sessions with a draft model's tokens and probabilities, with guesses, and with none, in one step: what each keeps and
+    draws is what the rejection rule gives for the logits of that step and the session's uniforms. The draft model has the
+    target's weights, seeds and temperature, so nearly all of its tokens are accepted; one guess in many thousands is."""
+    eng, cfg = _engine()
+    draft, _ = _engine(graphs=False)
+    V, n_new = cfg.vocab_size, 26
+    prompts = [_prompt(cfg, n, seed=n) for n in (5, 33, 16, 47, 20)]
+    temps, seeds = [1.0, 0.7, 1.3, 1.0, 1.0], [0, 0, 9, 9, 12345]
+    sids = [eng.submit(p, n_new, temperature=t, seed_base=z) for p, t, z in zip(prompts, temps, seeds)]
+    eng.prefill_step(token_budget=1 << 20)
+    eng.flush_history()
+    accepted = refused = 0
+    for turn in range(n_new):
+        act = [i for i, s in enumerate(sids) if eng.sessions[s].status == "decoding"]
+        if not act:
+            break
+        state = {i: (list(eng.sessions[sids[i]].generated), eng.sessions[sids[i]].kv_len) for i in act}
+        modelled = [i for i in act if (i + turn) % 4 < 2]
+        drafts, probs = {sids[i]: [] for i in act}, {}
+        if modelled:
+            counts = [1 + (i + turn) % 5 for i in modelled]
+            got, q = _draft(draft, [prompts[i] + state[i][0] for i in modelled], counts, [temps[i] for i in modelled],
+                            [seeds[i] for i in modelled])
+            for i, d, x in zip(modelled, got, q):
+                drafts[sids[i]], probs[sids[i]] = d, x
+        for i in act:
+            if i not in modelled and (i + turn) % 4 == 2:
+                drafts[sids[i]] = [(17 * turn + k) % V for k in range(1 + turn % 3)]
+        new = eng.verify_step(drafts, probs)
+        T = eng.runner.last_logits.shape[0] // len(act)
+        logits = eng.runner.last_logits.view(len(act), T, V)
+        for j, i in enumerate(act):
+            d = drafts[sids[i]][:n_new - len(state[i][0]) - 1]
+            n = len(d)
+            acc, draw = _verify_thresholds(seeds[i], state[i][1], n)
+            q = probs[sids[i]][None, :n] if sids[i] in probs and n else None
+            tokens, a, _, near = _verify_plain(logits[j:j + 1, :n + 1], _i32([d]).view(1, n), torch.tensor([acc + [draw]], dtype=torch.float32),
+                                               torch.tensor([1.0 / temps[i]], dtype=torch.float32), q, None)
+            assert near > 1e-11  # no decision within the rounding of 64-bit sums
+            assert new[sids[i]] == tokens[0][:a[0] + 1], (turn, i)
+            assert eng.sessions[sids[i]].generated == state[i][0] + new[sids[i]]
+            accepted += a[0]
+            refused += n > a[0]
+    assert accepted >= 20 and refused >= 10
+    assert all(len(eng.sessions[s].generated) == n_new for s in sids) and eng.alloc.num_used == 0
+    eng.close()
+    draft.close()
