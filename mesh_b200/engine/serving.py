@@ -19,7 +19,7 @@ B200 specifics:
 from __future__ import annotations
 
 import time
-from collections import deque
+from collections import Counter, deque
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Tuple
 
@@ -666,8 +666,14 @@ class Engine:
     def compact(self) -> int:
         """Move the live KV pages to the front of the pool (after sessions of many lengths have come and gone), so that
         everything from the returned page number up is free. Sessions, block tables and captured decode graphs carry
-        on; call it between steps."""
+        on; call it between steps. An error that an earlier step recorded, or pages that something other than this engine's
+        sessions has taken from the allocator (they would be written over), are raised before anything moves."""
         from .. import ops
+        self.flush_history()
+        holders = Counter(p for s in self.running if s is not None for p in s.pages)
+        if len(holders) != self.alloc.num_used or any(self.alloc.refs(p) != n for p, n in holders.items()):
+            raise RuntimeError(f"compact: the sessions hold {len(holders)} pages, the allocator has given out "
+                               f"{self.alloc.num_used}, or some to other holders too")
         d = self.dec
         if self.bt_dirty:
             d.block_tables.copy_(torch.from_numpy(self.bt_host).pin_memory(), non_blocking=True)
@@ -676,13 +682,14 @@ class Engine:
         counts = torch.tensor(held, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
         _, remap, live = ops.kv_pages_compact(self.runner.kv.k, self.runner.kv.v, d.block_tables, counts,
                                               reserved=self.alloc_reserved, out_tables=d.block_tables)
+        # the pages have moved: the host follows before anything may be raised
         remap = remap.cpu().tolist()
-        self.check_device()
         self.alloc.remap(remap)
         for s in self.running:
             if s is not None:
                 s.pages = [remap[p] for p in s.pages]
                 self.bt_host[s.slot, :len(s.pages)] = s.pages
+        self.check_device()
         return int(live)
 
     # ----------------------------------------------------------------------------- drafts

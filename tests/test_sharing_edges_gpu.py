@@ -1,10 +1,11 @@
-"""Sessions that share pages and verify drafts, at their edges: drafts that another engine drew with the same seeds."""
+"""Sessions that share pages and verify drafts, at their edges: drafts that another engine drew with the same seeds, compactions
+that are refused."""
 import pytest
 import torch
 
 from mesh_b200 import ops
 from mesh_b200.engine.serving import _verify_thresholds
-from test_fork_verify_gpu import _engine, _prompt
+from test_fork_verify_gpu import _engine, _prompt, _start
 from test_sharing_gpu import _i32, _verify_plain
 
 pytestmark = pytest.mark.gpu
@@ -81,3 +82,49 @@ def test_sampled_verification_is_the_rule_on_the_targets_logits():
     assert all(len(eng.sessions[s].generated) == n_new for s in sids) and eng.alloc.num_used == 0
     eng.close()
     draft.close()
+
+
+@pytest.mark.parametrize("why", ["an earlier error", "a page of its own", "a second holder"])
+def test_a_refused_compaction_moves_nothing(why):
+    """The engine goes on with the tokens it gives without, and compacts once the reason is gone."""
+    eng, cfg = _engine(pages=60)
+    prompts, news = [_prompt(cfg, n, seed=n) for n in (50, 20, 33, 40, 9)], [6, 30, 4, 30, 30]
+
+    def run(refuse):
+        sids = _start(eng, prompts, 30)
+        for sid, n in zip(sids, news):
+            eng.sessions[sid].max_new_tokens = n
+        for _ in range(8):  # the first and the third are through: holes
+            eng.decode_step()
+        if refuse:
+            eng.flush_history()
+            torch.cuda.synchronize()
+            pages = {s.sid: list(s.pages) for s in eng.running if s}
+            kept = eng.runner.kv.k.clone(), eng.runner.kv.v.clone()
+            tables = eng.bt_host.copy()
+            if why == "an earlier error":
+                ops.scratch(eng.device).err.fill_(5)
+            elif why == "a page of its own":
+                extra = eng.alloc.alloc(eng.alloc.num_free)[-1:]  # the last one stays taken
+                eng.alloc.free([p for p in range(1, 60) if eng.alloc.refs(p) and p not in extra + sum(pages.values(), [])])
+            else:
+                extra = eng.running[1].pages[:1]
+                eng.alloc.share(extra)
+            used = eng.alloc.num_used
+            with pytest.raises(RuntimeError, match="bad argument" if why == "an earlier error" else "holders"):
+                eng.compact()
+            assert torch.equal(eng.runner.kv.k, kept[0]) and torch.equal(eng.runner.kv.v, kept[1])
+            assert pages == {s.sid: s.pages for s in eng.running if s} and (eng.bt_host == tables).all() and eng.alloc.num_used == used
+            for _ in range(3):
+                eng.decode_step()
+            if why != "an earlier error":
+                eng.alloc.free(extra)
+            live = eng.compact()
+            assert live == 1 + eng.alloc.num_used and max(p for s in eng.running if s for p in s.pages) < live
+        eng.run()
+        return [eng.sessions[s].generated for s in sids]
+
+    want = run(False)
+    assert run(True) == want
+    assert eng.alloc.num_used == 0
+    eng.close()
