@@ -699,7 +699,7 @@ class Engine:
         """One step in which sessions advance by several tokens: the target model scores each session's drafted tokens
         in one pass, keeps those that its own distribution allows and adds one of its own. ``drafts``: session id ->
         proposed next tokens (possibly none); ``probs``: session id -> [drafts, vocabulary] probabilities they were
-        drawn from (sessions without: guesses). Greedy sessions then generate exactly what ``decode_step`` would, sampled
+        drawn from, a row for each (sessions without: guesses). Greedy sessions then generate exactly what ``decode_step`` would, sampled
         ones (temperature with top_p 1) what it would in distribution. Drafts may come from an engine whose sessions have the
         same seeds and decode or prefill them; one that verifies drafts of its own needs other seeds. Returns the new tokens
         per session, which are appended to it."""
@@ -726,6 +726,11 @@ class Engine:
             if any(not 0 <= int(t) < self.cfg.vocab_size for t in d):
                 raise ValueError(f"session {s.sid}: a draft outside the vocabulary")
             want[s.sid] = [int(t) for t in d]
+            q = None if probs is None else probs.get(s.sid)
+            if q is not None and (q.dim() != 2 or q.shape[0] < len(drafts[s.sid]) or q.shape[1] != self.cfg.vocab_size
+                                  or not q.is_floating_point()):
+                raise ValueError(f"session {s.sid}: probabilities {tuple(q.shape)} {q.dtype} for {len(drafts[s.sid])} drafts "
+                                 f"of a vocabulary of {self.cfg.vocab_size}")
         self.flush_history()
         K = max(len(d) for d in want.values())
         T, B, V = K + 1, len(act), self.cfg.vocab_size
@@ -780,7 +785,7 @@ class Engine:
             q = torch.zeros(B, K, V, dtype=torch.float32, device=dev)
             for i, s in enumerate(act):
                 n = len(want[s.sid])
-                if s.sid in probs:
+                if probs.get(s.sid) is not None:
                     q[i, :n] = probs[s.sid][:n]
                 else:  # a guess: all of its draft distribution is on the token itself
                     q[i, :n].scatter_(1, up(draft_ids[i, :n].astype(np.int64))[:, None], 1.0)

@@ -1,5 +1,5 @@
 """Sessions that share pages and verify drafts, at their edges: drafts that another engine drew with the same seeds, compactions
-that are refused."""
+that are refused, probabilities that do not fit their drafts."""
 import pytest
 import torch
 
@@ -127,4 +127,22 @@ def test_a_refused_compaction_moves_nothing(why):
     want = run(False)
     assert run(True) == want
     assert eng.alloc.num_used == 0
+    eng.close()
+
+
+def test_probabilities_that_do_not_fit_their_drafts_are_refused():
+    """One row would be spread over all drafts. A refused step leaves the sessions as they were."""
+    eng, cfg = _engine()
+    V = cfg.vocab_size
+    a, b = _start(eng, [_prompt(cfg, 12), _prompt(cfg, 20)], 30, temperature=1.0)
+    eng.flush_history()
+    before = [(list(eng.sessions[s].generated), eng.sessions[s].kv_len) for s in (a, b)]
+    good = torch.full((3, V), 1.0 / V, device=DEV)
+    for bad in (good[:1], good[:2], good[0], good[:, :V - 1], good[:, :1], good[None], good.long()):
+        with pytest.raises(ValueError, match="probabilities"):
+            eng.verify_step({b: [1], a: [1, 2, 3]}, {a: bad})
+    assert before == [(eng.sessions[s].generated, eng.sessions[s].kv_len) for s in (a, b)]
+    got = eng.verify_step({a: [1, 2, 3], b: [4]}, {a: good, b: None})
+    assert all(1 <= len(g) <= 4 for g in got.values())
+    assert eng.verify_step({a: [1], b: []}, {a: good.cpu()})[b]  # rows behind the drafts are not looked at
     eng.close()
