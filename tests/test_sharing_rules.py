@@ -1,7 +1,10 @@
-"""Host rules of sessions that share pages and verify drafts (CPU): the uniforms of a verified step."""
+"""Host rules of sessions that share pages and verify drafts (CPU): the uniforms of a verified step, arguments that are
+refused."""
 import numpy as np
 import pytest
+import torch
 
+from mesh_b200 import ops
 from mesh_b200.engine import serving
 from mesh_b200.oracle.tensor_ops import deterministic_sample_threshold
 
@@ -42,3 +45,12 @@ def test_thresholds_of_a_session_are_all_different():
     assert serving._verify_thresholds(77, 40, 5)[0][3] == serving._verify_thresholds(77, 43, 1)[0][0]
     # without drafts the token is decode_step's
     assert serving._verify_thresholds(77, 40, 0) == ([], deterministic_sample_threshold(77 ^ 41))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, float("nan"), float("inf"), 1e-40])
+def test_attention_over_shared_prefixes_refuses_a_scale_that_is_not_positive(scale):
+    plan = ops.PrefixGroups(2, 4, 2, 64, device="cpu")
+    q, cache = torch.zeros(2, 256, dtype=torch.bfloat16), torch.zeros(3, 2, 16, 64, dtype=torch.bfloat16)
+    table, lens = torch.ones(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="scale"):
+        ops.attn_shared_prefix(q, cache, cache, table, lens, plan, torch.empty_like(q), scale)
