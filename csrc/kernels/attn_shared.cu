@@ -9,7 +9,8 @@
 //   own items      (sequence, KV head, key range): the rows of one sequence against the rest of its keys.
 // Every item leaves, per row, the maximum m, the sum l of 2^(s - m) and the unnormalised output in fp32; the
 // combine kernel merges a row's partials: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i. All partials of a row
-// are summed in a fixed order, so results do not depend on the schedule.
+// are summed in a fixed order, so results do not depend on the schedule. NaN in a row's query or in a key it attends makes
+// the row NaN however its keys are cut: its sums l are NaN, and only a sum of exactly 0 counts as nothing seen.
 //
 // Measured (32 query and 8 KV heads of 128): 64 sessions with up to 512 keys of their own behind 8192 shared ones 36.9 us, of
 // which reading every key once takes 15.8 at the copy rate; 128 with up to 1024 behind 16384 92 us (52.5); 4 forks of 512
@@ -359,13 +360,13 @@ __device__ __forceinline__ void own_worker(const CUtensorMap& tmK, const CUtenso
         const int x0 = row0 + r, t = x0 / a.G;
         __nv_bfloat16* out = a.out + ((long)(p.b * a.T + t) * hq + h * a.G + x0 - t * a.G) * D + (lane >> 2);
         float* po = a.po + (part + r) * D + (lane >> 2);
-        const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
+        const float inv = 1.f / l[i];  // a NaN sum stays one; rows without a key give zeros whatever the values hold
 #pragma unroll
         for (int x = 0; x < D / 16; ++x)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             if (whole)
-              out[x * 16 + e * 8] = f2bf(o[x][2 * e + i] * inv);
+              out[x * 16 + e * 8] = f2bf(l[i] == 0.f ? 0.f : o[x][2 * e + i] * inv);
             else
               po[x * 16 + e * 8] = o[x][2 * e + i];
           }
@@ -450,11 +451,12 @@ __global__ void __launch_bounds__(128) combine_kernel(const Args a) {
       float mx = ml.x;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      const float mn = fmaxf(M, mx);
-      if (mn == -INFINITY) continue;
-      const float corr = ex2_ftz(M - mn), f = ex2_ftz(ml.x - mn);  // 0 for a partial that saw nothing
+      const float mn = fmaxf(M, mx), mb = mn == -INFINITY ? 0.f : mn;
+      // 0 where nothing was seen: m is -inf and l is 0, or NaN where every score was one, which then stays in the sum
+      const float corr = ex2_ftz(M - mb), e = ex2_ftz(ml.x - mb);
+      const float f = ml.y == 0.f ? -1.f : e;  // the output of a partial that saw nothing may not have been written
       M = mn;
-      den = den * corr + (ml.x > -INFINITY ? ml.y * f : 0.f);
+      den = den * corr + ml.y * e;
 #pragma unroll
       for (int v = 0; v < V; ++v) acc[v] *= corr;
       for (int i = i0; i < min(n, i0 + 32); i += N) {
@@ -462,7 +464,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const Args a) {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
           const float w = __shfl_sync(0xffffffffu, f, (i + k) & 31);
-          if (i + k < n && w > 0.f)  // the output of a partial that saw nothing may not have been written
+          if (i + k < n && w >= 0.f)
 #pragma unroll
             for (int v = 0; v < V; ++v) acc[v] = fmaf(p[k][v], w, acc[v]);
         }
@@ -497,7 +499,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const Args a) {
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
-  const float inv = den > 0.f ? 1.f / den : 0.f;
+  const float inv = den == 0.f ? 0.f : 1.f / den;
   __nv_bfloat16* dst = a.out + (long)row * D + lane * V;
 #pragma unroll
   for (int v = 0; v < V; v += 2) *reinterpret_cast<uint32_t*>(dst + v) = pack_bf16x2(acc[v] * inv, acc[v + 1] * inv);

@@ -404,7 +404,7 @@ __global__ void __maxnreg__(MAX_REGS)
         named_bar_sync(1, ns * BM);  // every stream is done with the query tiles and the rings
         if (ok && warp_live) {
           if (slot >= 0) a.pml[slot] = make_float2(m_used, l);
-          const long to = slot >= 0 && l > 0.f ? slot : -1;
+          const long to = slot >= 0 && l != 0.f ? slot : -1;  // NaN too: the merge reads what has a sum
           if (nblk > 0 && __any_sync(0xffffffffu, to >= 0)) {
             // A row is one TMEM lane: the warp lays its 32 rows out in shared memory and writes them row by row.
             uint8_t* rows_sm = q_sm + (x - lane) * C::STAGED;

@@ -1,12 +1,14 @@
 """Sessions that share pages and verify drafts, at their edges: drafts that another engine drew with the same seeds, compactions
-that are refused, probabilities that do not fit their drafts."""
+that are refused, probabilities that do not fit their drafts, and NaN in queries and keys of the attention over shared prefixes."""
+import math
+
 import pytest
 import torch
 
 from mesh_b200 import ops
 from mesh_b200.engine.serving import _verify_thresholds
 from test_fork_verify_gpu import _engine, _prompt, _start
-from test_sharing_gpu import _i32, _verify_plain
+from test_sharing_gpu import _attn_64, _check_attn, _i32, _shared_case, _verify_plain
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -146,3 +148,45 @@ def test_probabilities_that_do_not_fit_their_drafts_are_refused():
     assert all(1 <= len(g) <= 4 for g in got.values())
     assert eng.verify_step({a: [1], b: []}, {a: good.cpu()})[b]  # rows behind the drafts are not looked at
     eng.close()
+
+
+@pytest.mark.parametrize("hq,hkv,D", [(8, 2, 128), (4, 2, 64), (8, 8, 128)])
+@pytest.mark.parametrize("T", [1, 2])
+@pytest.mark.parametrize("shared", [True, False])
+@pytest.mark.parametrize("where", ["query", "shared key", "own key", "last key"])
+def test_nan_makes_the_rows_that_meet_it_nan(hq, hkv, D, T, shared, where):
+    """Whether their keys are one worker's, cut over several, or behind a prefix, and whatever an earlier call left in the
+    workspace; the other rows keep their values."""
+    groups = [([3, 0, 1], 300), ([4, 2], 1000)]
+    own = [T + 5, T, 1500, 70, 2500, T + 1, 90, 3000, 0]
+    q, kc, vc, table, lens = _shared_case(9, T, hq, hkv, D, 16, groups, own, seed=61)
+    G, scale = hq // hkv, 1.0 / math.sqrt(D)
+    clean, mag = _attn_64(q, kc, vc, table, lens, T, scale)
+    plan = ops.PrefixGroups(9, hq, hkv, D, q_len=T).set(groups if shared else [])
+    out = torch.empty_like(q)
+    ops.attn_shared_prefix(q, kc, vc, table, lens, plan, out, scale)  # leaves finite partials behind
+    _check_attn(out, clean, mag)
+    hit = torch.zeros(9, T, hq, dtype=torch.bool)
+    pos = lens.cpu()[:, None] - T + torch.arange(T)
+    if where == "query":
+        for b, t, h in ((0, 0, 1), (2, T - 1, hq - 1), (5, 0, 0), (7, T - 1, 2), (8, 0, 0)):
+            q.view(9, T, hq, D)[b, t, h] = math.nan
+            hit[b, t, h] = pos[b, t] >= 0  # the empty slot has no key, so it stays zero
+    else:
+        h = hkv - 1
+        spots = {"shared key": [(3, 131), (4, 990)], "own key": [(2, 1700), (3, 310), (7, 40), (6, 33)],
+                 "last key": [(b, int(lens[b]) - 1) for b in (0, 2, 5, 7)]}[where]
+        for b, key in spots:
+            kc[table[b, key // 16].long(), h, key % 16, 3] = math.nan
+            members = next((g for g, n in groups if b in g and key < n), [b])
+            for m in members:
+                for t in range(T):
+                    if pos[m, t] >= key:
+                        hit[m, t, h * G:(h + 1) * G] = True
+    assert hit.any() and not hit.all()
+    for _ in range(2):
+        ops.attn_shared_prefix(q, kc, vc, table, lens, plan, out, scale)
+        bad = out.view(9 * T, hq, D).isnan()
+        assert torch.equal(bad.all(-1).cpu().view(9, T, hq), hit) and torch.equal(bad.any(-1), bad.all(-1))
+        keep = ~bad.view(9 * T, hq * D)
+        _check_attn(torch.where(keep, out, 0), torch.where(keep, clean, 0), mag)
