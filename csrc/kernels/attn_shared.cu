@@ -280,14 +280,16 @@ __device__ __forceinline__ void own_worker(const CUtensorMap& tmK, const CUtenso
         if (!ok) break;
         const int key0 = (s0 + i) * SLICE;
         const uint32_t kb = smem_u32(ring + s * g::SLICE_BYTES), vb = kb + g::HALVES * g::BOX;
-        // Keys past the range may hold anything (a page's unused tail): their values must not reach the products as
-        // NaN or infinity times a zero weight. Clearing them in the fragments costs two masks; clearing them in shared
-        // memory needs a proxy fence, which waited for the loads in flight.
+        // Keys past the range may hold anything (a page's unused tail), and so may those before it (this sequence's own
+        // copy of a prefix that ends inside the slice): their values must not reach the products as NaN or infinity times
+        // a zero weight. Clearing them in the fragments costs two masks; clearing them in shared memory needs a proxy
+        // fence, which waited for the loads in flight.
         uint32_t keep[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const int left = k1 - (key0 + x * 8 + (lane & 3) * 2);  // of this lane's two keys
+          const int key = key0 + x * 8 + (lane & 3) * 2, left = k1 - key;  // the first of this lane's two keys
           keep[x] = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+          if (key < k0) keep[x] &= key + 1 < k0 ? 0u : 0xffff0000u;
         }
         float sc[4], sd[4];  // keys lane / 4 and 8 below; two chains of products each
 #pragma unroll

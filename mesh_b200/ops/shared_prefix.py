@@ -63,9 +63,9 @@ class PrefixGroups:
 
     def set(self, groups: Sequence[Tuple[Sequence[int], int]]) -> "PrefixGroups":
         """``groups``: (sequences, shared keys) pairs. The first ``shared`` keys of every sequence of a group
-        must be the same tokens; they are read through the block table of the group's first sequence. A
-        sequence may be in one group at most; one in none attends its own pages alone. Not inside a capture: the
-        list comes from the host."""
+        must be the same tokens; they are read through the block table of the group's first sequence, which has to
+        hold them all, and what the others' tables hold for them is not used. A sequence may be in one group at
+        most; one in none attends its own pages alone. Not inside a capture: the list comes from the host."""
         if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("PrefixGroups.set copies from host memory: call it before the capture, or between replays")
         B, T, G = self.batch, self.q_len, self.group

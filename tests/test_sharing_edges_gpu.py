@@ -1,5 +1,6 @@
 """Sessions that share pages and verify drafts, at their edges: drafts that another engine drew with the same seeds, compactions
-that are refused, probabilities that do not fit their drafts, and NaN in queries and keys of the attention over shared prefixes."""
+that are refused, probabilities that do not fit their drafts, and NaN in queries and keys of the attention over shared prefixes
+or in pages that nobody attends."""
 import math
 
 import pytest
@@ -190,3 +191,32 @@ def test_nan_makes_the_rows_that_meet_it_nan(hq, hkv, D, T, shared, where):
         assert torch.equal(bad.all(-1).cpu().view(9, T, hq), hit) and torch.equal(bad.any(-1), bad.all(-1))
         keep = ~bad.view(9 * T, hq * D)
         _check_attn(torch.where(keep, out, 0), torch.where(keep, clean, 0), mag)
+
+
+@pytest.mark.parametrize("hq,hkv,D", [(8, 2, 128), (4, 2, 64), (16, 1, 128)])
+@pytest.mark.parametrize("T", [1, 3])
+@pytest.mark.parametrize("window", [0, 45])
+@pytest.mark.parametrize("prefix", [1, 15, 31, 200, 333])
+def test_what_nobody_attends_may_hold_anything(hq, hkv, D, T, window, prefix):
+    """The members' own copies of a prefix that ends inside a page (it is read through the first sequence), the keys that every
+    row's window has left behind, and the tails of pages hold NaN and infinity."""
+    groups = [([2, 0, 4, 1], prefix)]
+    own = [T + 60, T, T + 7, 900, T + 200, 77, T + 1]
+    q, kc, vc, table, lens = _shared_case(7, T, hq, hkv, D, 16, groups, own, seed=71, junk=True)
+    want, mag = _attn_64(q, kc, vc, table, lens, T, 1.0 / math.sqrt(D), window)
+    full = prefix // 16
+    for b in (0, 4, 1):
+        page = int(table[b, full])
+        kc[page, :, :prefix % 16] = math.nan
+        vc[page, :, :prefix % 16] = math.inf
+        table[b, :full] = 0  # as if they had never been told of the shared pages
+    kc[0], vc[0] = math.nan, math.inf
+    if window:
+        for b in (3, 5):
+            for key in range(max(0, int(lens[b]) - T + 1 - window)):
+                page = int(table[b, key // 16])
+                kc[page, :, key % 16], vc[page, :, key % 16] = math.nan, -math.inf
+    plan = ops.PrefixGroups(7, hq, hkv, D, q_len=T).set(groups)
+    out = torch.full_like(q, math.nan)
+    ops.attn_shared_prefix(q, kc, vc, table, lens, plan, out, 1.0 / math.sqrt(D), window=window)
+    _check_attn(out, want, mag)
