@@ -221,6 +221,61 @@ def _verify_thresholds(seed_base: int, kv_len: int, n: int) -> Tuple[List[float]
     return accept, deterministic_sample_threshold(seed_base ^ (kv_len + 1) ^ (_DRAW_SEED if n else 0))
 
 
+def _shared_prefixes(paths: List[List[int]]) -> List[Tuple[List[int], int]]:
+    """The groups [(members, first pages they have in common)] of sequences with these page lists that leave the fewest pages
+    to read, where a group reads its common pages once; a sequence is in one group at most.
+
+    The lists form a tree (equal pages at one place come from a fork, so all pages before are equal too). A group is a node of
+    it, of depth d pages: reading it once costs d and saves d for every sequence below it that no deeper group takes. So with
+    e the depth of the group further up that its sequences would be in otherwise (0: none), best(leaf, e) = e and
+    best(node, e) = max(sum best(child, e), sum best(child, d) - d), for all e at once."""
+    order = sorted(range(len(paths)), key=lambda i: paths[i])
+    depth, parent, leaves = [0], [-1], []  # nodes, the root first; leaves: (sequence, node it hangs from)
+    stack = [0]
+    for k, i in enumerate(order):
+        common = 0
+        if k:
+            a, b = paths[order[k - 1]], paths[i]
+            hi = min(len(a), len(b))
+            while common < hi:  # pages are equal up to one place and differ from there
+                mid = (common + hi + 1) // 2
+                common, hi = (mid, hi) if a[mid - 1] == b[mid - 1] else (common, mid - 1)
+        # this sequence hangs, for now, from the node of what it has in common with the one before
+        last = -1
+        while depth[stack[-1]] > common:
+            last = stack.pop()
+        if depth[stack[-1]] < common:
+            depth.append(common)
+            parent.append(stack[-1])
+            if last >= 0:
+                parent[last] = len(depth) - 1
+            elif leaves:
+                leaves[-1] = (leaves[-1][0], len(depth) - 1)
+            stack.append(len(depth) - 1)
+        leaves.append((i, stack[-1]))
+    below = sorted(range(1, len(depth)), key=lambda x: depth[x])  # parents first
+    chain = {0: [0]}  # depths from the root to a node
+    for x in below:
+        chain[x] = chain[parent[x]] + [depth[x]]
+    total = {x: np.zeros(len(chain[x]), dtype=np.int64) for x in chain}
+    for _, x in leaves:
+        total[x] += chain[x]
+    opened = {}
+    for x in reversed(below):
+        with_it = total[x][-1] - depth[x]
+        opened[x] = with_it > total[x][:-1]
+        total[parent[x]] += np.maximum(total[x][:-1], with_it)
+    group = {0: (0, 0)}  # the group that the sequences hanging from a node are in, and its place in the node's chain
+    for x in below:
+        up, at = group[parent[x]]
+        group[x] = (x, len(chain[x]) - 1) if opened[x][at] else (up, at)
+    members: Dict[int, List[int]] = {}
+    for i, x in sorted(leaves):
+        if group[x][0]:
+            members.setdefault(group[x][0], []).append(i)
+    return [(m, depth[x]) for x, m in members.items()]
+
+
 class Engine:
     """One rank's engine. All ranks of a TP group must call the same methods in the same order."""
 
@@ -603,23 +658,18 @@ class Engine:
     def _prefix_groups(self, act: List[Session], slot=None, min_bytes: Optional[int] = None) -> List[tuple]:
         """[(slots, keys)] of the sessions among ``act`` that hold the same first pages, where reading those once
         pays. Sessions come to share pages by ``fork_session``; without forks this is one look at each session."""
-        first: Dict[int, List[Session]] = {}
-        for s in act:
-            if s.forked and s.pages:
-                first.setdefault(s.pages[0], []).append(s)
-        r = self.runner
-        if not first or self.page_size % 16 or r.D not in (64, 128) or r.hq // r.hkv > 64 or self.max_batch > 1024:
+        forked = [s for s in act if s.forked and s.pages]
+        r, ps = self.runner, self.page_size
+        if len(forked) < 2 or ps % 16 or r.D not in (64, 128) or r.hq // r.hkv > 64 or self.max_batch > 1024:
             return []
         out, saved = [], 0
-        for group in first.values():
-            n = min(s.kv_len for s in group) // self.page_size  # full pages
-            a = group[0].pages
-            for s in group[1:]:
-                while s.pages[:n] != a[:n]:
-                    n -= 1
-            if len(group) > 1 and n > 0:
-                out.append(([s.slot if slot is None else slot[s.sid] for s in group], n * self.page_size))
-                saved += (len(group) - 1) * n * self.page_size * r.hkv * r.D * 4
+        for members, n in _shared_prefixes([s.pages[:s.kv_len // ps] for s in forked]):
+            keys = n * ps
+            # a window: attn_decode would read what it still covers, the prefix is read whole
+            again = sum(keys if not r.window else max(0, keys - max(0, forked[i].kv_len + 1 - r.window)) for i in members) - keys
+            if again > 0:
+                out.append(([forked[i].slot if slot is None else slot[forked[i].sid] for i in members], keys))
+                saved += again * r.hkv * r.D * 4
         return out if saved >= (SHARED_PREFIX_MIN_BYTES if min_bytes is None else min_bytes) else []
 
     @_on_device

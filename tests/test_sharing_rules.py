@@ -1,5 +1,8 @@
 """Host rules of sessions that share pages and verify drafts (CPU): the uniforms of a verified step, arguments that are
-refused."""
+refused, which sessions read their prefixes together."""
+import random
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 import torch
@@ -54,3 +57,89 @@ def test_attention_over_shared_prefixes_refuses_a_scale_that_is_not_positive(sca
     table, lens = torch.ones(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
     with pytest.raises(ValueError, match="scale"):
         ops.attn_shared_prefix(q, cache, cache, table, lens, plan, torch.empty_like(q), scale)
+
+
+# ------------------------------------------------------------------------------------ which sessions share
+def _forest(r, sessions, roots, step):
+    """Page lists as forks leave them: a child has the full pages of its parent at that moment, both go on with new ones."""
+    page = iter(range(1, 1 << 30))
+    paths = [[next(page) for _ in range(r.randint(0, step))] for _ in range(roots)]
+    while len(paths) < sessions:
+        for p in paths:
+            if r.random() < 0.5:
+                p.extend(next(page) for _ in range(r.randint(0, step)))
+        paths.append(list(r.choice(paths)))
+    for p in paths:
+        p.extend(next(page) for _ in range(r.randint(0, 2)))
+    r.shuffle(paths)
+    return paths
+
+
+def _common(paths):
+    return next((i for i, x in enumerate(zip(*paths)) if len(set(x)) > 1), min(len(p) for p in paths))
+
+
+def _partitions(items):
+    if not items:
+        yield []
+        return
+    for rest in _partitions(items[1:]):
+        yield [[items[0]]] + rest
+        for i in range(len(rest)):
+            yield rest[:i] + [[items[0]] + rest[i]] + rest[i + 1:]
+
+
+@pytest.mark.parametrize("seed", range(120))
+def test_prefix_groups_save_the_most(seed):
+    """Against every partition of up to seven sequences."""
+    r = random.Random(seed)
+    paths = _forest(r, r.randint(1, 7), r.randint(1, 2), r.choice((1, 3, 9)))
+    best = max(sum((len(b) - 1) * _common([paths[i] for i in b]) for b in part) for part in _partitions(list(range(len(paths)))))
+    got = serving._shared_prefixes(paths)
+    flat = [i for m, _ in got for i in m]
+    assert len(flat) == len(set(flat)) and all(len(m) > 1 and 0 < n <= _common([paths[i] for i in m]) for m, n in got)
+    assert sum((len(m) - 1) * n for m, n in got) == best
+
+
+def test_prefix_groups_of_a_long_chain_of_forks():
+    """Every session forked from the one before, a page later: deeper than the interpreter's stack."""
+    paths = [list(range(1, i + 2)) + [10 ** 6 + i] for i in range(1500)]
+    got = serving._shared_prefixes(paths)
+    # halves above halves: groups of the deeper sequences leave the rest to a group further up
+    assert sum((len(m) - 1) * n for m, n in got) >= 1499 * 1500 // 4
+    assert all(paths[i][:n] == paths[m[0]][:n] for m, n in got for i in m)
+
+
+def _engine_of(sessions, window=0, hkv=8, D=128, ps=16):
+    eng = SimpleNamespace(runner=SimpleNamespace(hq=4 * hkv, hkv=hkv, D=D, window=window), page_size=ps, max_batch=128)
+    return lambda **kw: serving.Engine._prefix_groups(eng, sessions, **kw)
+
+
+def _session(sid, pages, kv_len, forked=True):
+    return serving.Session(sid, [1], 10, pages=pages, kv_len=kv_len, slot=sid, status="decoding", forked=forked)
+
+
+def test_an_early_branch_leaves_the_others_together():
+    """64 sessions share 8192 keys, one more parted from them after two pages."""
+    shared = list(range(1, 513))
+    many = [_session(i, shared + [1000 + i], 8192 + 5) for i in range(64)]
+    early = _session(64, shared[:2] + [2000, 2001], 50)
+    alone = _session(65, [3000, 3001], 20, forked=False)
+    for order in (many + [early, alone], [early] + many, [alone, early] + many[::-1]):
+        ((slots, keys),) = _engine_of(order)()
+        assert sorted(slots) == list(range(64)) and keys == 8192
+    # two that share too little by themselves still count where there is no least saving
+    other = [_session(70 + i, [4000, 4001 + i], 20) for i in range(2)]
+    assert sorted((len(s), k) for s, k in _engine_of(many + other)(min_bytes=0)) == [(2, 16), (64, 8192)]
+    assert _engine_of(other)() == [] and _engine_of([early, alone])(min_bytes=0) == []
+
+
+def test_a_window_counts_only_what_it_covers():
+    """Ordinary decoding reads the keys inside the window alone, a shared prefix is read whole."""
+    shared = list(range(1, 513))
+    many = [_session(i, shared + [1000 + i], 8192 + 5) for i in range(16)]
+    assert len(_engine_of(many)()) == 1
+    assert len(_engine_of(many, window=8192)()) == 1
+    assert _engine_of(many, window=512)(min_bytes=0) == []       # 16 x 506 keys against 8192
+    assert len(_engine_of(many, window=1024)(min_bytes=0)) == 1  # 16 x 1018
+    assert _engine_of(many, window=4)(min_bytes=0) == []
