@@ -290,6 +290,7 @@ class Engine:
         self.alloc_reserved = 1  # page 0: padded batch slots
         self.alloc = PageAllocator(runner.kv.num_pages, reserved=self.alloc_reserved)
         self._verify_groups: Dict[Tuple[int, int], object] = {}  # (sessions, tokens each) -> ops.PrefixGroups
+        self._prefixes: Dict[tuple, list] = {}  # ids of forked sessions -> their groups (_shared_prefixes)
         self.max_pages_per_seq = (ecfg.max_seq_len + ps - 1) // ps
         self.dec = DecodeGraphs(runner, max_batch, self.max_pages_per_seq, ecfg.use_cuda_graphs,
                                 ecfg.decode_batch_buckets)
@@ -662,8 +663,15 @@ class Engine:
         r, ps = self.runner, self.page_size
         if len(forked) < 2 or ps % 16 or r.D not in (64, 128) or r.hq // r.hkv > 64 or self.max_batch > 1024:
             return []
+        # What sessions have in common was settled when they forked: pages are only added behind it, and a compaction
+        # renumbers everyone's alike. So the groups stand until another set of sessions takes the step.
+        key = tuple(s.sid for s in forked)
+        if key not in self._prefixes:
+            if len(self._prefixes) >= 8:
+                self._prefixes.clear()
+            self._prefixes[key] = _shared_prefixes([s.pages[:s.kv_len // ps] for s in forked])
         out, saved = [], 0
-        for members, n in _shared_prefixes([s.pages[:s.kv_len // ps] for s in forked]):
+        for members, n in self._prefixes[key]:
             keys = n * ps
             # a window: attn_decode would read what it still covers, the prefix is read whole
             again = sum(keys if not r.window else max(0, keys - max(0, forked[i].kv_len + 1 - r.window)) for i in members) - keys

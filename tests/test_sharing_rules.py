@@ -111,7 +111,7 @@ def test_prefix_groups_of_a_long_chain_of_forks():
 
 
 def _engine_of(sessions, window=0, hkv=8, D=128, ps=16):
-    eng = SimpleNamespace(runner=SimpleNamespace(hq=4 * hkv, hkv=hkv, D=D, window=window), page_size=ps, max_batch=128)
+    eng = SimpleNamespace(runner=SimpleNamespace(hq=4 * hkv, hkv=hkv, D=D, window=window), page_size=ps, max_batch=128, _prefixes={})
     return lambda **kw: serving.Engine._prefix_groups(eng, sessions, **kw)
 
 
@@ -143,3 +143,70 @@ def test_a_window_counts_only_what_it_covers():
     assert _engine_of(many, window=512)(min_bytes=0) == []       # 16 x 506 keys against 8192
     assert len(_engine_of(many, window=1024)(min_bytes=0)) == 1  # 16 x 1018
     assert _engine_of(many, window=4)(min_bytes=0) == []
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_groups_that_stand_are_those_of_a_fresh_look(seed):
+    """Decoding, forks, departures and compactions in any order, with the allocator's own pages."""
+    from mesh_b200.engine.pages import _PyPageAllocator
+    r, ps = random.Random(seed), 16
+    alloc = _PyPageAllocator(600, 1)
+    live = []
+    eng = SimpleNamespace(runner=SimpleNamespace(hq=32, hkv=8, D=128, window=0), page_size=ps, max_batch=128, _prefixes={})
+
+    def grow(s, n):
+        s.kv_len += n
+        while len(s.pages) * ps < s.kv_len:
+            s.pages += alloc.alloc(1)
+
+    for sid in range(2):
+        live.append(_session(sid, [], 0, forked=False))
+        grow(live[-1], r.randint(20, 120))
+    sid = 2
+    for _ in range(120):
+        for s in live:
+            grow(s, 1)
+        op = r.random()
+        if op < 0.15 and len(live) < 9:
+            a = r.choice(live)
+            full = a.kv_len // ps
+            alloc.share(a.pages[:full])
+            a.forked = True
+            live.append(_session(sid, a.pages[:full] + (alloc.alloc(1) if a.kv_len % ps else []), a.kv_len))
+            sid += 1
+        elif op < 0.22 and len(live) > 2:
+            alloc.free(live.pop(r.randrange(len(live))).pages)
+        elif op < 0.3:
+            used = sorted({p for s in live for p in s.pages})
+            n = 1 + len(used)
+            remap = [-1] * 600
+            for p in used:
+                remap[p] = p if p < n else remap[p]
+            for p, q in zip([p for p in used if p >= n], [q for q in range(1, n) if q not in used]):
+                remap[p] = q
+            alloc.remap(remap)
+            for s in live:
+                s.pages = [remap[p] for p in s.pages]
+        act = [s for s in live if r.random() < 0.9]
+        got = serving.Engine._prefix_groups(eng, act, min_bytes=0)
+        assert got == serving.Engine._prefix_groups(SimpleNamespace(**{**vars(eng), "_prefixes": {}}), act, min_bytes=0)
+        for slots, keys in got:
+            by = {s.slot: s for s in act}
+            assert all(by[x].pages[:keys // ps] == by[slots[0]].pages[:keys // ps] and keys <= by[x].kv_len for x in slots)
+
+
+def test_groups_are_worked_out_once_for_a_set_of_sessions(monkeypatch):
+    looks, real = [], serving._shared_prefixes
+    monkeypatch.setattr(serving, "_shared_prefixes", lambda paths: looks.append(len(paths)) or real(paths))
+    sessions = [_session(i, list(range(1, 41)) + [100 + i], 645) for i in range(4)]
+    groups = _engine_of(sessions)
+    for step in range(20):
+        assert groups(min_bytes=0) == [([0, 1, 2, 3], 640)]
+        for s in sessions:
+            s.kv_len += 1
+            if s.kv_len > 16 * len(s.pages):
+                s.pages.append(200 + 4 * step + s.sid)
+    sessions.append(_session(4, sessions[0].pages[:41] + [900], 660))
+    assert groups(min_bytes=0) == [([0, 1, 2, 3, 4], 640)]
+    del sessions[1]
+    assert groups(min_bytes=0) == [([0, 2, 3, 4], 640)] and looks == [4, 5, 4]
