@@ -227,7 +227,7 @@ int64_t attn_shared(const at::Tensor& q, const at::Tensor& kcache, const at::Ten
   a.page_size = (int)ps;
   a.n_prefix = (int)(c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None ? n_items : item_cap);
   a.own_at = own_at;
-  a.window = (int)window;
+  a.window = (int)std::min<int64_t>(window, 1 << 30);  // positions are subtracted from it in 32 bits
   a.slot_cap = po.numel() / D;
   a.num_sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   a.pool_pages = kcache.size(0);

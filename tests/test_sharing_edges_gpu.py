@@ -9,7 +9,7 @@ import torch
 from mesh_b200 import ops
 from mesh_b200.engine.serving import _verify_thresholds
 from test_fork_verify_gpu import _engine, _prompt, _start
-from test_sharing_gpu import _attn_64, _check_attn, _i32, _shared_case, _verify_plain
+from test_sharing_gpu import _attn_64, _check_attn, _i32, _run_shared, _shared_case, _verify_plain
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -220,3 +220,13 @@ def test_what_nobody_attends_may_hold_anything(hq, hkv, D, T, window, prefix):
     out = torch.full_like(q, math.nan)
     ops.attn_shared_prefix(q, kc, vc, table, lens, plan, out, 1.0 / math.sqrt(D), window=window)
     _check_attn(out, want, mag)
+
+
+@pytest.mark.parametrize("window", [2 ** 30, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, 2 ** 40])
+def test_a_window_beyond_every_key_is_none(window):
+    groups = [([1, 2], 100)]
+    case = _shared_case(5, 8, 8, 2, 64, 16, groups, [5, 8, 30, 40, 0], seed=81)
+    plain, _ = _run_shared(case, 8, 8, 2, 64, groups)
+    out, _ = _run_shared(case, 8, 8, 2, 64, groups, window=window)
+    assert torch.equal(out, plain)
+    _check_attn(out, *_attn_64(*case, 8, 1.0 / math.sqrt(64)))
