@@ -348,19 +348,20 @@ def kv_pages_copy(k_pool: torch.Tensor, v_pool: torch.Tensor, src, dst, tokens=N
     be a source or another pair's destination (recorded as an error, the pages' contents are then undefined)."""
     if not isinstance(src, torch.Tensor):
         src, dst = [int(p) for p in src], [int(p) for p in dst]
+        tokens = None if tokens is None else [int(t) for t in tokens]
         if len(src) != len(dst) or (tokens is not None and len(tokens) != len(src)):
             raise ValueError(f"{len(src)} source pages, {len(dst)} destinations")
         _check_pages(src + dst, k_pool.shape[1])
         if len(set(dst)) != len(dst) or set(dst) & set(src):
             raise ValueError("a destination page is also a source or another pair's destination")
-        if tokens is not None and any(not 0 <= int(t) <= k_pool.shape[3] for t in tokens):
+        if tokens is not None and any(not 0 <= t <= k_pool.shape[3] for t in tokens):
             raise ValueError(f"token counts outside a page of {k_pool.shape[3]}")
         if not src:
             return
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("lists of pages come from host memory: give device tensors inside a capture")
         n = len(src)
-        idx = torch.tensor(src + dst + [int(t) for t in tokens or ()], dtype=torch.int32)
+        idx = torch.tensor(src + dst + (tokens or []), dtype=torch.int32)
         idx = idx.pin_memory().to(k_pool.device, non_blocking=True)
         src, dst, tokens = idx[:n], idx[n:2 * n], idx[2 * n:] if tokens is not None else None
     ext().kv_pages_move(k_pool, v_pool, src, dst, tokens, scratch(k_pool.device).err)

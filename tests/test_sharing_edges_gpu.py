@@ -3,13 +3,14 @@ that are refused, probabilities that do not fit their drafts, and NaN in queries
 or in pages that nobody attends."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
 from mesh_b200 import ops
 from mesh_b200.engine.serving import _verify_thresholds
 from test_fork_verify_gpu import _engine, _prompt, _start
-from test_sharing_gpu import _attn_64, _check_attn, _i32, _run_shared, _shared_case, _verify_plain
+from test_sharing_gpu import _attn_64, _check_attn, _gen, _i32, _run_shared, _shared_case, _verify_plain
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -230,3 +231,16 @@ def test_a_window_beyond_every_key_is_none(window):
     out, _ = _run_shared(case, 8, 8, 2, 64, groups, window=window)
     assert torch.equal(out, plain)
     _check_attn(out, *_attn_64(*case, 8, 1.0 / math.sqrt(64)))
+
+
+@pytest.mark.parametrize("kind", [list, tuple, np.array, torch.tensor])
+def test_page_lists_of_any_kind(kind):
+    """Counts beside a list of pages may be an array or a tensor, with zeros among them."""
+    pool = torch.randn(2, 9, 2, 16, 64, device=DEV, generator=_gen(91)).to(torch.bfloat16)
+    k, v = pool.clone(), -pool
+    for src, dst, tokens in (([1, 1, 2], [3, 4, 5], [0, 7, 16]), ([1], [6], [0]), ([8], [7], [1])):
+        want = k.clone()
+        for a, b, t in zip(src, dst, tokens):
+            want[:, b, :, :t] = k[:, a, :, :t]
+        ops.kv_pages_copy(k, v, src, dst, kind(tokens))
+        assert torch.equal(k, want) and torch.equal(v, -want)
