@@ -203,9 +203,14 @@ class DecodeGraphs:
 
 
 # Decode steps read shared prefixes once (attn_shared_prefix) from this many K/V bytes a layer that attn_decode would read
-# again. Measured with 8 KV heads: 2 sessions behind 4096 keys (17 MB) 13.8 us against 11.3, 4 behind 4096 (50 MB) 14.4 against
-# 15.9, 16 behind 4096 (252 MB) 18.5 against 66.2; 64 behind 256 (66 MB, mostly found in L2) 18.2 against 15.5.
-SHARED_PREFIX_MIN_BYTES = 64 << 20
+# again. Measured in captured graphs, us of attn_decode against attn_shared_prefix, 100 keys of its own for every session:
+# 8 KV heads of 128: 2 sessions behind 4096 keys (17 MB) 11.3 and 13.0, 8 behind 1024 (29 MB) 10.9 and 13.6, 2 behind 8192 (34 MB)
+# 16.7 and 16.0, 4 behind 4096 (50 MB) 15.8 and 14.0, 8 behind 2048 (59 MB) 16.5 and 14.0, 16 behind 4096 (252 MB) 66.7 and 16.7;
+# what L2 serves again costs less: 32 behind 512 (65 MB) 12.9 and 13.9, 64 behind 256 (66 MB) 17.9 and 17.6.
+# 1 KV head of 128: 64 behind 1024 (33 MB) 12.3 and 15.7, 64 behind 4096 (132 MB) 28.4 and 24.0.
+# head_dim 64, whose attn_decode keeps the weights in fp32 on CUDA cores, would gain from 4 MB on (4 KV heads, 2 behind 4096: 39.3
+# and 12.0); it has the same threshold, so that few forks do not move a session to weights rounded to bf16.
+SHARED_PREFIX_MIN_BYTES = 40 << 20
 # Rejection sampling needs its uniforms to be independent of the drafts, and a draft model served by an engine like this one
 # may have drawn them with the session's own seed: the thresholds that accept drafts, and the one that draws the token after
 # them, are apart from decode_step's and prefill's at every position, and from one another (they differ above any position).

@@ -210,3 +210,11 @@ def test_groups_are_worked_out_once_for_a_set_of_sessions(monkeypatch):
     assert groups(min_bytes=0) == [([0, 1, 2, 3, 4], 640)]
     del sessions[1]
     assert groups(min_bytes=0) == [([0, 2, 3, 4], 640)] and looks == [4, 5, 4]
+
+
+def test_prefixes_are_shared_where_that_is_faster():
+    """The measured sides of the threshold, 8 KV heads of 128."""
+    for n, keys, shared in ((2, 4096, False), (8, 1024, False), (4, 4096, True), (8, 2048, True), (16, 4096, True)):
+        pages = list(range(1, keys // 16 + 1))
+        sessions = [_session(i, pages + [9000 + i], keys + 7) for i in range(n)]
+        assert bool(_engine_of(sessions)()) == shared, (n, keys)
