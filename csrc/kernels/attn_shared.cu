@@ -12,9 +12,10 @@
 // are summed in a fixed order, so results do not depend on the schedule. NaN in a row's query or in a key it attends makes
 // the row NaN however its keys are cut: its sums l are NaN, and only a sum of exactly 0 counts as nothing seen.
 //
-// Measured (32 query and 8 KV heads of 128): 64 sessions with up to 512 keys of their own behind 8192 shared ones 36.9 us, of
-// which reading every key once takes 15.8 at the copy rate; 128 with up to 1024 behind 16384 92 us (52.5); 4 forks of 512
-// keys 10.7 us in a captured graph. About 19 us of the large calls go by before and after the keys: first queries and pages (5), partials
+// Measured (32 query and 8 KV heads of 128): 64 sessions with up to 512 keys of their own behind 8192 shared ones 36.5 us, of
+// which reading every key once takes 15.8 at the copy rate; 128 with up to 1024 behind 16384 94 us (52.5); 4 forks of 512
+// keys 10.9 us in a captured graph. About 19 us of the large calls do not depend on the shared keys (64 sessions with one key of their
+// own, captured: 20.0 us with 64 shared keys for every SM, 27.5 with 512, 53.4 with 2048): first queries and pages (5), partials
 // written (3: 256 rows x 128 fp32 from every SM) and merged (5), and three kernels following one another.
 //
 // The item list is made on the host when the groups change (PrefixGroups) and lives in device memory, so a
@@ -322,7 +323,8 @@ __device__ __forceinline__ void own_worker(const CUtensorMap& tmK, const CUtenso
             o[x][2 + i] *= corr;
           }
         }
-        // the weights are rounded to bf16 for the product (half a step of 2^-8 each); their sum keeps fp32
+        // The weights are rounded to bf16 for the product (half a step of 2^-8 each), whose operands are of one type; their
+        // sum keeps fp32.
         pf[0] = transposed(pack_bf16x2(sc[0], sc[1]));
         pf[1] = transposed(pack_bf16x2(sc[2], sc[3]));
 #pragma unroll
@@ -384,7 +386,7 @@ __device__ __forceinline__ void own_worker(const CUtensorMap& tmK, const CUtenso
   }
 }
 
-// 128 registers a thread, so that a CTA fits beside one of the prefix kernel.
+// 128 registers a thread, so that a CTA fits beside one of the prefix kernel; nothing is spilled.
 template <int D>
 __global__ void __launch_bounds__(WARPS * 32, 4) own_kernel(const __grid_constant__ CUtensorMap tmK,
                                                             const __grid_constant__ CUtensorMap tmV, const Args a) {

@@ -18,9 +18,9 @@
 // Two launches:
 //   stats    grid (chunk, row): one CTA reads one chunk of a row once, keeps it in registers, and writes its
 //            maximum (first index) and its mass relative to that maximum. Rows past a session's drafts are
-//            not read. Bound by the 64-bit exponentials: 64 sessions of 5 rows over 128256 tokens (164 MB of fp32) take
-//            56 us; with greedy sessions, which need none, the whole call takes 28, 5.9 TB/s. More or fewer warps on an
-//            SM, and warps that load ahead of their exponentials, cost more.
+//            not read. The 64-bit exponentials cost most: 64 sessions of 5 rows over 128256 tokens (164 MB of fp32) take
+//            57 us (fp64 pipe 43 %, issue 64 %, DRAM 35 %); with greedy sessions, which need none, the whole call takes 29,
+//            5.6 TB/s. More or fewer warps on an SM, and warps that load ahead of their exponentials, cost more.
 //   resolve  one cluster of 8 CTAs per session: joins the chunks of the session's rows and decides. Drawing from p (or
 //            p without one token) the chunks' masses are known and one CTA goes on: it picks the chunk, the
 //            256-token unit in it, and the token. For max(p - q, 0) every CTA first sums the units of its eighth of the
@@ -39,14 +39,16 @@ constexpr int SNT = 256;                // threads of a stats CTA
 constexpr int RNT = 256;                // threads of a resolve CTA
 constexpr int CLUSTER = 8;
 constexpr int MAX_DRAFTS = VERIFY_MAX_DRAFTS;
-constexpr int STEP = 4;                 // exponentials of a thread side by side (64 registers keep four CTAs on an SM)
+// Exponentials of a thread side by side. 64 registers keep four CTAs on an SM; under them stats_kernel with 32 logits spills
+// 32 to 56 bytes and resolve_kernel 24 to 124.
+constexpr int STEP = 4;
 constexpr int PER_LANE = 8;            // tokens of a unit per lane
 constexpr int UNIT = 32 * PER_LANE;     // tokens whose sum one warp of the resolve kernel makes
 constexpr int MAX_SUMS = 4096;          // chunks of a row, units of a CTA's share
-// Logits per stats thread, by the CTAs that 32 each would make: 8 below two per SM (one session of 5 rows over 128256
-// tokens then makes 315 CTAs instead of 80), 16 below sixteen per SM (33 sessions of 1-8 rows over 32000 tokens: 19.8 us,
-// with 32 each 25.9), else 32, which spreads a CTA's fixed work over more logits (64 sessions of 5 rows over 128256:
-// 77 us, with 16 each 86; both pairs before the exponentials ran side by side).
+// Logits per stats thread, by the CTAs that 32 each would make: 8 below two per SM, 16 below sixteen per SM, else 32, which
+// spreads a CTA's fixed work over more logits. Whole calls in captured graphs, us with 8, 16 and 32 each (rows x tokens):
+// 8 sessions of 5 x 4096 8.8, 9.2, 10.4; one of 5 x 128256 14.5, 14.2, 15.4; 33 of 8 x 32000 (bf16) 29.1, 26.7, 32.0;
+// 64 of 5 x 32000 35.2, 28.9, 29.9; 16 of 5 x 128256 44.7, 37.3, 36.9; 64 of 5 x 128256 110, 82, 75.4, greedy 56, 34, 29.2.
 constexpr int EPT_MANY = 32, EPT_SOME = 16, EPT_FEW = 8;
 inline int logits_per_thread(int64_t rows, int64_t V) {
   const int64_t ctas = rows * ((V + SNT * EPT_MANY - 1) / (SNT * EPT_MANY));

@@ -762,10 +762,11 @@ class Engine:
         """One step in which sessions advance by several tokens: the target model scores each session's drafted tokens
         in one pass, keeps those that its own distribution allows and adds one of its own. ``drafts``: session id ->
         proposed next tokens (possibly none); ``probs``: session id -> [drafts, vocabulary] probabilities they were
-        drawn from, a row for each (sessions without: guesses). Greedy sessions then generate exactly what ``decode_step`` would, sampled
-        ones (temperature with top_p 1) what it would in distribution. Drafts may come from an engine whose sessions have the
-        same seeds and decode or prefill them; one that verifies drafts of its own needs other seeds. Returns the new tokens
-        per session, which are appended to it."""
+        drawn from, a row for each (sessions without: guesses). Greedy sessions then generate what ``decode_step`` would, up
+        to near ties (other kernels and row counts round their logits differently), sampled ones (temperature with top_p
+        1) what it would in distribution. Drafts may come from an engine whose sessions have the same seeds and decode
+        or prefill them; one that verifies drafts of its own needs other seeds. Returns the new tokens per session,
+        which are appended to it."""
         from .. import ops
         r, ps = self.runner, self.page_size
         if r.world > 1:

@@ -131,8 +131,9 @@ def attn_shared_prefix(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tens
     ``groups`` read once per group. q, out [B * q_len, hq * D] bf16 (the tokens of a sequence together);
     kcache, vcache [pages, hkv, page, D] bf16 (pages of a multiple of 16 tokens); block_tables [B, pages] and
     seq_lens [B] int32 as in ``attn_decode``, lengths including the new tokens. A token without any key gives
-    zeros. ``window``: attend the last ``window`` keys only. ``scale`` must be positive: the largest score is looked for
-    before it is applied."""
+    zeros, one that meets NaN gives NaN. ``window``: attend the last ``window`` keys only. ``scale`` must be
+    positive: the largest score is looked for before it is applied. Softmax sums and outputs are held in fp32, the
+    weights are rounded to bf16 for the product."""
     from . import _count, ext
     if not 1e-30 <= scale <= 1e30:
         raise ValueError(f"a scale of {scale}: must be positive and finite")
