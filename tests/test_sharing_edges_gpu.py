@@ -9,7 +9,7 @@ import torch
 
 from mesh_b200 import ops
 from mesh_b200.engine.serving import _verify_thresholds
-from test_fork_verify_gpu import _engine, _prompt, _start
+from test_fork_verify_gpu import _check_greedy, _engine, _prompt, _start
 from test_sharing_gpu import _attn_64, _check_attn, _gen, _i32, _run_shared, _shared_case, _verify_plain
 
 pytestmark = pytest.mark.gpu
@@ -244,3 +244,34 @@ def test_page_lists_of_any_kind(kind):
             want[:, b, :, :t] = k[:, a, :, :t]
         ops.kv_pages_copy(k, v, src, dst, kind(tokens))
         assert torch.equal(k, want) and torch.equal(v, -want)
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+def test_two_families_and_an_early_branch_decode_together(graphs, monkeypatch):
+    """Sessions of two prompts, forked at several lengths: groups of different prefixes in one step, which change as branches fork
+    and finish. Every token is the greedy one after those before it."""
+    from mesh_b200.engine import serving
+    monkeypatch.setattr(serving, "SHARED_PREFIX_MIN_BYTES", 0)
+    eng, cfg = _engine(pages=120, max_batch=16, graphs=graphs)
+    ref, _ = _engine(pages=200, graphs=False, max_tokens=2048)
+    prompts = [_prompt(cfg, 20, seed=1), _prompt(cfg, 70, seed=2), _prompt(cfg, 33, seed=3)]
+    a, b, alone = _start(eng, prompts, 60)
+    early = eng.fork_session(a, 1)                    # one page in common with what follows
+    for _ in range(30):
+        eng.decode_step()
+    kids = eng.fork_session(a, 3) + eng.fork_session(b, 2)
+    eng.decode_step()
+    groups = sorted((len(s), n) for s, n in eng._prefix_groups([s for s in eng.running if s]))
+    assert groups == [(3, 96), (4, 48)]
+    eng.sessions[kids[0]].max_new_tokens = 36         # one leaves while the others go on
+    for _ in range(8):
+        eng.decode_step()
+    more = eng.fork_session(kids[3], 1)
+    eng.compact()
+    eng.run()
+    done = {a: 0, b: 1, alone: 2, early[0]: 0, **{k: 0 for k in kids[:3]}, **{k: 1 for k in kids[3:] + more}}
+    assert all(len(eng.sessions[s].generated) == (36 if s == kids[0] else 60) for s in done)
+    _check_greedy(ref, [(prompts[i], eng.sessions[s].generated) for s, i in done.items()])
+    assert eng.alloc.num_used == 0
+    eng.close()
+    ref.close()
